@@ -111,6 +111,40 @@ class MBOptimConfig(C.Structure):
     _fields_ = [(k, C.c_float) for k in ("lr", "mu", "beta2", "eps", "clip_norm", "weight_decay")]
 
 
+DTYPE_F32, DTYPE_BF16 = 0, 1
+
+
+class KMBDeltaParams(C.Structure):
+    """include/kmamba_delta.h"""
+    _fields_ = [("batch", C.c_long), ("T", C.c_long), ("Hk", C.c_long), ("Hv", C.c_long), ("dk", C.c_long),
+                ("dv", C.c_long), ("dtype", C.c_int), ("scale", C.c_float), ("cu_seqlens", C.c_void_p),
+                ("n_seq", C.c_long), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p),
+                ("beta", C.c_void_p), ("o", C.c_void_p), ("h0", C.c_void_p), ("hT", C.c_void_p),
+                ("ld_q", C.c_long), ("ld_k", C.c_long), ("ld_v", C.c_long), ("ld_o", C.c_long)]
+
+
+class KMBDeltaGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("do_", "dhT", "dq", "dk", "dv", "dg", "dbeta", "dh0")] + \
+               [(n, C.c_long) for n in ("ld_do", "ld_dq", "ld_dk", "ld_dv")]
+
+
+class KMBNormParams(C.Structure):
+    """include/kmamba_norm.h"""
+    _fields_ = [("rows", C.c_long), ("D", C.c_long), ("dtype", C.c_int), ("eps", C.c_float)] + \
+               [(n, C.c_void_p) for n in ("x", "residual", "total", "y", "w", "b", "mean", "rstd")] + \
+               [(n, C.c_long) for n in ("ld_x", "ld_residual", "ld_total", "ld_y")]
+
+
+class KMBNormGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "dtotal", "dx", "dw", "db")] + \
+               [(n, C.c_long) for n in ("ld_dy", "ld_dtotal", "ld_dx")] + [("accumulate", C.c_int)]
+
+
+class KMBGradTensor(C.Structure):
+    """include/kmamba_clip.h"""
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("n", C.c_longlong), ("dtype", C.c_int)]
+
+
 CONVND_FORWARD, CONVND_BACKWARD, CONVND_COMPLETE = 1, 2, 3
 
 # every symbol the public headers declare (checked by the CPU tests)
@@ -145,6 +179,9 @@ EXPORTS = [
     "kmamba_init", "kmamba_enable_training", "kmamba_forward", "kmamba_train_batch", "kmamba_train_step",
     "kmamba_get_config", "kmamba_step_count", "kmamba_update_lr", "kmamba_get_tensor", "kmamba_set_tensor",
     "kmb_model_forward_backward", "kmb_model_optimizer_step", "kmb_model_grad_arena", "kmb_model_param_arena", "kmb_model_tensor_offset",
+    "kmb_delta_workspace_floats", "kmb_delta_forward", "kmb_delta_backward", "kmb_delta_step",
+    "kmb_layernorm_forward", "kmb_layernorm_workspace_floats", "kmb_layernorm_backward",
+    "kmb_grad_clip_workspace_floats", "kmb_grad_clip", "kmb_model_clip_gradients",
     "kmb_gemm_f32", "kmb_gemm_bf16", "kmb_gemm_set_f32_kind", "kmb_gemm_get_f32_kind", "kmb_gemm_set_f32_flush", "kmb_gemm_last_path",
 ]
 
@@ -306,6 +343,20 @@ def lib():
         L.wavefront_nd_total_points.restype = C.c_long
         L.wavefront_nd_max_level.argtypes = [_l, C.c_long]
         L.wavefront_nd_max_level.restype = C.c_long
+        DP, NP = C.POINTER(KMBDeltaParams), C.POINTER(KMBNormParams)
+        L.kmb_delta_workspace_floats.argtypes = [DP, C.c_int]
+        L.kmb_delta_workspace_floats.restype = sz
+        L.kmb_delta_forward.argtypes = [DP, vp, C.c_int, vp]
+        L.kmb_delta_backward.argtypes = [DP, C.POINTER(KMBDeltaGrads), vp, vp]
+        L.kmb_delta_step.argtypes = [DP, vp, C.c_long, vp, vp]
+        L.kmb_layernorm_forward.argtypes = [NP, vp]
+        L.kmb_layernorm_workspace_floats.argtypes = [NP]
+        L.kmb_layernorm_workspace_floats.restype = sz
+        L.kmb_layernorm_backward.argtypes = [NP, C.POINTER(KMBNormGrads), vp, vp]
+        L.kmb_grad_clip_workspace_floats.argtypes = [C.c_long]
+        L.kmb_grad_clip_workspace_floats.restype = sz
+        L.kmb_grad_clip.argtypes = [vp, C.c_long, C.c_float, vp, vp, vp]
+        L.kmb_model_clip_gradients.argtypes = [vp, C.c_float, vp, vp, vp]
         _lib = L
     return _lib
 
@@ -403,6 +454,190 @@ def model_config(dims, vocab, dim, N, R, n_layers):
     for i, d in enumerate(dims):
         c.spatial_dims[i] = int(d)
     return c
+
+
+def _dtype_of(t):
+    """KMB_DTYPE_* of a tensor (float32 or bfloat16)."""
+    name = str(t.dtype)
+    if name.endswith("bfloat16"):
+        return DTYPE_BF16
+    if name.endswith("float32"):
+        return DTYPE_F32
+    raise TypeError(f"float32 or bfloat16 expected, got {name}")
+
+
+def _rows_ld(t, inner, what):
+    """Elements between two tokens (or rows) of t, whose last `inner` axes must be contiguous and whose leading axes
+    must be walked by one stride."""
+    st, sh = t.stride(), t.shape
+    want = 1
+    for i in range(1, inner + 1):
+        if sh[-i] != 1 and st[-i] != want:
+            raise ValueError(f"{what}: the last {inner} axes must be contiguous")
+        want *= sh[-i]
+    lead = [(n, s) for n, s in zip(sh[:-inner], st[:-inner]) if n != 1]
+    if not lead:
+        return want
+    for (n, s), (n1, s1) in zip(lead, lead[1:]):
+        if s != n1 * s1:
+            raise ValueError(f"{what}: rows must follow each other at one stride")
+    if lead[-1][1] < want:
+        raise ValueError(f"{what}: rows overlap")
+    return lead[-1][1]
+
+
+def _f32(t, what, shape=None):
+    if t is None:
+        return
+    if _dtype_of(t) != DTYPE_F32 or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous float32 tensor is expected")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(shape)} expected, got {tuple(t.shape)}")
+
+
+def _typed(t, like, shape, what):
+    if t is None:
+        return
+    if t.dtype != like.dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {like.dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
+
+
+def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=None):
+    """KMBDeltaParams of device tensors: q, k [batch, T, Hk, dk], v, o [batch, T, Hv, dv] (slices of a wider token row
+    are fine), g, beta [batch, T, Hv] or None, states [sequences, Hv, dk, dv] or None, cu_seqlens int32
+    [sequences + 1] with batch 1.  The struct holds pointers: keep the tensors alive while it is used."""
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2], v.shape[3]
+    _typed(k, q, q.shape, "k")
+    _typed(v, q, (B, T, Hv, dv), "v")
+    _typed(o, q, v.shape, "o")
+    for t, n in ((g, "g"), (beta, "beta")):
+        _f32(t, n, (B, T, Hv))
+    if cu_seqlens is not None and (not str(cu_seqlens.dtype).endswith("int32") or not cu_seqlens.is_contiguous()):
+        raise ValueError("cu_seqlens: a contiguous int32 tensor is expected")
+    n = B if cu_seqlens is None else cu_seqlens.numel() - 1
+    for t, name in ((h0, "h0"), (hT, "hT")):
+        _f32(t, name, (n, Hv, dk, dv))
+    p = KMBDeltaParams()
+    p.batch, p.T, p.Hk, p.Hv, p.dk, p.dv = B, T, Hk, Hv, dk, dv
+    p.dtype, p.scale = _dtype_of(q), float(scale)
+    p.cu_seqlens, p.n_seq = _ptr(cu_seqlens), n if cu_seqlens is not None else 0
+    p.q, p.k, p.v, p.g, p.beta, p.o = _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(o)
+    p.h0, p.hT = _ptr(h0), _ptr(hT)
+    p.ld_q, p.ld_k, p.ld_v, p.ld_o = (_rows_ld(t, 2, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
+    p._keep = (q, k, v, g, beta, o, h0, hT, cu_seqlens)
+    return p
+
+
+def delta_workspace_floats(p, train=False):
+    return lib().kmb_delta_workspace_floats(C.byref(p), int(bool(train)))
+
+
+def delta_grads(p, do, dq, dk, dv, dg=None, dbeta=None, dh0=None, dhT=None):
+    """KMBDeltaGrads for a KMBDeltaParams of delta_params."""
+    q, k, v = p._keep[:3]
+    for t, like, n in ((do, v, "do"), (dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+        _typed(t, q, like.shape, n)
+    for t, n in ((dg, "dg"), (dbeta, "dbeta")):
+        _f32(t, n, v.shape[:3])
+    seqs = p.n_seq if p.cu_seqlens else p.batch
+    for t, n in ((dh0, "dh0"), (dhT, "dhT")):
+        _f32(t, n, (seqs, p.Hv, p.dk, p.dv))
+    g = KMBDeltaGrads()
+    g.do_, g.dhT, g.dq, g.dk, g.dv = _ptr(do), _ptr(dhT), _ptr(dq), _ptr(dk), _ptr(dv)
+    g.dg, g.dbeta, g.dh0 = _ptr(dg), _ptr(dbeta), _ptr(dh0)
+    g.ld_do, g.ld_dq, g.ld_dk, g.ld_dv = (_rows_ld(t, 2, n) for t, n in
+                                          ((do, "do"), (dq, "dq"), (dk, "dk"), (dv, "dv")))
+    g._keep = (do, dq, dk, dv, dg, dbeta, dh0, dhT)
+    return g
+
+
+def delta_forward(p, ws, keep=False, stream=None):
+    """Chunked gated delta rule; keep=True leaves in ws (a training workspace) what delta_backward reads."""
+    check(lib().kmb_delta_forward(C.byref(p), ws.data_ptr(), int(bool(keep)), stream), "kmb_delta_forward")
+
+
+def delta_backward(p, grads, ws, stream=None):
+    check(lib().kmb_delta_backward(C.byref(p), C.byref(grads), ws.data_ptr(), stream), "kmb_delta_backward")
+
+
+def delta_step(p, pool, slots=None, stream=None):
+    """Recurrent form: the T tokens of each row against its state in pool [entries, Hv, dk, dv], updated in place."""
+    if pool.shape[1:] != (p.Hv, p.dk, p.dv) or not pool.is_contiguous():
+        raise ValueError("pool: a contiguous [entries, Hv, dk, dv] tensor is expected")
+    check(lib().kmb_delta_step(C.byref(p), pool.data_ptr(), pool.shape[0], _ptr(slots), stream), "kmb_delta_step")
+
+
+def norm_params(x, w, b, y, eps=1e-5, residual=None, total=None, stats=None):
+    """KMBNormParams of device tensors: x, residual, total, y [..., D]; w, b float32 [D] or None; stats float32
+    [2, rows] (mean, rstd) or None."""
+    D = x.shape[-1]
+    rows = x.numel() // D if D else 0
+    for t, n in ((y, "y"), (residual, "residual"), (total, "total")):
+        _typed(t, x, x.shape, n)
+    for t, n in ((w, "w"), (b, "b")):
+        _f32(t, n, (D,))
+    _f32(stats, "stats", (2, rows))
+    p = KMBNormParams()
+    p.rows, p.D, p.dtype, p.eps = rows, D, _dtype_of(x), float(eps)
+    p.x, p.residual, p.total, p.y, p.w, p.b = _ptr(x), _ptr(residual), _ptr(total), _ptr(y), _ptr(w), _ptr(b)
+    if stats is not None:
+        p.mean, p.rstd = stats.data_ptr(), stats.data_ptr() + 4 * rows
+    p.ld_x, p.ld_residual, p.ld_total, p.ld_y = (0 if t is None else _rows_ld(t, 1, n) for t, n in
+                                                 ((x, "x"), (residual, "residual"), (total, "total"), (y, "y")))
+    p._keep = (x, w, b, y, residual, total, stats)
+    return p
+
+
+def norm_grads(p, dy, dx=None, dw=None, db=None, dtotal=None, accumulate=False):
+    """KMBNormGrads for a KMBNormParams of norm_params."""
+    x = p._keep[0]
+    for t, n in ((dy, "dy"), (dx, "dx"), (dtotal, "dtotal")):
+        _typed(t, x, x.shape, n)
+    for t, n in ((dw, "dw"), (db, "db")):
+        _f32(t, n, (p.D,))
+    g = KMBNormGrads()
+    g.dy, g.dtotal, g.dx, g.dw, g.db = _ptr(dy), _ptr(dtotal), _ptr(dx), _ptr(dw), _ptr(db)
+    g.ld_dy, g.ld_dtotal, g.ld_dx = (0 if t is None else _rows_ld(t, 1, n) for t, n in
+                                     ((dy, "dy"), (dtotal, "dtotal"), (dx, "dx")))
+    g.accumulate = int(bool(accumulate))
+    g._keep = (dy, dx, dw, db, dtotal)
+    return g
+
+
+def norm_workspace_floats(p):
+    return lib().kmb_layernorm_workspace_floats(C.byref(p))
+
+
+def norm_forward(p, stream=None):
+    check(lib().kmb_layernorm_forward(C.byref(p), stream), "kmb_layernorm_forward")
+
+
+def norm_backward(p, grads, ws=None, stream=None):
+    check(lib().kmb_layernorm_backward(C.byref(p), C.byref(grads), _ptr(ws), stream), "kmb_layernorm_backward")
+
+
+def grad_list(grads, outs=None):
+    """KMBGradTensor array of contiguous gradient tensors; outs: where the clipped ones go (default: in place)."""
+    outs = grads if outs is None else outs
+    arr = (KMBGradTensor * len(grads))()
+    for e, t, o in zip(arr, grads, outs):
+        if not t.is_contiguous():
+            raise ValueError("grad_list: contiguous tensors are expected")
+        if o is not None and (o.dtype != t.dtype or o.numel() != t.numel() or not o.is_contiguous()):
+            raise ValueError("grad_list: an output does not match its gradient")
+        e.in_, e.out, e.n, e.dtype = t.data_ptr(), _ptr(o), t.numel(), _dtype_of(t)
+    arr._keep = (list(grads), list(outs))
+    return arr
+
+
+def grad_clip_workspace_floats(lst):
+    return lib().kmb_grad_clip_workspace_floats(len(lst))
+
+
+def grad_clip(lst, max_norm, result, ws, stream=None):
+    """Global norm of a grad_list and clipping by it; result: float32 [2], norm and coefficient."""
+    check(lib().kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream), "kmb_grad_clip")
 
 
 class DeviceArray:

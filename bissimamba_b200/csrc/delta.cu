@@ -1,0 +1,605 @@
+// delta.cu -- gated delta rule (include/kmamba_delta.h): entry points, the
+// per-chunk matrices that need no state, and the recurrent form.
+#include <cmath>
+#include <cstring>
+#include "kmb_delta.cuh"
+#include "../../include/kmamba_delta.h"
+
+namespace kmb {
+int set_error(const char* msg);
+int set_cuda_error(const char* where, cudaError_t e);
+void clear_error();
+
+namespace {
+
+// ------------------------------------------------------------------ packed sequences
+// One block: offsets clamped to [0, total] and made non-decreasing (cu), and the first chunk of each sequence
+// (cstart).  Whatever the caller's offsets hold, the kernels stay inside the tensors.
+__global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ in, int nseq, int total, int C,
+                                                       int* __restrict__ cu, int* __restrict__ cstart) {
+    __shared__ int sh[256];
+    const int t = threadIdx.x;
+    const int per = (nseq + 1 + 255) / 256;
+    const int a = min(t * per, nseq + 1), b = min(a + per, nseq + 1);
+    int mx = 0;
+    for (int i = a; i < b; i++) mx = max(mx, min(max(in[i], 0), total));
+    sh[t] = mx;
+    __syncthreads();
+    for (int o = 1; o < 256; o <<= 1) {
+        const int v = t >= o ? sh[t - o] : 0;
+        __syncthreads();
+        sh[t] = max(sh[t], v);
+        __syncthreads();
+    }
+    int run = t ? sh[t - 1] : 0;
+    __syncthreads();
+    for (int i = a; i < b; i++) {
+        run = max(run, min(max(in[i], 0), total));
+        cu[i] = run;
+    }
+    __threadfence_block();
+    __syncthreads();
+    int n = 0;   // chunks of sequences a .. b - 1
+    for (int i = a; i < b && i < nseq; i++) n += (cu[i + 1] - cu[i] + C - 1) / C;
+    sh[t] = n;
+    __syncthreads();
+    for (int o = 1; o < 256; o <<= 1) {
+        const int v = t >= o ? sh[t - o] : 0;
+        __syncthreads();
+        sh[t] += v;
+        __syncthreads();
+    }
+    n = t ? sh[t - 1] : 0;
+    for (int i = a; i < b; i++) {
+        cstart[i] = n;
+        if (i < nseq) n += (cu[i + 1] - cu[i] + C - 1) / C;
+    }
+}
+
+// ------------------------------------------------------------------ per-chunk matrices
+// Block = (chunk, key head), four warps of 16 rows: the chunk's K and Q as swizzled fp16 tiles (zero behind the
+// last token and behind dk), K K^T and Q K^T once per key head; then for each of its value heads the token
+// factors, T = (I + A)^-1 and P in two fp16 pieces.  T comes from 16 x 16 diagonal blocks by forward
+// substitution, one column per lane, merged in pairs: [[a, 0], [c, b]]^-1 = [[a^-1, 0], [-b^-1 c a^-1, b^-1]].
+// The running sums of g are 64-bit: their differences are what G needs, after a reset (g = -inf, held at -104,
+// where exp is 0 in fp32) too.  beta = 0 is replaced by 2^-100 with a factor 0 beside it, so that u / beta exists.
+constexpr float kBetaTiny = 7.888609052210118e-31f;
+
+template <int DKP, typename IO>
+__global__ void __launch_bounds__(128)
+delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
+    constexpr int C = kDeltaC;
+    constexpr bool F32 = sizeof(IO) == 4;
+    constexpr int NPK = F32 ? 2 : 1;
+    constexpr int TILE = C * DKP * 2;                     // bytes of one piece
+    constexpr int LDA = C + 1;
+    constexpr int G8 = DKP / 8;                           // threads per row of the tiles
+    extern __shared__ __align__(128) unsigned char sm[];
+    const uint32_t sK = (uint32_t)__cvta_generic_to_shared(sm), sQ = sK + NPK * TILE;
+    float* Am = (float*)(sm + 2 * NPK * TILE);
+    float* X = Am + C * LDA;
+    float* W = X + C * LDA;                               // [C / 2][LDA]
+    __shared__ double gam[C];
+    __shared__ float bet[C], fK[C], fQ[C], red[2][4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunk = blockIdx.x, hk = blockIdx.y;
+    long long tok0;
+    int cnt;
+    if (!chunk_range<C>(d, chunk, tok0, cnt)) return;
+
+    char* gK = (char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+    char* gQ = (char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+    for (int i = threadIdx.x; i < 2 * C * G8; i += 128) {
+        const bool isq = i >= C * G8;
+        const int j = isq ? i - C * G8 : i;
+        const int row = j / G8, c8 = j % G8 * 8;
+        const IO* src = isq ? (const IO*)d.q + (tok0 + row) * d.ld_q + (long long)hk * d.dk
+                            : (const IO*)d.k + (tok0 + row) * d.ld_k + (long long)hk * d.dk;
+        float x[8];
+        if (vec && row < cnt && c8 + 8 <= d.dk) {
+            if constexpr (F32) {
+                const float4 a = *(const float4*)(src + c8), b = *(const float4*)(src + c8 + 4);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
+                const uint4 a = *(const uint4*)(src + c8);
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[2 * e] = __uint_as_float(w[e] << 16);
+                    x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = row < cnt && c8 + e < d.dk ? ldt(src, c8 + e) : 0.0f;
+        }
+        float m = 0.0f, up, down;
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]));
+#pragma unroll
+        for (int o = 1; o < G8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        row_scale(m, up, down);
+        if (c8 == 0) (isq ? fQ : fK)[row] = down;
+        uint32_t w[4][NPK];
+#pragma unroll
+        for (int e = 0; e < 4; e++) split_pair<NPK>(x[2 * e] * up, x[2 * e + 1] * up, w[e]);
+        const uint32_t o = wide_off<C>(row, c8);
+#pragma unroll
+        for (int k = 0; k < NPK; k++) {
+            const uint4 p = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
+            *(uint4*)(sm + (isq ? NPK * TILE : 0) + k * TILE + o) = p;
+            *(uint4*)((isq ? gQ : gK) + k * TILE + o) = p;
+        }
+    }
+    __syncthreads();
+    const int rg = warp;
+    const int r = lane >> 2, c2 = (lane & 3) * 2;
+    float kk[C / 8][4], qk[C / 8][4];
+#pragma unroll
+    for (int t = 0; t < C / 8; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) kk[t][e] = qk[t][e] = 0.0f;
+    for (int s = 0; s < DKP / 16; s++) {
+        uint32_t ak[NPK][4], aq[NPK][4];
+        const uint32_t oa = wide_off<C>(rg * 16 + la_row(lane), s * 16 + la_col(lane));
+#pragma unroll
+        for (int p = 0; p < NPK; p++) {
+            ldm4(ak[p], sK + p * TILE + oa);
+            ldm4(aq[p], sQ + p * TILE + oa);
+        }
+        auto ldb = [&](int p, int t2, uint32_t (&b)[4]) {
+            ldm4(b, sK + p * TILE + wide_off<C>(t2 * 16 + lb_row(lane), s * 16 + lb_col(lane)));
+        };
+        mma_row<NPK, NPK>(kk, ak, 0, C / 16, ldb);
+        mma_row<NPK, NPK>(qk, aq, 0, C / 16, ldb);
+    }
+    for (int hh = 0; hh < d.grp; hh++) {
+        const int hv = hk * d.grp + hh;
+        const size_t head = (size_t)chunk * d.Hv + hv;
+        float* tk = d.tok + head * TOK_ROWS * C;
+        __syncthreads();   // the last head's matrices are read
+        if (warp == 0) {   // running sums: lane holds tokens lane and lane + 32
+            double carry = 0.0;
+#pragma unroll
+            for (int h = 0; h < C / 32; h++) {
+                const int i = h * 32 + lane;
+                float g = (d.g && i < cnt) ? d.g[(tok0 + i) * d.Hv + hv] : 0.0f;
+                if (g < -104.0f) g = -104.0f;
+                double s = g;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double t = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += t;
+                }
+                s += carry;
+                gam[i] = s;
+                carry = __shfl_sync(0xffffffffu, s, 31);
+                float b = i < cnt ? (d.beta ? d.beta[(tok0 + i) * d.Hv + hv] : 1.0f) : 0.0f;
+                const float on = fabsf(b) < kBetaTiny ? 0.0f : 1.0f;
+                if (on == 0.0f) b = kBetaTiny;
+                bet[i] = b;
+                tk[TOK_EG * C + i] = expf((float)s);
+                tk[TOK_BETA * C + i] = b;
+                tk[TOK_ON * C + i] = on;
+                tk[TOK_FK * C + i] = fK[i];
+                tk[TOK_FQ * C + i] = fQ[i];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < C / 32; h++) {
+                const int i = h * 32 + lane;
+                tk[TOK_GC * C + i] = expf((float)(gam[C - 1] - gam[i]));
+            }
+        }
+        for (int i = threadIdx.x; i < C * LDA; i += 128) X[i] = 0.0f;
+        __syncthreads();
+        float pv[C / 8][4], pm = 0.0f;
+#pragma unroll
+        for (int t = 0; t < C / 8; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = rg * 16 + r + (e >> 1) * 8, j = t * 8 + c2 + (e & 1);
+                const float G = j <= i ? expf((float)(gam[i] - gam[j])) * fK[j] : 0.0f;
+                pv[t][e] = j <= i ? G * fQ[i] * qk[t][e] : 0.0f;
+                pm = fmaxf(pm, fabsf(pv[t][e]));
+                Am[i * LDA + j] = j < i ? bet[i] * G * fK[i] * kk[t][e] : 0.0f;
+            }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, o));
+        if (lane == 0) red[0][warp] = pm;
+        __syncthreads();
+        if (lane < 16) {   // column `lane` of the inverse of diagonal block `warp`
+            const int b0 = warp * 16;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float s = i == lane ? 1.0f : 0.0f;
+#pragma unroll
+                for (int j = 0; j < i; j++) s = fmaf(-Am[(b0 + i) * LDA + b0 + j], x[j], s);
+                x[i] = s;
+                X[(b0 + i) * LDA + b0 + lane] = s;
+            }
+        }
+        float pup, pdown;
+        row_scale(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), pup, pdown);
+        char* gP = (char*)(d.Pt + head * 2 * C * C);
+#pragma unroll
+        for (int t = 0; t < C / 8; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t p[2];
+                split_pair<2>(pv[t][h * 2] * pup, pv[t][h * 2 + 1] * pup, p);
+                const uint32_t o = tile_off<C>(rg * 16 + r + h * 8, t * 8 + c2);
+#pragma unroll
+                for (int k = 0; k < 2; k++) *(uint32_t*)(gP + k * (C * C * 2) + o) = p[k];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int s = 16; s < C; s *= 2) {
+            // thread: one row, a run of columns, of the block below each pair of inverted blocks
+            const int pairs = C / (2 * s), run = pairs * s * s / 128;
+            const int e0 = threadIdx.x * run, pr = e0 / (s * s), i = (e0 / s) % s, j0 = e0 % s;
+            const int b0 = pr * 2 * s;
+            float acc[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[e] = 0.0f;
+            for (int m = 0; m < s; m++) {
+                const float a = Am[(b0 + s + i) * LDA + b0 + m];
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (e < run) acc[e] = fmaf(a, X[(b0 + m) * LDA + b0 + j0 + e], acc[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < run) W[(pr * s + i) * LDA + j0 + e] = acc[e];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[e] = 0.0f;
+            for (int m = 0; m <= i; m++) {
+                const float a = X[(b0 + s + i) * LDA + b0 + s + m];
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (e < run) acc[e] = fmaf(-a, W[(pr * s + m) * LDA + j0 + e], acc[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < run) X[(b0 + s + i) * LDA + b0 + j0 + e] = acc[e];
+            __syncthreads();
+        }
+        float tm = 0.0f;
+        for (int i = threadIdx.x; i < C * C; i += 128) tm = fmaxf(tm, fabsf(X[i / C * LDA + i % C]));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+        if (lane == 0) red[1][warp] = tm;
+        __syncthreads();
+        float tup, tdown;
+        row_scale(fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), tup, tdown);
+        if (threadIdx.x == 0) {
+            tk[TOK_MISC * C] = tdown;
+            tk[TOK_MISC * C + 1] = pdown;
+        }
+        char* gT = (char*)(d.Tt + head * 2 * C * C);
+        for (int i = threadIdx.x; i < C * C / 2; i += 128) {
+            const int row = i / (C / 2), cc = i % (C / 2) * 2;
+            uint32_t p[2];
+            split_pair<2>(X[row * LDA + cc] * tup, X[row * LDA + cc + 1] * tup, p);
+            const uint32_t o = tile_off<C>(row, cc);
+#pragma unroll
+            for (int k = 0; k < 2; k++) *(uint32_t*)(gT + k * (C * C * 2) + o) = p[k];
+        }
+    }
+}
+
+template <int DKP, typename IO>
+cudaError_t prep_go(const DeltaDesc& d, cudaStream_t st) {
+    constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
+    const int sm = 2 * NPK * C * DKP * 2 + (2 * C + C / 2) * (C + 1) * 4;
+    auto kern = delta_prep_kernel<DKP, IO>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm);
+    if (e != cudaSuccess) return e;
+    const int V = 16 / (int)sizeof(IO);
+    const int vec = d.dk % V == 0 && d.ld_q % V == 0 && d.ld_k % V == 0 && ((uintptr_t)d.q & 15) == 0 &&
+                    ((uintptr_t)d.k & 15) == 0;
+    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 128, sm, st>>>(d, vec);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ recurrent form
+// A warp owns 16 columns of one head's state, all dk rows: lane = 8 row groups x 4 groups of 4 columns, NR rows
+// per lane, so the state is read and written once in 16-byte pieces and stays in registers for the T tokens.
+// Per token two sums over dk (k.S and q.S), each a chain over the lane's rows and three shuffles.  Bound by the
+// state's bytes: 8 dk dv of them a head.
+struct StepDesc {
+    long long batch, T;
+    int Hk, Hv, grp, dk, dv, units;
+    float scale;
+    const void *q, *k, *v;
+    const float *g, *beta;
+    void* o;
+    long long ld_q, ld_k, ld_v, ld_o;
+    float* pool;
+    long long n_slots;
+    const int* slots;
+};
+
+template <typename IO, int NR, bool VEC>
+__global__ void __launch_bounds__(128)
+delta_step_kernel(const __grid_constant__ StepDesc d) {
+    const int lane = threadIdx.x & 31;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (id >= d.batch * d.Hv * d.units) return;
+    const int u = (int)(id % d.units), hv = (int)(id / d.units % d.Hv);
+    const long long b = id / d.units / d.Hv;
+    const int hk = hv / d.grp, rl = lane >> 2, cl = lane & 3;
+    const int c0 = u * 16 + cl * 4, r0 = rl * NR;
+    const long long slot = d.slots ? d.slots[b] : b;
+    const IO *q = (const IO*)d.q, *k = (const IO*)d.k, *v = (const IO*)d.v;
+    IO* o = (IO*)d.o;
+    if (slot < 0 || slot >= d.n_slots) {
+        for (long long t = 0; t < d.T; t++)
+            for (int e = 0; e < 4; e++)
+                if (rl == 0 && c0 + e < d.dv) stt(o, (b * d.T + t) * d.ld_o + (long long)hv * d.dv + c0 + e, 0.0f);
+        return;
+    }
+    float* Sg = d.pool + ((size_t)slot * d.Hv + hv) * d.dk * d.dv;
+    float S[NR][4];
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = r0 + i;
+        if (VEC && row < d.dk && c0 < d.dv) {
+            const float4 x = *(const float4*)(Sg + (size_t)row * d.dv + c0);
+            S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) S[i][e] = row < d.dk && c0 + e < d.dv ? Sg[(size_t)row * d.dv + c0 + e] : 0.0f;
+        }
+    }
+    for (long long t = 0; t < d.T; t++) {
+        const long long tok = b * d.T + t;
+        const float al = d.g ? expf(d.g[tok * d.Hv + hv]) : 1.0f;
+        const float be = d.beta ? d.beta[tok * d.Hv + hv] : 1.0f;
+        float kr[NR], qr[NR], vc[4];
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const bool ok = r0 + i < d.dk;
+            kr[i] = ok ? ldt(k, tok * d.ld_k + (long long)hk * d.dk + r0 + i) : 0.0f;
+            qr[i] = ok ? ldt(q, tok * d.ld_q + (long long)hk * d.dk + r0 + i) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            vc[e] = c0 + e < d.dv ? ldt(v, tok * d.ld_v + (long long)hv * d.dv + c0 + e) : 0.0f;
+        float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                S[i][e] *= al;
+                p[e] = fmaf(S[i][e], kr[i], p[e]);
+            }
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] += __shfl_xor_sync(0xffffffffu, p[e], s);
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e] = be * (vc[e] - p[e]);
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                S[i][e] = fmaf(kr[i], p[e], S[i][e]);
+                y[e] = fmaf(S[i][e], qr[i], y[e]);
+            }
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] += __shfl_xor_sync(0xffffffffu, y[e], s);
+        if (rl == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c0 + e < d.dv) stt(o, tok * d.ld_o + (long long)hv * d.dv + c0 + e, d.scale * y[e]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = r0 + i;
+        if (VEC && row < d.dk && c0 < d.dv) {
+            *(float4*)(Sg + (size_t)row * d.dv + c0) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (row < d.dk && c0 + e < d.dv) Sg[(size_t)row * d.dv + c0 + e] = S[i][e];
+        }
+    }
+}
+template <typename IO>
+cudaError_t step_go(const StepDesc& d, cudaStream_t st) {
+    const long long warps = d.batch * d.Hv * d.units;
+    const unsigned blocks = (unsigned)((warps + 3) / 4);
+    const bool vec = d.dv % 4 == 0 && ((uintptr_t)d.pool & 15) == 0;
+    if (d.dk <= 64) {
+        if (vec) delta_step_kernel<IO, 8, true><<<blocks, 128, 0, st>>>(d);
+        else delta_step_kernel<IO, 8, false><<<blocks, 128, 0, st>>>(d);
+    } else {
+        if (vec) delta_step_kernel<IO, 16, true><<<blocks, 128, 0, st>>>(d);
+        else delta_step_kernel<IO, 16, false><<<blocks, 128, 0, st>>>(d);
+    }
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ host
+const char* check(const KMBDeltaParams* p) {
+    if (!p) return "delta: null parameters";
+    if (p->batch < 0 || p->T < 0) return "delta: batch and T must be >= 0";
+    if (p->Hk < 1 || p->Hv < 1 || p->Hv % p->Hk) return "delta: Hv must be a positive multiple of Hk";
+    if (p->Hk > 65535 || p->Hv > 65535) return "delta: at most 65535 heads";
+    if (p->dk < 1 || p->dv < 1 || p->dk > KMB_DELTA_MAX_DIM || p->dv > KMB_DELTA_MAX_DIM)
+        return "delta: dk and dv must be in 1 .. 128";
+    if (p->dtype != KMB_DTYPE_F32 && p->dtype != KMB_DTYPE_BF16) return "delta: unknown dtype";
+    if (p->cu_seqlens) {
+        if (p->batch != 1 || p->n_seq < 1) return "delta: packed sequences need batch = 1 and n_seq >= 1";
+        if (p->n_seq > (1L << 24)) return "delta: at most 2^24 packed sequences";
+    }
+    if (p->batch > (1L << 24) || p->T > 0x7fffffc0L || (double)p->batch * (double)p->T > 2147483584.0)
+        return "delta: at most 2^31 - 64 tokens";
+    if ((p->ld_q && p->ld_q < p->Hk * p->dk) || (p->ld_k && p->ld_k < p->Hk * p->dk) ||
+        (p->ld_v && p->ld_v < p->Hv * p->dv) || (p->ld_o && p->ld_o < p->Hv * p->dv))
+        return "delta: a token stride is shorter than a token";
+    if (p->ld_q > 0x7fffffffL || p->ld_k > 0x7fffffffL || p->ld_v > 0x7fffffffL || p->ld_o > 0x7fffffffL)
+        return "delta: a token stride is at most 2^31 - 1 elements";
+    return nullptr;
+}
+const char* check_launch(const KMBDeltaParams* p, const DeltaDesc& d) {
+    if ((double)d.nseq * d.Hv * d.units > 2147483647.0) return "delta: too many sequences times heads for one launch";
+    if ((double)d.nch * d.Hv > 2147483647.0) return "delta: too many chunks times heads for one launch";
+    (void)p;
+    return nullptr;
+}
+
+// Shapes, pieces and workspace of a call; returns the workspace's bytes
+size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int& DKP) {
+    constexpr int C = kDeltaC;
+    memset(&d, 0, sizeof d);
+    DKP = p->dk <= 64 ? 64 : 128;
+    const int NPK = p->dtype == KMB_DTYPE_BF16 ? 1 : 2;
+    d.T = p->T;
+    d.total = p->batch * p->T;
+    d.nseq = p->cu_seqlens ? (int)p->n_seq : (int)p->batch;
+    d.cu_in = p->cu_seqlens;
+    d.nc = (int)((p->T + C - 1) / C);
+    d.nch = p->cu_seqlens ? (int)(p->T / C + p->n_seq) : (int)(p->batch * d.nc);
+    d.Hk = (int)p->Hk; d.Hv = (int)p->Hv; d.grp = d.Hv / d.Hk; d.dk = (int)p->dk; d.dv = (int)p->dv;
+    d.units = (d.dv + 15) / 16;
+    d.scale = p->scale;
+    d.q = p->q; d.k = p->k; d.v = p->v; d.g = p->g; d.beta = p->beta; d.h0 = p->h0; d.o = p->o; d.hT = p->hT;
+    d.ld_q = p->ld_q ? p->ld_q : p->Hk * p->dk;
+    d.ld_k = p->ld_k ? p->ld_k : p->Hk * p->dk;
+    d.ld_v = p->ld_v ? p->ld_v : p->Hv * p->dv;
+    d.ld_o = p->ld_o ? p->ld_o : p->Hv * p->dv;
+    size_t o = 0;
+    char* base = (char*)ws;
+    auto take = [&](size_t bytes) {
+        char* r = base + o;
+        o += (bytes + 127) & ~(size_t)127;
+        return r;
+    };
+    if (p->cu_seqlens) {
+        d.cu = (const int*)take((size_t)(d.nseq + 1) * 4);
+        d.cstart = (const int*)take((size_t)(d.nseq + 1) * 4);
+    }
+    const size_t ck = (size_t)d.nch * d.Hk, cv = (size_t)d.nch * d.Hv;
+    d.Kt = (__half*)take(ck * NPK * C * DKP * 2);
+    d.Qt = (__half*)take(ck * NPK * C * DKP * 2);
+    d.Tt = (__half*)take(cv * 2 * C * C * 2);
+    d.Pt = (__half*)take(cv * 2 * C * C * 2);
+    d.tok = (float*)take(cv * TOK_ROWS * C * 4);
+    if (train) {
+        const size_t f = cv * d.units * 32 * 4 * 4;   // one 16-byte piece per lane and unit
+        d.Sf = (float*)take(f * (DKP / 8));
+        d.dSf = (float*)take(f * (DKP / 8));
+        d.Uf = (float*)take(f * (C / 8));
+        d.Of = (float*)take(f * (C / 8));
+        d.Rf = (float*)take(f * (C / 8));
+        d.part = (float*)take(cv * d.units * 2 * C * 4);
+        d.anchor = (float*)take(cv * d.units * 4);
+        d.mx = (float*)take(cv * d.units * MX_ROWS * 4);
+    }
+    return o;
+}
+
+}  // namespace
+
+static cudaError_t delta_prep(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st) {
+    if (bf16) return DKP == 64 ? prep_go<64, __nv_bfloat16>(d, st) : prep_go<128, __nv_bfloat16>(d, st);
+    return DKP == 64 ? prep_go<64, float>(d, st) : prep_go<128, float>(d, st);
+}
+
+}  // namespace kmb
+
+using namespace kmb;
+
+extern "C" {
+
+size_t kmb_delta_workspace_floats(const KMBDeltaParams* p, int train) {
+    if (check(p)) return 0;
+    DeltaDesc d;
+    int DKP;
+    return (layout(p, train != 0, nullptr, d, DKP) + 3) / 4;
+}
+
+int kmb_delta_forward(const KMBDeltaParams* p, float* ws, int keep, void* stream) {
+    clear_error();
+    if (const char* m = check(p)) return set_error(m);
+    DeltaDesc d;
+    int DKP;
+    layout(p, keep != 0, ws, d, DKP);
+    if (d.nseq == 0) return 0;
+    if (d.total > 0 && (!p->q || !p->k || !p->v || !p->o)) return set_error("delta: q, k, v and o are required");
+    if (!ws || ((uintptr_t)ws & 15)) return set_error("delta: a 16-byte aligned workspace is required");
+    if (const char* m = check_launch(p, d)) return set_error(m);
+    const bool bf16 = p->dtype == KMB_DTYPE_BF16;
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = cudaSuccess;
+    if (d.cu) {
+        delta_cu_kernel<<<1, 256, 0, st>>>(d.cu_in, d.nseq, (int)d.total, kDeltaC, (int*)d.cu, (int*)d.cstart);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess && d.nch > 0) e = delta_prep(d, DKP, bf16, st);
+    if (e == cudaSuccess) e = delta_chain_fwd(d, DKP, bf16, keep != 0, st);
+    return e == cudaSuccess ? 0 : set_cuda_error("kmb_delta_forward", e);
+}
+
+int kmb_delta_backward(const KMBDeltaParams* p, const KMBDeltaGrads* g, float* ws, void* stream) {
+    clear_error();
+    if (const char* m = check(p)) return set_error(m);
+    if (!g) return set_error("delta backward: null gradients");
+    DeltaDesc d;
+    int DKP;
+    layout(p, true, ws, d, DKP);
+    if (d.nseq == 0) return 0;
+    if (d.total > 0 && (!p->q || !p->k || !p->v || !g->do_ || !g->dq || !g->dk || !g->dv))
+        return set_error("delta backward: q, k, v, do, dq, dk and dv are required");
+    if ((g->ld_do && g->ld_do < p->Hv * p->dv) || (g->ld_dq && g->ld_dq < p->Hk * p->dk) ||
+        (g->ld_dk && g->ld_dk < p->Hk * p->dk) || (g->ld_dv && g->ld_dv < p->Hv * p->dv))
+        return set_error("delta backward: a token stride is shorter than a token");
+    if (g->ld_do > 0x7fffffffL || g->ld_dq > 0x7fffffffL || g->ld_dk > 0x7fffffffL || g->ld_dv > 0x7fffffffL)
+        return set_error("delta backward: a token stride is at most 2^31 - 1 elements");
+    if (!ws || ((uintptr_t)ws & 15)) return set_error("delta backward: the forward's workspace is required");
+    if (const char* m = check_launch(p, d)) return set_error(m);
+    d.go = g->do_; d.dhT = g->dhT; d.dq = g->dq; d.dkk = g->dk; d.dvv = g->dv;
+    d.dg = g->dg; d.dbeta = g->dbeta; d.dh0 = g->dh0;
+    d.ld_do = g->ld_do ? g->ld_do : p->Hv * p->dv;
+    d.ld_dq = g->ld_dq ? g->ld_dq : p->Hk * p->dk;
+    d.ld_dk = g->ld_dk ? g->ld_dk : p->Hk * p->dk;
+    d.ld_dv = g->ld_dv ? g->ld_dv : p->Hv * p->dv;
+    const bool bf16 = p->dtype == KMB_DTYPE_BF16;
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = delta_chain_bwd(d, DKP, bf16, st);
+    if (e == cudaSuccess && d.nch > 0) e = delta_grads(d, DKP, bf16, st);
+    return e == cudaSuccess ? 0 : set_cuda_error("kmb_delta_backward", e);
+}
+
+int kmb_delta_step(const KMBDeltaParams* p, float* pool, long n_slots, const int* slots, void* stream) {
+    clear_error();
+    if (const char* m = check(p)) return set_error(m);
+    if (p->cu_seqlens || p->h0 || p->hT) return set_error("kmb_delta_step: cu_seqlens, h0 and hT must be NULL");
+    if (p->batch == 0 || p->T == 0) return 0;
+    if (!p->q || !p->k || !p->v || !p->o || !pool) return set_error("kmb_delta_step: q, k, v, o and the pool are required");
+    if (n_slots < 0) return set_error("kmb_delta_step: n_slots must be >= 0");
+    StepDesc d{};
+    d.batch = p->batch; d.T = p->T; d.Hk = (int)p->Hk; d.Hv = (int)p->Hv; d.grp = d.Hv / d.Hk;
+    d.dk = (int)p->dk; d.dv = (int)p->dv; d.units = (d.dv + 15) / 16; d.scale = p->scale;
+    if ((double)d.batch * d.Hv * d.units > 4.0 * 2147483647.0) return set_error("kmb_delta_step: batch times heads is too large");
+    d.q = p->q; d.k = p->k; d.v = p->v; d.g = p->g; d.beta = p->beta; d.o = p->o;
+    d.ld_q = p->ld_q ? p->ld_q : p->Hk * p->dk;
+    d.ld_k = p->ld_k ? p->ld_k : p->Hk * p->dk;
+    d.ld_v = p->ld_v ? p->ld_v : p->Hv * p->dv;
+    d.ld_o = p->ld_o ? p->ld_o : p->Hv * p->dv;
+    d.pool = pool; d.n_slots = n_slots; d.slots = slots;
+    cudaError_t e = p->dtype == KMB_DTYPE_BF16 ? step_go<__nv_bfloat16>(d, (cudaStream_t)stream)
+                                               : step_go<float>(d, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : set_cuda_error("kmb_delta_step", e);
+}
+
+}  // extern "C"

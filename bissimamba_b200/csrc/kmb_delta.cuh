@@ -1,0 +1,292 @@
+// kmb_delta.cuh -- shared pieces of the gated delta rule's kernels (delta.cu,
+// delta_fwd.cu, delta_bwd.cu).
+//
+// Chunk of C tokens of one value head, gamma_i the running sum of g inside it,
+// G_ij = exp(gamma_i - gamma_j):
+//   (I + A) U = diag(beta) (V - diag(e^gamma) K S_0),  A_ij = beta_i G_ij k_i.k_j (j < i)
+//   O = scale (diag(e^gamma) Q S_0 + P U),             P_ij = G_ij q_i.k_j (j <= i)
+//   S_C = e^gamma_C S_0 + sum_j G_Cj k_j u_j^T
+// T = (I + A)^-1 and P depend on no state: a first kernel computes them for all
+// chunks at once; the recurrence over chunks then is three products a chunk.
+//
+// Products run on mma.sync (fp16 factors, fp32 accumulation).  A row of an fp32
+// factor is scaled by a power of two to a largest entry in [2^14, 2^15) and cut
+// into two fp16 pieces x = x0 + x1, each rounded to nearest: 22 bits, and an
+// absolute floor 2^-40 below the row's largest entry, so it holds what an fp32
+// product needs.  The three products x0 y0, x0 y1, x1 y0 are summed; a bf16 row
+// is a single piece (8 bits fit in 11).  Where a sum is rounded to bf16 right
+// after, one piece of each factor (11 bits) serves.  Three bf16 pieces would take
+// six products for the same accuracy.  The powers of two are undone in the fp32
+// factors that multiply the accumulators anyway.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace kmb {
+
+// rows of the token factors of a chunk and value head
+enum {
+    TOK_EG = 0,    // e^gamma_i
+    TOK_GC = 1,    // G_Ci = exp(gamma_C - gamma_i)
+    TOK_BETA = 2,  // beta, 2^-100 where it is 0
+    TOK_ON = 3,    // 1, 0 where beta is 0
+    TOK_FK = 4,    // k_i = FK_i * row i of the K tile
+    TOK_FQ = 5,
+    TOK_MISC = 6,  // [0], [1]: T and P = that factor times their tiles
+    TOK_ROWS = 7
+};
+enum { MX_S = 0, MX_U = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
+constexpr int kDeltaC = 64;      // tokens per chunk
+constexpr float kStateFloor = 2.98023223876953125e-08f;   // 2^-25: times a row's `down` (its largest entry / 2^14) = 2^-39..-40 of it
+
+struct DeltaDesc {
+    long long T, total;          // tokens per sequence (fixed length), tokens in all
+    int nseq;
+    const int* cu;               // ws: sanitised offsets [nseq + 1] (packed), else NULL
+    const int* cstart;           // ws: first chunk of each sequence [nseq + 1] (packed)
+    const int* cu_in;            // the caller's offsets
+    int nch, nc;                 // chunks at most; chunks per sequence (fixed length)
+    int Hk, Hv, grp, dk, dv, units;   // units: 16-column slices of dv
+    float scale;
+    const void *q, *k, *v;
+    const float *g, *beta, *h0;
+    void* o;
+    float* hT;
+    long long ld_q, ld_k, ld_v, ld_o;
+    // workspace
+    __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
+    __half *Tt, *Pt;             // [nch][Hv][2][C * C], scaled as a whole
+    float* tok;                  // [nch][Hv][TOK_ROWS][C], see TOK_*
+    // kept for the backward; "fragment order": [nch][Hv][units][tiles][32 lanes][4]
+    float *Sf, *Uf, *Of;         // state at the chunk's start, U, O
+    float *Rf, *dSf;             // backward: dR = T^T dU, adjoint of the state at the chunk's end
+    float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units]
+    float* mx;                   // [nch][Hv][units][MX_ROWS]: down-scale of the largest entry of S, U, dO, dR, dS
+    // gradients
+    const void* go;
+    const float* dhT;
+    void *dq, *dkk, *dvv;
+    float *dg, *dbeta, *dh0;
+    long long ld_do, ld_dq, ld_dk, ld_dv;
+};
+
+// 16-byte pieces of a row are XOR-swizzled by the row so that ldmatrix reads 8 rows without bank conflicts.
+// Tiles are W = 64 or 32 columns wide; wider matrices are several 64-column tiles, `rows` * 128 bytes apart.
+template <int W>
+__device__ __forceinline__ uint32_t tile_off(int row, int col) {
+    if (W == 64) return (uint32_t)(row * 128 + ((((col >> 3) ^ row) & 7) << 4) + ((col & 7) << 1));
+    return (uint32_t)(row * 64 + ((((col >> 3) ^ (row >> 1)) & 3) << 4) + ((col & 7) << 1));
+}
+// matrix of `rows` rows and a multiple of 64 columns
+template <int ROWS>
+__device__ __forceinline__ uint32_t wide_off(int row, int col) {
+    return (uint32_t)((col >> 6) * (ROWS * 128)) + tile_off<64>(row, col & 63);
+}
+
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// lane addresses of ldmatrix.x4, for a 16 x 16 block at (r0, c0):
+//   as stored  -> A fragment a0..a3 (rows = m, columns = k)
+__device__ __forceinline__ int la_row(int lane) { return (lane & 7) + ((lane >> 3) & 1) * 8; }
+__device__ __forceinline__ int la_col(int lane) { return (lane >> 4) * 8; }
+//   as stored  -> B fragments b0 b1 | b0 b1 of two n-tiles (rows = n, columns = k); with .trans and rows = m
+//   (stored transposed, [k][m]) the A fragment takes the same addresses
+__device__ __forceinline__ int lb_row(int lane) { return (lane & 7) + (lane >> 4) * 8; }
+__device__ __forceinline__ int lb_col(int lane) { return ((lane >> 3) & 1) * 8; }
+//   .trans, rows = k, columns = n -> B fragments of two n-tiles: la_row, la_col
+
+// fp16 pieces of the pair (x, y), rounded to nearest
+template <int NP>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[NP]) {
+    __half2 h = __floats2half2_rn(x, y);
+    p[0] = *reinterpret_cast<const uint32_t*>(&h);
+    if constexpr (NP == 2) {
+        h = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+        p[1] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// Power of two that takes m (the largest magnitude of a row) into [2^14, 2^15), and its inverse.  Rows below
+// 2^-112 (zero rows among them) take the factors of 2^-112; an infinite or NaN entry stays one.
+__device__ __forceinline__ void row_scale(float m, float& up, float& down) {
+    int e = (int)(__float_as_uint(m) >> 23);
+    e = e < 15 ? 15 : e;
+    up = __uint_as_float((uint32_t)(268 - e) << 23);
+    down = __uint_as_float((uint32_t)(e - 14) << 23);
+}
+// of the two rows (lane / 4, lane / 4 + 8) of accumulator tiles; m0, m1: least magnitudes to assume
+template <int N>
+__device__ __forceinline__ void frag_scale(const float (&t)[N][4], float (&up)[2], float (&down)[2],
+                                           float m0 = 0.0f, float m1 = 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        m0 = fmaxf(m0, fmaxf(fabsf(t[i][0]), fabsf(t[i][1])));
+        m1 = fmaxf(m1, fmaxf(fabsf(t[i][2]), fabsf(t[i][3])));
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+    }
+    row_scale(m0, up[0], down[0]);
+    row_scale(m1, up[1], down[1]);
+}
+// A fragment pieces of 16 k columns of two accumulator tiles, rows scaled by up (an accumulator is laid out as
+// an A fragment: no data moves between lanes)
+template <int NP>
+__device__ __forceinline__ void frag_pieces(const float (&t0)[4], const float (&t1)[4], const float (&up)[2],
+                                            uint32_t (&a)[NP][4]) {
+    uint32_t p[NP];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float* t = i < 2 ? t0 : t1;
+        split_pair<NP>(t[(i & 1) * 2] * up[i & 1], t[(i & 1) * 2 + 1] * up[i & 1], p);
+#pragma unroll
+        for (int k = 0; k < NP; k++) a[k][i] = p[k];
+    }
+}
+// the larger of the two rows' down-scales, over the warp's 16 rows
+__device__ __forceinline__ float warp_down(const float (&down)[2]) {
+    float m = fmaxf(down[0], down[1]);
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+// acc[t] += sum over pieces of a * B for the column blocks t2 (16 columns) in [from, to): B fragments by
+// load(piece, t2, regs).  Two blocks at a time keep four accumulators in turn; smaller products first.
+template <int NA, int NB, int N, typename LOAD>
+__device__ __forceinline__ void mma_row(float (&acc)[N][4], const uint32_t (&a)[NA][4], int from, int to,
+                                        LOAD load) {
+    constexpr int LIM = NA == 1 && NB == 1 ? 0 : 1;
+#pragma unroll
+    for (int t2 = 0; t2 < N / 2; t2 += 2) {
+        if (t2 + 1 < from || t2 >= to) continue;
+        uint32_t b[NB][2][4];
+#pragma unroll
+        for (int p = 0; p < NB; p++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if (t2 + h >= from && t2 + h < to) load(p, t2 + h, b[p][h]);
+#pragma unroll
+        for (int sum = LIM; sum >= 0; sum--)
+#pragma unroll
+            for (int pb = 0; pb < NB; pb++)
+#pragma unroll
+                for (int pa = 0; pa < NA; pa++)
+                    if (pa + pb == sum) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            if (t2 + h >= from && t2 + h < to) {
+                                mma(acc[2 * (t2 + h)], a[pa], b[pb][h][0], b[pb][h][1]);
+                                mma(acc[2 * (t2 + h) + 1], a[pa], b[pb][h][2], b[pb][h][3]);
+                            }
+                    }
+    }
+}
+
+__device__ __forceinline__ float ldt(const float* p, long long i) { return p[i]; }
+__device__ __forceinline__ float ldt(const __nv_bfloat16* p, long long i) { return __bfloat162float(p[i]); }
+__device__ __forceinline__ void stt(float* p, long long i, float v) { p[i] = v; }
+__device__ __forceinline__ void stt(__nv_bfloat16* p, long long i, float v) { p[i] = __float2bfloat16_rn(v); }
+
+// first token and token count of sequence n
+__device__ __forceinline__ void seq_range(const DeltaDesc& d, int n, long long& start, long long& len) {
+    if (d.cu) {
+        start = d.cu[n];
+        len = d.cu[n + 1] - start;
+    } else {
+        start = (long long)n * d.T;
+        len = d.T;
+    }
+}
+// first token and tokens of a chunk; false if there is no such chunk
+template <int C>
+__device__ __forceinline__ bool chunk_range(const DeltaDesc& d, int chunk, long long& tok0, int& cnt) {
+    int n, c;
+    if (d.cu) {
+        if (chunk >= d.cstart[d.nseq]) return false;
+        int a = 0, b = d.nseq;   // last sequence whose first chunk is <= chunk and that is not empty
+        while (b - a > 1) {
+            const int m = (a + b) >> 1;
+            if (d.cstart[m] <= chunk) a = m;
+            else b = m;
+        }
+        n = a;
+        c = chunk - d.cstart[n];
+    } else {
+        n = chunk / d.nc;
+        c = chunk - n * d.nc;
+    }
+    long long start, len;
+    seq_range(d, n, start, len);
+    tok0 = start + (long long)c * C;
+    cnt = (int)(len - (long long)c * C < C ? len - (long long)c * C : C);
+    return true;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared-memory stage of the chunk recurrences: K, Q tiles, T and P pieces, token factors
+template <int C, int DKP, int NPK, int NPP>
+struct DeltaStage {
+    static constexpr int KQ = NPK * C * DKP * 2;   // bytes of K (and of Q)
+    static constexpr int TT = C * C * 2;           // one piece of T or P
+    static constexpr int oQ = KQ, oT = 2 * KQ, oP = oT + 2 * TT, oTok = oP + NPP * TT;
+    static constexpr int BYTES = oTok + TOK_ROWS * C * 4;
+
+    // copies of one chunk into the stage at `dst`; of T and P only what lies on or below the diagonal blocks
+    static __device__ __forceinline__ void load(const DeltaDesc& d, uint32_t dst, int chunk, int hv) {
+        const int hk = hv / d.grp;
+        const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+        const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+        for (int i = threadIdx.x; i < KQ / 16; i += blockDim.x) {
+            cp16(dst + i * 16, ks + i * 16);
+            cp16(dst + oQ + i * 16, qs + i * 16);
+        }
+        const size_t th = ((size_t)chunk * d.Hv + hv) * 2 * C * C;
+        const char *ts = (const char*)(d.Tt + th), *ps = (const char*)(d.Pt + th);
+        constexpr int CPR = C / 8;   // 16-byte pieces per row
+        for (int i = threadIdx.x; i < C * CPR; i += blockDim.x) {
+            const int r = i / CPR, c8 = i % CPR;
+            if (c8 > 2 * (r >> 4) + 1) continue;
+            const uint32_t o = tile_off<C>(r, c8 * 8);
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                cp16(dst + oT + p * TT + o, ts + p * TT + o);
+                if (p < NPP) cp16(dst + oP + p * TT + o, ps + p * TT + o);
+            }
+        }
+        const char* tk = (const char*)(d.tok + ((size_t)chunk * d.Hv + hv) * TOK_ROWS * C);
+        for (int i = threadIdx.x; i < TOK_ROWS * C / 4; i += blockDim.x) cp16(dst + oTok + i * 16, tk + i * 16);
+    }
+};
+
+cudaError_t delta_chain_fwd(const DeltaDesc& d, int DKP, bool bf16, bool keep, cudaStream_t st);
+cudaError_t delta_chain_bwd(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st);
+cudaError_t delta_grads(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st);
+
+// Warps per block of the chunk recurrences (each owns 16 columns of dv): four, one per SM sub-partition, share
+// the staged tiles.
+inline int delta_warps(const DeltaDesc& d) { return d.units < 4 ? d.units : 4; }
+
+}  // namespace kmb

@@ -17,6 +17,7 @@
 #include "kmb_common.cuh"
 #include "../../include/kmamba.h"
 #include "../../include/kmamba_block.h"
+#include "../../include/kmamba_clip.h"
 
 namespace kmb {
 int set_error(const char* msg);
@@ -501,6 +502,18 @@ int kmb_model_optimizer_step(KMamba* m, void* stream) {
         m->opt.weight_decay, m->lr_eh, m->wd_eh, b1, b2, m->opt.eps, bc1, bc2);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : set_cuda_error("adamw", e);
+}
+
+int kmb_model_clip_gradients(KMamba* m, float max_norm, float* result, float* ws, void* stream) {
+    if (!m) return set_error("kmb_model_clip_gradients: null model");
+    if (!(max_norm > 0.0f)) {
+        if (!m->training) return set_error("kmb_model_clip_gradients: clip_norm needs kmamba_enable_training");
+        max_norm = m->opt.clip_norm;
+    }
+    cudaSetDevice(m->dev);
+    // the arena's padding between tensors holds zeros, so it counts as one tensor
+    const KMBGradTensor t = {m->grads, m->grads, (long long)m->n_params, KMB_DTYPE_F32};
+    return kmb_grad_clip(&t, 1, max_norm, result, ws, stream);
 }
 
 float kmamba_train_batch(KMamba* m, const uint32_t* batch_tokens, size_t batch_size) {
