@@ -470,6 +470,8 @@ def _rows_ld(t, inner, what):
     """Elements between two tokens (or rows) of t, whose last `inner` axes must be contiguous and whose leading axes
     must be walked by one stride."""
     st, sh = t.stride(), t.shape
+    if t.numel() == 0:
+        return 0
     want = 1
     for i in range(1, inner + 1):
         if sh[-i] != 1 and st[-i] != want:

@@ -59,15 +59,16 @@ __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ i
 // ------------------------------------------------------------------ per-chunk matrices
 // Block = (chunk, key head), four warps of 16 rows: the chunk's K and Q as swizzled fp16 tiles (zero behind the
 // last token and behind dk), K K^T and Q K^T once per key head; then for each of its value heads the token
-// factors, T = (I + A)^-1 and P in two fp16 pieces.  T comes from 16 x 16 diagonal blocks by forward
+// factors, T (or M, see kmb_delta.cuh) and P in two fp16 pieces.  T comes from 16 x 16 diagonal blocks by forward
 // substitution, one column per lane, merged in pairs: [[a, 0], [c, b]]^-1 = [[a^-1, 0], [-b^-1 c a^-1, b^-1]].
 // The running sums of g are 64-bit: their differences are what G needs, after a reset (g = -inf, held at -104,
-// where exp is 0 in fp32) too.  beta = 0 is replaced by 2^-100 with a factor 0 beside it, so that u / beta exists.
+// where exp is 0 in fp32) too.  M_ij = T_ij beta_j / beta_i; a beta of 0 is 2^-100 in both: T is then the same in
+// fp32, and the quotient is the one that the limit has.
 constexpr float kBetaTiny = 7.888609052210118e-31f;
 
 template <int DKP, typename IO>
 __global__ void __launch_bounds__(128)
-delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
+delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NPK = F32 ? 2 : 1;
@@ -80,7 +81,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     float* X = Am + C * LDA;
     float* W = X + C * LDA;                               // [C / 2][LDA]
     __shared__ double gam[C];
-    __shared__ float bet[C], fK[C], fQ[C], red[2][4];
+    __shared__ float bet[C], fK[C], fQ[C], red[3][4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunk = blockIdx.x, hk = blockIdx.y;
     long long tok0;
@@ -176,12 +177,9 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 gam[i] = s;
                 carry = __shfl_sync(0xffffffffu, s, 31);
                 float b = i < cnt ? (d.beta ? d.beta[(tok0 + i) * d.Hv + hv] : 1.0f) : 0.0f;
-                const float on = fabsf(b) < kBetaTiny ? 0.0f : 1.0f;
-                if (on == 0.0f) b = kBetaTiny;
-                bet[i] = b;
                 tk[TOK_EG * C + i] = expf((float)s);
                 tk[TOK_BETA * C + i] = b;
-                tk[TOK_ON * C + i] = on;
+                bet[i] = fabsf(b) < kBetaTiny ? kBetaTiny : b;
                 tk[TOK_FK * C + i] = fK[i];
                 tk[TOK_FQ * C + i] = fQ[i];
             }
@@ -267,24 +265,43 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 if (e < run) X[(b0 + s + i) * LDA + b0 + j0 + e] = acc[e];
             __syncthreads();
         }
-        float tm = 0.0f;
-        for (int i = threadIdx.x; i < C * C; i += 128) tm = fmaxf(tm, fabsf(X[i / C * LDA + i % C]));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-        if (lane == 0) red[1][warp] = tm;
-        __syncthreads();
-        float tup, tdown;
-        row_scale(fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), tup, tdown);
-        if (threadIdx.x == 0) {
-            tk[TOK_MISC * C] = tdown;
-            tk[TOK_MISC * C + 1] = pdown;
+        float tm = 0.0f, mm = 0.0f;
+        for (int i = threadIdx.x; i < C * C; i += 128) {
+            const int row = i / C, cc = i % C;
+            const float x = fabsf(X[row * LDA + cc]);
+            tm = fmaxf(tm, x);
+            mm = fmaxf(mm, x * fabsf(bet[cc] / bet[row]));
         }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+        }
+        if (lane == 0) {
+            red[1][warp] = tm;
+            red[2][warp] = mm;
+        }
+        __syncthreads();
+        float tup, tdown, mup, mdown;
+        row_scale(fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), tup, tdown);
+        row_scale(fmaxf(fmaxf(red[2][0], red[2][1]), fmaxf(red[2][2], red[2][3])), mup, mdown);
+        if (threadIdx.x == 0) {
+            tk[TOK_MISC * C] = mdown;
+            tk[TOK_MISC * C + 1] = pdown;
+            tk[TOK_MISC * C + 2] = tdown;
+        }
+        char* gM = (char*)(d.Mt + head * 2 * C * C);
         char* gT = (char*)(d.Tt + head * 2 * C * C);
         for (int i = threadIdx.x; i < C * C / 2; i += 128) {
             const int row = i / (C / 2), cc = i % (C / 2) * 2;
+            const float x = X[row * LDA + cc], y = X[row * LDA + cc + 1];
             uint32_t p[2];
-            split_pair<2>(X[row * LDA + cc] * tup, X[row * LDA + cc + 1] * tup, p);
             const uint32_t o = tile_off<C>(row, cc);
+            split_pair<2>(x * (bet[cc] / bet[row]) * mup, y * (bet[cc + 1] / bet[row]) * mup, p);
+#pragma unroll
+            for (int k = 0; k < 2; k++) *(uint32_t*)(gM + k * (C * C * 2) + o) = p[k];
+            if (!train) continue;
+            split_pair<2>(x * tup, y * tup, p);
 #pragma unroll
             for (int k = 0; k < 2; k++) *(uint32_t*)(gT + k * (C * C * 2) + o) = p[k];
         }
@@ -292,7 +309,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 }
 
 template <int DKP, typename IO>
-cudaError_t prep_go(const DeltaDesc& d, cudaStream_t st) {
+cudaError_t prep_go(const DeltaDesc& d, int train, cudaStream_t st) {
     constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
     const int sm = 2 * NPK * C * DKP * 2 + (2 * C + C / 2) * (C + 1) * 4;
     auto kern = delta_prep_kernel<DKP, IO>;
@@ -301,7 +318,7 @@ cudaError_t prep_go(const DeltaDesc& d, cudaStream_t st) {
     const int V = 16 / (int)sizeof(IO);
     const int vec = d.dk % V == 0 && d.ld_q % V == 0 && d.ld_k % V == 0 && ((uintptr_t)d.q & 15) == 0 &&
                     ((uintptr_t)d.k & 15) == 0;
-    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 128, sm, st>>>(d, vec);
+    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 128, sm, st>>>(d, vec, train);
     return cudaGetLastError();
 }
 
@@ -491,14 +508,15 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     const size_t ck = (size_t)d.nch * d.Hk, cv = (size_t)d.nch * d.Hv;
     d.Kt = (__half*)take(ck * NPK * C * DKP * 2);
     d.Qt = (__half*)take(ck * NPK * C * DKP * 2);
-    d.Tt = (__half*)take(cv * 2 * C * C * 2);
+    d.Mt = (__half*)take(cv * 2 * C * C * 2);
     d.Pt = (__half*)take(cv * 2 * C * C * 2);
     d.tok = (float*)take(cv * TOK_ROWS * C * 4);
     if (train) {
         const size_t f = cv * d.units * 32 * 4 * 4;   // one 16-byte piece per lane and unit
         d.Sf = (float*)take(f * (DKP / 8));
         d.dSf = (float*)take(f * (DKP / 8));
-        d.Uf = (float*)take(f * (C / 8));
+        d.Tt = (__half*)take(cv * 2 * C * C * 2);
+        d.Wf = (float*)take(f * (C / 8));
         d.Of = (float*)take(f * (C / 8));
         d.Rf = (float*)take(f * (C / 8));
         d.part = (float*)take(cv * d.units * 2 * C * 4);
@@ -510,9 +528,10 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
 
 }  // namespace
 
-static cudaError_t delta_prep(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st) {
-    if (bf16) return DKP == 64 ? prep_go<64, __nv_bfloat16>(d, st) : prep_go<128, __nv_bfloat16>(d, st);
-    return DKP == 64 ? prep_go<64, float>(d, st) : prep_go<128, float>(d, st);
+static cudaError_t delta_prep(const DeltaDesc& d, int DKP, bool bf16, int train, cudaStream_t st) {
+    if (bf16)
+        return DKP == 64 ? prep_go<64, __nv_bfloat16>(d, train, st) : prep_go<128, __nv_bfloat16>(d, train, st);
+    return DKP == 64 ? prep_go<64, float>(d, train, st) : prep_go<128, float>(d, train, st);
 }
 
 }  // namespace kmb
@@ -545,7 +564,7 @@ int kmb_delta_forward(const KMBDeltaParams* p, float* ws, int keep, void* stream
         delta_cu_kernel<<<1, 256, 0, st>>>(d.cu_in, d.nseq, (int)d.total, kDeltaC, (int*)d.cu, (int*)d.cstart);
         e = cudaGetLastError();
     }
-    if (e == cudaSuccess && d.nch > 0) e = delta_prep(d, DKP, bf16, st);
+    if (e == cudaSuccess && d.nch > 0) e = delta_prep(d, DKP, bf16, keep != 0, st);
     if (e == cudaSuccess) e = delta_chain_fwd(d, DKP, bf16, keep != 0, st);
     return e == cudaSuccess ? 0 : set_cuda_error("kmb_delta_forward", e);
 }

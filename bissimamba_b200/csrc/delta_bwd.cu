@@ -15,7 +15,7 @@
 // factors e^gamma leaves
 //   dgamma_t = do_t.o_t - v_t.dv_t;   dg_t = <S_0, dS_0> - sum_{s < t in chunk} dgamma_s
 // (the state's inner product at the chunk's start anchors the sum, so errors do
-// not add up along the sequence), and dbeta_t = dR_t.u_t / beta_t.  Both are sums
+// not add up along the sequence), and dbeta_t = dR_t.w_t.  Both are sums
 // over dv of what the recurrence holds in fp32.
 #include "kmb_delta.cuh"
 
@@ -57,11 +57,11 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
             S[t][e] = (d.dhT && i < d.dk && cok[e >> 1]) ? d.dhT[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
 
-    if (nch > 0) ST::load(d, sb, chunk0 + nch - 1, hv);
+    if (nch > 0) ST::load(d, d.Tt, sb, chunk0 + nch - 1, hv);
     cp_commit();
     for (int it = 0; it < nch; it++) {
         const int c = nch - 1 - it;
-        if (c > 0) ST::load(d, sb + ((it + 1) & 1) * ST::BYTES, chunk0 + c - 1, hv);
+        if (c > 0) ST::load(d, d.Tt, sb + ((it + 1) & 1) * ST::BYTES, chunk0 + c - 1, hv);
         cp_commit();
         const long long tok0 = start + (long long)c * C;
         const int cnt = (int)(len - (long long)c * C < C ? len - (long long)c * C : C);
@@ -128,7 +128,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
                     ldm4t(b, st + ST::oP + p * ST::TT + tile_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
                 });
             }
-            const float ft = tk[TOK_MISC * C], fp = tk[TOK_MISC * C + 1] * d.scale;
+            const float ft = tk[TOK_MISC * C + 2], fp = tk[TOK_MISC * C + 1] * d.scale;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -157,7 +157,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
             }
             // dV, and what the gates' gradients sum over dv
             {
-                const float4* pu = (const float4*)d.Uf + fb * NT * 32 + lane;
+                const float4* pu = (const float4*)d.Wf + fb * NT * 32 + lane;
                 const float4* po = (const float4*)d.Of + fb * NT * 32 + lane;
                 float4* pr = (float4*)d.Rf + fb * NT * 32 + lane;
                 const IO* pv = (const IO*)d.v + tok0 * d.ld_v + (long long)hv * d.dv + col[0];
@@ -170,9 +170,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int i = t * 8 + c2 + (e & 1);
-                        const float be = tk[TOK_BETA * C + i];
-                        const float dv = be * tk[TOK_ON * C + i] * Y[t][e];
-                        bs[t][e & 1] = fmaf(Y[t][e], uu[e] / be, bs[t][e & 1]);
+                        const float dv = tk[TOK_BETA * C + i] * Y[t][e];
+                        bs[t][e & 1] = fmaf(Y[t][e], uu[e], bs[t][e & 1]);
                         ts[t][e & 1] = fmaf(G[t][e], oo[e], ts[t][e & 1]);
                         if (i < cnt && cok[e >> 1]) {
                             ts[t][e & 1] = fmaf(-ldt(pv + (long long)i * ldv, (e >> 1) * 8), dv, ts[t][e & 1]);
@@ -209,7 +208,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
                     const int i = t * 8 + c2 + (e & 1);
                     const float eg = tk[TOK_EG * C + i];
                     G[t][e] *= d.scale * eg * tk[TOK_FQ * C + i];
-                    Y[t][e] *= -(tk[TOK_BETA * C + i] * tk[TOK_ON * C + i]) * eg * tk[TOK_FK * C + i];
+                    Y[t][e] *= -tk[TOK_BETA * C + i] * eg * tk[TOK_FK * C + i];
                     if (e < 2) m0 = fmaxf(m0, fabsf(G[t][e]));
                     else m1 = fmaxf(m1, fabsf(G[t][e]));
                 }
@@ -432,11 +431,11 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 float4 uu = make_float4(0.0f, 0.0f, 0.0f, 0.0f), rr = uu;
                 if (u0 + x < d.units) {
                     const size_t at = ((head * d.units + u0 + x) * NT + t) * 32 + l;
-                    uu = ((const float4*)d.Uf)[at];
+                    uu = ((const float4*)d.Wf)[at];
                     rr = ((const float4*)d.Rf)[at];
                 }
                 const int tok = t * 8 + (l & 3) * 2, row = x * 16 + (l >> 2);
-                const float a0 = tk[TOK_ON * C + tok] * uU, a1 = tk[TOK_ON * C + tok + 1] * uU;
+                const float a0 = tk[TOK_BETA * C + tok] * uU, a1 = tk[TOK_BETA * C + tok + 1] * uU;
                 uint32_t p[NP], q[NP];
                 const uint32_t o0 = tile_off<64>(row, tok), o1 = tile_off<64>(row + 8, tok);
                 split_pair<NP>(uu.x * a0, uu.y * a1, p);
@@ -523,7 +522,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 const int i = rg * 16 + r + (e >> 1) * 8, j = ch * 32 + t * 8 + c2 + (e & 1);
                 const float g = j <= i ? expf((float)(gam[i] - gam[j])) : 0.0f;
                 dP[t][e] = j <= i ? g * wP * dP[t][e] : 0.0f;
-                dA[t][e] = j < i ? g * wA * tk[TOK_BETA * C + i] * tk[TOK_ON * C + i] * dA[t][e] : 0.0f;
+                dA[t][e] = j < i ? g * wA * tk[TOK_BETA * C + i] * dA[t][e] : 0.0f;
                 m[0] = fmaxf(m[0], fabsf(dP[t][e] * tk[TOK_FK * C + j]));
                 m[1] = fmaxf(m[1], fabsf(dP[t][e] * tk[TOK_FQ * C + i]));
                 m[2] = fmaxf(m[2], fabsf(dA[t][e] * tk[TOK_FK * C + j]));
@@ -571,7 +570,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             const int i = rg * 16 + r + h * 8;
             const float eg = tk[TOK_EG * C + i];
             fq[h] = d.scale * eg * sG * sS;
-            fz[h] = -tk[TOK_BETA * C + i] * tk[TOK_ON * C + i] * eg * sR * sS;
+            fz[h] = -tk[TOK_BETA * C + i] * eg * sR * sS;
             fu[h] = tk[TOK_GC * C + i] * sU * sD;
         }
 #pragma unroll

@@ -5,7 +5,7 @@
 // accumulators of m16n8 products.  Transposed, every product of a chunk takes
 // its fp32 factor from the registers of the same warp (an accumulator tile is
 // laid out as an A operand) and its other factor from shared memory:
-//   (K S)^T = S^T K^T;  U^T = (beta (V - e^gamma K S))^T T^T;  O^T = e^gamma S^T Q^T + U^T P^T
+//   (K S)^T = S^T K^T;  W^T = (V - e^gamma K S)^T M^T;  U = beta W;  O^T = e^gamma S^T Q^T + U^T P^T
 //   S^T <- e^gamma_C S^T + (G_C. U)^T K
 // so the chain of a chunk needs no exchange between warps; the block's warps
 // only share the staged tiles (cp.async, two stages, one chunk ahead).
@@ -50,10 +50,10 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
             S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
 
-    if (nch > 0) ST::load(d, sb, chunk0, hv);
+    if (nch > 0) ST::load(d, d.Mt, sb, chunk0, hv);
     cp_commit();
     for (int c = 0; c < nch; c++) {
-        if (c + 1 < nch) ST::load(d, sb + ((c + 1) & 1) * ST::BYTES, chunk0 + c + 1, hv);
+        if (c + 1 < nch) ST::load(d, d.Mt, sb + ((c + 1) & 1) * ST::BYTES, chunk0 + c + 1, hv);
         cp_commit();
         const long long tok0 = start + (long long)c * C;
         const int cnt = (int)(len - (long long)c * C < C ? len - (long long)c * C : C);
@@ -104,17 +104,17 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
                 mma_row<2, NPK>(X, a, 0, C / 16, ldk);
                 mma_row<NPO, NPK>(O, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, C / 16, ldq);
             }
-            // right-hand side beta (v - e^gamma K S), and e^gamma Q S
+            // right-hand side v - e^gamma K S, and e^gamma Q S
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int i = t * 8 + c2 + (e & 1);
                     const float eg = tk[TOK_EG * C + i] * dn[e >> 1];
-                    X[t][e] = tk[TOK_BETA * C + i] * (V[t][e] - eg * tk[TOK_FK * C + i] * X[t][e]);
+                    X[t][e] = V[t][e] - eg * tk[TOK_FK * C + i] * X[t][e];
                     O[t][e] *= eg * tk[TOK_FQ * C + i];
                 }
-            // U^T = X T^T: row i of T reaches columns j <= i only
+            // W^T = X M^T: row i of M reaches columns j <= i only
             float U[NT][4];
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -135,16 +135,16 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) U[t][e] *= ft * dn[e >> 1];
             if (KEEP) {
-                float4* p = (float4*)d.Uf + fb * NT * 32 + lane;
+                float4* p = (float4*)d.Wf + fb * NT * 32 + lane;
 #pragma unroll
                 for (int t = 0; t < NT; t++) p[t * 32] = make_float4(U[t][0], U[t][1], U[t][2], U[t][3]);
             }
-            // a token whose beta is 0 has an exactly empty u
+            // U = beta W
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    U[t][e] *= tk[TOK_ON * C + t * 8 + c2 + (e & 1)];
+                    U[t][e] *= tk[TOK_BETA * C + t * 8 + c2 + (e & 1)];
                     X[t][e] = 0.0f;
                 }
             // O^T += U^T P^T

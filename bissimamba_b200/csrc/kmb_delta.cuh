@@ -3,11 +3,14 @@
 //
 // Chunk of C tokens of one value head, gamma_i the running sum of g inside it,
 // G_ij = exp(gamma_i - gamma_j):
-//   (I + A) U = diag(beta) (V - diag(e^gamma) K S_0),  A_ij = beta_i G_ij k_i.k_j (j < i)
-//   O = scale (diag(e^gamma) Q S_0 + P U),             P_ij = G_ij q_i.k_j (j <= i)
+//   w_i = v_i - e^gamma_i S_0^T k_i - sum_{j < i} G_ij (k_i.k_j) u_j,   u_i = beta_i w_i
+//   O = scale (diag(e^gamma) Q S_0 + P U),   P_ij = G_ij q_i.k_j (j <= i)
 //   S_C = e^gamma_C S_0 + sum_j G_Cj k_j u_j^T
-// T = (I + A)^-1 and P depend on no state: a first kernel computes them for all
-// chunks at once; the recurrence over chunks then is three products a chunk.
+// With a_ij = G_ij k_i.k_j (j < i):  W = M (V - diag(e^gamma) K S_0), M = (I + a diag(beta))^-1,
+// and the adjoint of U is T^T dU, T = (I + diag(beta) a)^-1 = diag(beta) M diag(beta)^-1.  W and T^T dU exist where
+// beta is 0, and their product is beta's gradient, so the forward takes M and the backward T.
+// M, T and P depend on no state: a first kernel computes them for all chunks at
+// once; the recurrence over chunks then is three products a chunk.
 //
 // Products run on mma.sync (fp16 factors, fp32 accumulation).  A row of an fp32
 // factor is scaled by a power of two to a largest entry in [2^14, 2^15) and cut
@@ -30,12 +33,11 @@ namespace kmb {
 enum {
     TOK_EG = 0,    // e^gamma_i
     TOK_GC = 1,    // G_Ci = exp(gamma_C - gamma_i)
-    TOK_BETA = 2,  // beta, 2^-100 where it is 0
-    TOK_ON = 3,    // 1, 0 where beta is 0
-    TOK_FK = 4,    // k_i = FK_i * row i of the K tile
-    TOK_FQ = 5,
-    TOK_MISC = 6,  // [0], [1]: T and P = that factor times their tiles
-    TOK_ROWS = 7
+    TOK_BETA = 2,  // beta, 0 behind the last token
+    TOK_FK = 3,    // k_i = FK_i * row i of the K tile
+    TOK_FQ = 4,
+    TOK_MISC = 5,  // [0], [1], [2]: M, P and T = that factor times their tiles
+    TOK_ROWS = 6
 };
 enum { MX_S = 0, MX_U = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
 constexpr int kDeltaC = 64;      // tokens per chunk
@@ -57,10 +59,10 @@ struct DeltaDesc {
     long long ld_q, ld_k, ld_v, ld_o;
     // workspace
     __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
-    __half *Tt, *Pt;             // [nch][Hv][2][C * C], scaled as a whole
+    __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], scaled as a whole; Tt for training only
     float* tok;                  // [nch][Hv][TOK_ROWS][C], see TOK_*
     // kept for the backward; "fragment order": [nch][Hv][units][tiles][32 lanes][4]
-    float *Sf, *Uf, *Of;         // state at the chunk's start, U, O
+    float *Sf, *Wf, *Of;         // state at the chunk's start, W, O
     float *Rf, *dSf;             // backward: dR = T^T dU, adjoint of the state at the chunk's end
     float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units]
     float* mx;                   // [nch][Hv][units][MX_ROWS]: down-scale of the largest entry of S, U, dO, dR, dS
@@ -246,7 +248,7 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared-memory stage of the chunk recurrences: K, Q tiles, T and P pieces, token factors
+// Shared-memory stage of the chunk recurrences: K, Q tiles, pieces of M (or T) and P, token factors
 template <int C, int DKP, int NPK, int NPP>
 struct DeltaStage {
     static constexpr int KQ = NPK * C * DKP * 2;   // bytes of K (and of Q)
@@ -254,8 +256,9 @@ struct DeltaStage {
     static constexpr int oQ = KQ, oT = 2 * KQ, oP = oT + 2 * TT, oTok = oP + NPP * TT;
     static constexpr int BYTES = oTok + TOK_ROWS * C * 4;
 
-    // copies of one chunk into the stage at `dst`; of T and P only what lies on or below the diagonal blocks
-    static __device__ __forceinline__ void load(const DeltaDesc& d, uint32_t dst, int chunk, int hv) {
+    // copies of one chunk into the stage at `dst`, T or M from `tiles`; of it and of P only what lies on or below the diagonal blocks
+    static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t dst, int chunk,
+                                                int hv) {
         const int hk = hv / d.grp;
         const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
         const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
@@ -264,7 +267,7 @@ struct DeltaStage {
             cp16(dst + oQ + i * 16, qs + i * 16);
         }
         const size_t th = ((size_t)chunk * d.Hv + hv) * 2 * C * C;
-        const char *ts = (const char*)(d.Tt + th), *ps = (const char*)(d.Pt + th);
+        const char *ts = (const char*)(tiles + th), *ps = (const char*)(d.Pt + th);
         constexpr int CPR = C / 8;   // 16-byte pieces per row
         for (int i = threadIdx.x; i < C * CPR; i += blockDim.x) {
             const int r = i / CPR, c8 = i % CPR;
