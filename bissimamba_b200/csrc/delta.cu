@@ -9,6 +9,7 @@ namespace kmb {
 int set_error(const char* msg);
 int set_cuda_error(const char* where, cudaError_t e);
 void clear_error();
+int* device_status();
 
 namespace {
 
@@ -520,13 +521,19 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
         d.Of = (float*)take(f * (C / 8));
         d.Rf = (float*)take(f * (C / 8));
         d.part = (float*)take(cv * d.units * 2 * C * 4);
-        d.anchor = (float*)take(cv * d.units * 4);
-        d.mx = (float*)take(cv * d.units * MX_ROWS * 4);
+        d.anchor = (float*)take(cv * d.units * 4 * 4);
+        d.mx = (float*)take(cv * d.units * 4 * MX_ROWS * 4);
     }
     return o;
 }
 
 }  // namespace
+
+int delta_sms() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
 
 static cudaError_t delta_prep(const DeltaDesc& d, int DKP, bool bf16, int train, cudaStream_t st) {
     if (bf16)
@@ -559,6 +566,7 @@ int kmb_delta_forward(const KMBDeltaParams* p, float* ws, int keep, void* stream
     if (const char* m = check_launch(p, d)) return set_error(m);
     const bool bf16 = p->dtype == KMB_DTYPE_BF16;
     cudaStream_t st = (cudaStream_t)stream;
+    d.status = device_status();
     cudaError_t e = cudaSuccess;
     if (d.cu) {
         delta_cu_kernel<<<1, 256, 0, st>>>(d.cu_in, d.nseq, (int)d.total, kDeltaC, (int*)d.cu, (int*)d.cstart);
@@ -594,6 +602,7 @@ int kmb_delta_backward(const KMBDeltaParams* p, const KMBDeltaGrads* g, float* w
     d.ld_dv = g->ld_dv ? g->ld_dv : p->Hv * p->dv;
     const bool bf16 = p->dtype == KMB_DTYPE_BF16;
     cudaStream_t st = (cudaStream_t)stream;
+    d.status = device_status();
     cudaError_t e = delta_chain_bwd(d, DKP, bf16, st);
     if (e == cudaSuccess && d.nch > 0) e = delta_grads(d, DKP, bf16, st);
     return e == cudaSuccess ? 0 : set_cuda_error("kmb_delta_backward", e);

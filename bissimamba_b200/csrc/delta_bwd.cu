@@ -4,8 +4,8 @@
 // to the first,
 //   dU = scale P^T dO + diag(G_C.) K dS_C;   dR = T^T dU;   dV = beta dR
 //   dS_0 = e^gamma_C dS_C + scale (e^gamma Q)^T dO - (beta e^gamma K)^T dR
-// the forward's three products again, run the other way by the same scheme (a
-// warp owns 16 columns of dv and keeps dS^T in registers).  All else has no
+// the forward's three products again, run the other way by the same scheme (four
+// warps on 16 columns of dv, dS^T in registers).  All else has no
 // recurrence and is a second kernel, one block per chunk and key head:
 //   dP = scale dO U^T (j <= i);   dA = -dR U^T (j < i)
 //   dQ = scale e^gamma dO S_0^T + (dP*G) K
@@ -22,222 +22,262 @@
 namespace kmb {
 namespace {
 
-template <int DKP, typename IO>
-__global__ void __launch_bounds__(128, 2)
-delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
+template <int DKP, typename IO, int NU>
+__global__ void __launch_bounds__(128 * NU, 2 / NU)
+delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NPK = F32 ? 2 : 1;
     using ST = DeltaStage<C, DKP, NPK, 2>;
-    constexpr int NT = C / 8, KT = DKP / 8;
+    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;
     constexpr int PK = C * DKP * 2;
+    using FS = FragBuf<DKP / 16, 2>;
+    using FX = FragBuf<C / 16, 2>;
+    using FG = FragBuf<C / 16, NPK>;
+    constexpr int EX = FS::BYTES + 3 * FX::BYTES + FG::BYTES;
     extern __shared__ __align__(128) unsigned char sm[];
+    __shared__ __align__(8) uint64_t full[2];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ub = (d.units + nw - 1) / nw;
-    const int u = (int)(blockIdx.x % ub) * nw + warp;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 2, w = warp & 3;
+    unsigned char* exS = sm + 2 * ST::BYTES + grp * EX;
+    unsigned char *exG = exS + FS::BYTES, *exX = exG + FG::BYTES, *exE = exX + FX::BYTES, *exF = exE + FX::BYTES;
+    const int ub = (d.units + NU - 1) / NU;
+    const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, n = (int)(blockIdx.x / ub) / d.Hv;
     const bool on = u < d.units;
     const int r = lane >> 2, c2 = (lane & 3) * 2;
     const int col[2] = {u * 16 + r, u * 16 + r + 8};
-    const bool cok[2] = {on && col[0] < d.dv, on && col[1] < d.dv};
-    const int ldv = (int)d.ld_v, ldo = (int)d.ld_do, lddv = (int)d.ld_dv;
+    const bool cok[2] = {col[0] < d.dv, col[1] < d.dv};
+    const int ldv = (int)d.ld_v, ldg = (int)d.ld_do, lddv = (int)d.ld_dv;
     long long start, len;
     seq_range(d, n, start, len);
     const int chunk0 = d.cu ? d.cstart[n] : n * d.nc;
     const int nch = (int)((len + C - 1) / C);
 
-    float S[KT][4];   // dS^T
+    float S[KTW][4];   // dS^T, the warp's quarter of dk
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
 #pragma unroll
-    for (int t = 0; t < KT; t++)
+    for (int t = 0; t < KTW; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int i = t * 8 + c2 + (e & 1);
+            const int i = (w * KTW + t) * 8 + c2 + (e & 1);
             S[t][e] = (d.dhT && i < d.dk && cok[e >> 1]) ? d.dhT[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
-
-    if (nch > 0) ST::load(d, d.Tt, sb, chunk0 + nch - 1, hv);
-    cp_commit();
+    const auto load_t = [&](const void* base, long long ld, int ldi, int c, float (&V)[2][4]) {
+        const long long t0 = (long long)c * C + w * 16;
+        const IO* p = (const IO*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + c2 + (e & 1);
+                V[t][e] = (t0 + i < len && cok[e >> 1]) ? ldt(p + (long long)i * ldi, (e >> 1) * 8) : 0.0f;
+            }
+    };
+    float sup[2], sdn[2], up[2], dn[2];
+    const auto put_state = [&]() {
+        frag_scale(S, sup, sdn);
+#pragma unroll
+        for (int b = 0; b < KBW; b++) FS::put(exS, w * KBW + b, lane, S[2 * b], S[2 * b + 1], sup, sdn);
+    };
+    float G[2][4];   // dO^T of the warp's tokens
+    float gdn[2];
+    const auto put_go = [&]() {
+        frag_scale(G, up, gdn);
+        FG::put(exG, w, lane, G[0], G[1], up, gdn);
+    };
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&full[0]), 1);
+        mbar_init(smem_u32(&full[1]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (nch > 0) ST::load(d, d.Tt, sb, smem_u32(&full[0]), chunk0 + nch - 1, hv);
+    }
+    put_state();
+    float Gn[2][4];
+    if (nch > 0) {
+        load_t(d.go, d.ld_do, ldg, nch - 1, G);
+        put_go();
+    }
+    __syncthreads();
     for (int it = 0; it < nch; it++) {
         const int c = nch - 1 - it;
-        if (c > 0) ST::load(d, d.Tt, sb + ((it + 1) & 1) * ST::BYTES, chunk0 + c - 1, hv);
-        cp_commit();
-        const long long tok0 = start + (long long)c * C;
-        const int cnt = (int)(len - (long long)c * C < C ? len - (long long)c * C : C);
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        float G[NT][4];   // dO^T
-        {
-            const IO* p = (const IO*)d.go + tok0 * d.ld_do + (long long)hv * d.dv + col[0];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    G[t][e] = (i < cnt && cok[e >> 1]) ? ldt(p + (long long)i * ldo, (e >> 1) * 8) : 0.0f;
-                }
+        const bool got = mbar_wait(smem_u32(&full[it & 1]), (it >> 1) & 1);
+        if (!__syncthreads_and(got)) {
+            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            return;
         }
-        cp_wait<1>();
-        __syncthreads();
+        if (threadIdx.x == 0 && c > 0)
+            ST::load(d, d.Tt, sb + ((it + 1) & 1) * ST::BYTES, smem_u32(&full[(it + 1) & 1]), chunk0 + c - 1, hv);
+        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);
         const uint32_t st = sb + (it & 1) * ST::BYTES;
         const float* tk = (const float*)(sm + (it & 1) * ST::BYTES + ST::oTok);
+        const float* tw = tk + w * 16 + c2;
+        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+        // what the end of the chunk reads: in flight under the products
+        float V[2][4];
+        float4 w4[2], o4[2];
+        load_t(d.v, d.ld_v, ldv, c, V);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const size_t at = (fb * (C / 8) + w * 2 + t) * 32 + lane;
+            w4[t] = on ? ((const float4*)d.Wf)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            o4[t] = on ? ((const float4*)d.Of)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
         if (on) {
-            float X[NT][4], Y[NT][4], up[2], dn[2], ts[NT][2], bs[NT][2];
+            float4* p = (float4*)d.dSf + (fb * KT + w * KTW) * 32 + lane;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
+            for (int t = 0; t < KTW; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
+            const float m = warp_down(sdn), mg = warp_down(gdn);
+            if (lane == 0) {
+                d.mx[(fb * 4 + w) * MX_ROWS + MX_DS] = m;
+                d.mx[(fb * 4 + w) * MX_ROWS + MX_DO] = mg;
+            }
+        }
+        // K dS_C
+        float X[2][4], Y[2][4], part[2][4];
+        zero(X);
+        zero(Y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) X[t][e] = Y[t][e] = 0.0f;
+        for (int s = 0; s < 4; s++) {
+            zero(part);
+#pragma unroll
+            for (int b = 0; b < KBW; b++) {
+                const int kk = s * KBW + b;
+                uint32_t a[2][4];
+                FS::template get<2>(exS, kk, lane, a);
+                const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
+            }
+            FS::scale(exS, s * KBW, lane, dn);
+            add_scaled(X, part, dn);
+        }
+        // P^T dO: column j of P has rows i >= j only
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            if (kk < w) continue;
+            uint32_t a[NPK][4];
+            FG::template get<NPK>(exG, kk, lane, a);
+            FG::scale(exG, kk, lane, dn);
+            const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
+            zero(part);
+            mma_row<NPK, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
+            add_scaled(Y, part, dn);
+        }
+        const float ft = tk[TOK_MISC * C + 2], fp = tk[TOK_MISC * C + 1] * d.scale;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                X[t][e] = fmaf(Y[t][e], fp, X[t][e] * (tw[TOK_GC * C + i] * tw[TOK_FK * C + i]));
+                Y[t][e] = 0.0f;
+            }
+        frag_scale(X, up, dn);
+        FX::put(exX, w, lane, X[0], X[1], up, dn);
+        // dO with the factors of the state's product
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                X[t][e] = G[t][e] * (d.scale * tw[TOK_EG * C + i] * tw[TOK_FQ * C + i]);
+            }
+        frag_scale(X, up, dn);
+        FX::put(exE, w, lane, X[0], X[1], up, dn);
+        unit_bar(grp);
+        // dR^T = dU^T T
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            if (kk < w) continue;
+            uint32_t a[2][4];
+            FX::template get<2>(exX, kk, lane, a);
+            FX::scale(exX, kk, lane, dn);
+            const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
+            zero(part);
+            mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oT + p * ST::TT + o); });
+            add_scaled(Y, part, dn);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                Y[t][e] *= ft;
+                X[t][e] = Y[t][e] * -(tw[TOK_BETA * C + i] * tw[TOK_EG * C + i] * tw[TOK_FK * C + i]);
+            }
+        frag_scale(X, up, dn);
+        FX::put(exF, w, lane, X[0], X[1], up, dn);
+        unit_bar(grp);
+        // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q - (beta e^gamma dR)^T K
+        const float last = tk[TOK_EG * C + C - 1];
+#pragma unroll
+        for (int t = 0; t < KTW; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) S[t][e] *= last;
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            uint32_t a[2][4];
+            float ps[KTW][4];
+            FX::template get<2>(exE, kk, lane, a);
+            FX::scale(exE, kk, lane, dn);
+            zero(ps);
+            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                ldm4t(f, st + ST::oQ + p * PK +
+                             wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+            });
+            add_scaled(S, ps, dn);
+            FX::template get<2>(exF, kk, lane, a);
+            FX::scale(exF, kk, lane, dn);
+            zero(ps);
+            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+            });
+            add_scaled(S, ps, dn);
+        }
+        put_state();
+        // dV, and what the gates' gradients sum over dv
+        frag_scale(Y, up, dn);
+        {
+            const float m = warp_down(dn);
+            if (on && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_R] = m;
+            const long long t0 = (long long)c * C + w * 16;
+            IO* pd = (IO*)d.dvv + (start + t0) * d.ld_dv + (long long)hv * d.dv + col[0];
+            float ts[2][2], bs[2][2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if (on)
+                    *((float4*)d.Rf + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(Y[t][0], Y[t][1], Y[t][2], Y[t][3]);
+                const float ww[4] = {w4[t].x, w4[t].y, w4[t].z, w4[t].w}, oo[4] = {o4[t].x, o4[t].y, o4[t].z, o4[t].w};
                 ts[t][0] = ts[t][1] = bs[t][0] = bs[t][1] = 0.0f;
-            }
-            // K dS_C
-            frag_scale(S, up, dn);
-            const float sd[2] = {dn[0], dn[1]};
-            {
-                const float m = warp_down(dn);
-                if (lane == 0) d.mx[fb * MX_ROWS + MX_DS] = m;
-                float4* p = (float4*)d.dSf + fb * KT * 32 + lane;
-#pragma unroll
-                for (int t = 0; t < KT; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
-            }
-#pragma unroll
-            for (int kk = 0; kk < DKP / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(S[2 * kk], S[2 * kk + 1], up, a);
-                mma_row<2, NPK>(X, a, 0, C / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4(b, st + p * PK + wide_off<C>(t2 * 16 + lb_row(lane), kk * 16 + lb_col(lane)));
-                });
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int i = t * 8 + c2 + (e & 1);
-                    X[t][e] *= tk[TOK_GC * C + i] * tk[TOK_FK * C + i] * dn[e >> 1];
+                    const float dv = tw[TOK_BETA * C + t * 8 + (e & 1)] * Y[t][e];
+                    bs[t][e & 1] = fmaf(Y[t][e], ww[e], bs[t][e & 1]);
+                    ts[t][e & 1] = fmaf(G[t][e], oo[e], ts[t][e & 1]);
+                    ts[t][e & 1] = fmaf(-V[t][e], dv, ts[t][e & 1]);
+                    if (t0 + i < len && cok[e >> 1]) stt(pd + (long long)i * lddv, (e >> 1) * 8, dv);
                 }
-            // P^T dO: column j of P has rows i >= j only
-            frag_scale(G, up, dn);
-            {
-                const float m = warp_down(dn);
-                if (lane == 0) d.mx[fb * MX_ROWS + MX_DO] = m;
-            }
 #pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[NPK][4];
-                frag_pieces<NPK>(G[2 * kk], G[2 * kk + 1], up, a);
-                mma_row<NPK, 2>(Y, a, 0, kk + 1, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, st + ST::oP + p * ST::TT + tile_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
-                });
-            }
-            const float ft = tk[TOK_MISC * C + 2], fp = tk[TOK_MISC * C + 1] * d.scale;
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    X[t][e] = fmaf(Y[t][e], fp * dn[e >> 1], X[t][e]);
-                    Y[t][e] = 0.0f;
-                }
-            // dR^T = dU^T T
-            frag_scale(X, up, dn);
-#pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(X[2 * kk], X[2 * kk + 1], up, a);
-                mma_row<2, 2>(Y, a, 0, kk + 1, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, st + ST::oT + p * ST::TT + tile_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
-                });
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) Y[t][e] *= ft * dn[e >> 1];
-            frag_scale(Y, up, dn);
-            {
-                const float m = warp_down(dn);
-                if (lane == 0) d.mx[fb * MX_ROWS + MX_R] = m;
-            }
-            // dV, and what the gates' gradients sum over dv
-            {
-                const float4* pu = (const float4*)d.Wf + fb * NT * 32 + lane;
-                const float4* po = (const float4*)d.Of + fb * NT * 32 + lane;
-                float4* pr = (float4*)d.Rf + fb * NT * 32 + lane;
-                const IO* pv = (const IO*)d.v + tok0 * d.ld_v + (long long)hv * d.dv + col[0];
-                IO* pd = (IO*)d.dvv + tok0 * d.ld_dv + (long long)hv * d.dv + col[0];
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const float4 u4 = pu[t * 32], o4 = po[t * 32];
-                    pr[t * 32] = make_float4(Y[t][0], Y[t][1], Y[t][2], Y[t][3]);
-                    const float uu[4] = {u4.x, u4.y, u4.z, u4.w}, oo[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int i = t * 8 + c2 + (e & 1);
-                        const float dv = tk[TOK_BETA * C + i] * Y[t][e];
-                        bs[t][e & 1] = fmaf(Y[t][e], uu[e], bs[t][e & 1]);
-                        ts[t][e & 1] = fmaf(G[t][e], oo[e], ts[t][e & 1]);
-                        if (i < cnt && cok[e >> 1]) {
-                            ts[t][e & 1] = fmaf(-ldt(pv + (long long)i * ldv, (e >> 1) * 8), dv, ts[t][e & 1]);
-                            stt(pd + (long long)i * lddv, (e >> 1) * 8, dv);
-                        }
+                    for (int o = 4; o < 32; o <<= 1) {
+                        ts[t][h] += __shfl_xor_sync(0xffffffffu, ts[t][h], o);
+                        bs[t][h] += __shfl_xor_sync(0xffffffffu, bs[t][h], o);
                     }
+                if (on && r == t) {
+                    float* pp = d.part + fb * 2 * C + w * 16 + t * 8 + c2;
+                    *(float2*)pp = make_float2(ts[t][0], ts[t][1]);
+                    *(float2*)(pp + C) = make_float2(bs[t][0], bs[t][1]);
                 }
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) {
-                            ts[t][h] += __shfl_xor_sync(0xffffffffu, ts[t][h], o);
-                            bs[t][h] += __shfl_xor_sync(0xffffffffu, bs[t][h], o);
-                        }
-                float* pp = d.part + fb * 2 * C;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-                    if (r == t) {
-                        pp[t * 8 + c2] = ts[t][0];
-                        pp[t * 8 + c2 + 1] = ts[t][1];
-                        pp[C + t * 8 + c2] = bs[t][0];
-                        pp[C + t * 8 + c2 + 1] = bs[t][1];
-                    }
             }
-            // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q - (beta e^gamma dR)^T K, one scale per row for both
-            const float last = tk[TOK_EG * C + C - 1];
-            float m0 = sd[0] * last * kStateFloor, m1 = sd[1] * last * kStateFloor;
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    const float eg = tk[TOK_EG * C + i];
-                    G[t][e] *= d.scale * eg * tk[TOK_FQ * C + i];
-                    Y[t][e] *= -tk[TOK_BETA * C + i] * eg * tk[TOK_FK * C + i];
-                    if (e < 2) m0 = fmaxf(m0, fabsf(G[t][e]));
-                    else m1 = fmaxf(m1, fabsf(G[t][e]));
-                }
-            frag_scale(Y, up, dn, m0, m1);
-            const float s0 = last * up[0], s1 = last * up[1];
-#pragma unroll
-            for (int t = 0; t < KT; t++) {
-                S[t][0] *= s0; S[t][1] *= s0;
-                S[t][2] *= s1; S[t][3] *= s1;
-            }
-#pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(G[2 * kk], G[2 * kk + 1], up, a);
-                mma_row<2, NPK>(S, a, 0, DKP / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, st + ST::oQ + p * PK + wide_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
-                });
-                frag_pieces<2>(Y[2 * kk], Y[2 * kk + 1], up, a);
-                mma_row<2, NPK>(S, a, 0, DKP / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
-                });
-            }
-            // <S_0, dS_0> over the warp's columns
+        }
+        // <S_0, dS_0> over the warp's entries
+        if (on) {
             float an = 0.0f;
-            const float4* ps = (const float4*)d.Sf + fb * KT * 32 + lane;
+            const float4* ps = (const float4*)d.Sf + (fb * KT + w * KTW) * 32 + lane;
 #pragma unroll
-            for (int t = 0; t < KT; t++) {
-                S[t][0] *= dn[0]; S[t][1] *= dn[0];
-                S[t][2] *= dn[1]; S[t][3] *= dn[1];
+            for (int t = 0; t < KTW; t++) {
                 const float4 x = ps[t * 32];
                 an = fmaf(S[t][0], x.x, an);
                 an = fmaf(S[t][1], x.y, an);
@@ -246,20 +286,25 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
-            if (lane == 0) d.anchor[fb] = an;
+            if (lane == 0) d.anchor[fb * 4 + w] = an;
         }
-        __syncthreads();
+        if (c > 0) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) G[t][e] = Gn[t][e];
+            put_go();
+        }
     }
     if (d.dh0) {
 #pragma unroll
-        for (int t = 0; t < KT; t++)
+        for (int t = 0; t < KTW; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + c2 + (e & 1);
+                const int i = (w * KTW + t) * 8 + c2 + (e & 1);
                 if (i < d.dk && cok[e >> 1]) d.dh0[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
             }
     }
-    cp_wait<0>();
 }
 
 // ------------------------------------------------------------------ gradients without recurrence
@@ -348,7 +393,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         } else if (warp == 1 && (d.dg || d.dbeta)) {
             // gates: tokens lane and lane + 32
             double before = 0.0, anchor = 0.0;
-            for (int x = 0; x < d.units; x++) anchor += d.anchor[head * d.units + x];
+            for (int x = 0; x < d.units * 4; x++) anchor += d.anchor[head * d.units * 4 + x];
 #pragma unroll
             for (int h = 0; h < C / 32; h++) {
                 const int i = h * 32 + lane;
@@ -374,13 +419,13 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 before += __shfl_sync(0xffffffffu, s, 31);
             }
         }
-        const float* mx = d.mx + head * d.units * MX_ROWS;
+        const float* mx = d.mx + head * d.units * 4 * MX_ROWS;
         float uS, sS, uU, sU, uG, sG, uR, sR, uD, sD;
-        units_scale(mx, d.units, MX_S, uS, sS);
-        units_scale(mx, d.units, MX_U, uU, sU);
-        units_scale(mx, d.units, MX_DO, uG, sG);
-        units_scale(mx, d.units, MX_R, uR, sR);
-        units_scale(mx, d.units, MX_DS, uD, sD);
+        units_scale(mx, d.units * 4, MX_S, uS, sS);
+        units_scale(mx, d.units * 4, MX_U, uU, sU);
+        units_scale(mx, d.units * 4, MX_DO, uG, sG);
+        units_scale(mx, d.units * 4, MX_R, uR, sR);
+        units_scale(mx, d.units * 4, MX_DS, uD, sD);
 
         float dP[4][4], dA[4][4], q1[HT][4], z1[HT][4], k1[HT][4];
 #pragma unroll
@@ -632,16 +677,25 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     }
 }
 
-template <int DKP, typename IO>
+template <int DKP, typename IO, int NU>
 cudaError_t chain_go(const DeltaDesc& d, cudaStream_t st) {
-    using ST = DeltaStage<kDeltaC, DKP, sizeof(IO) == 4 ? 2 : 1, 2>;
-    const int nw = delta_warps(d);
-    auto kern = delta_chain_bwd_kernel<DKP, IO>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ST::BYTES);
+    constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
+    using ST = DeltaStage<C, DKP, NPK, 2>;
+    constexpr int EX = FragBuf<DKP / 16, 2>::BYTES + 3 * FragBuf<C / 16, 2>::BYTES + FragBuf<C / 16, NPK>::BYTES;
+    constexpr int SMEM = 2 * ST::BYTES + NU * EX;
+    auto kern = delta_chain_bwd_kernel<DKP, IO, NU>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    const long long blocks = (long long)d.nseq * d.Hv * ((d.units + nw - 1) / nw);
-    kern<<<(unsigned)blocks, 32 * nw, 2 * ST::BYTES, st>>>(d, nw);
+    const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
+    kern<<<(unsigned)blocks, 128 * NU, SMEM, st>>>(d);
     return cudaGetLastError();
+}
+template <int DKP, typename IO>
+cudaError_t chain_pick(const DeltaDesc& d, cudaStream_t st) {
+    if constexpr (!(DKP == 128 && sizeof(IO) == 4)) {
+        if (delta_units(d) > 1) return chain_go<DKP, IO, 2>(d, st);
+    }
+    return chain_go<DKP, IO, 1>(d, st);
 }
 template <int DKP, typename IO>
 cudaError_t grads_go(const DeltaDesc& d, cudaStream_t st) {
@@ -657,8 +711,8 @@ cudaError_t grads_go(const DeltaDesc& d, cudaStream_t st) {
 }  // namespace
 
 cudaError_t delta_chain_bwd(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st) {
-    if (bf16) return DKP == 64 ? chain_go<64, __nv_bfloat16>(d, st) : chain_go<128, __nv_bfloat16>(d, st);
-    return DKP == 64 ? chain_go<64, float>(d, st) : chain_go<128, float>(d, st);
+    if (bf16) return DKP == 64 ? chain_pick<64, __nv_bfloat16>(d, st) : chain_pick<128, __nv_bfloat16>(d, st);
+    return DKP == 64 ? chain_pick<64, float>(d, st) : chain_pick<128, float>(d, st);
 }
 cudaError_t delta_grads(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st) {
     if (bf16) return DKP == 64 ? grads_go<64, __nv_bfloat16>(d, st) : grads_go<128, __nv_bfloat16>(d, st);

@@ -1,243 +1,270 @@
-// delta_fwd.cu -- gated delta rule, forward recurrence over chunks.
-//
-// The columns of the state evolve independently, so a warp owns 16 of them and
-// keeps the transposed state S^T [16 columns of dv][dk] in registers as
-// accumulators of m16n8 products.  Transposed, every product of a chunk takes
-// its fp32 factor from the registers of the same warp (an accumulator tile is
-// laid out as an A operand) and its other factor from shared memory:
-//   (K S)^T = S^T K^T;  W^T = (V - e^gamma K S)^T M^T;  U = beta W;  O^T = e^gamma S^T Q^T + U^T P^T
-//   S^T <- e^gamma_C S^T + (G_C. U)^T K
-// so the chain of a chunk needs no exchange between warps; the block's warps
-// only share the staged tiles (cp.async, two stages, one chunk ahead).
+// delta_fwd.cu -- gated delta rule, forward recurrence over chunks
+// (kmb_delta.cuh: a unit of 16 columns of dv, four warps):
+//   X = V - e^gamma K S;  W = M X;  U = beta W;  O = scale (e^gamma Q S + P U);  S <- e^gamma_C S + K^T (G_C. U)
+// all transposed.  The chain of a chunk is latency: three products that each wait
+// for the last, with fp16 pieces made and passed on between them.
 #include "kmb_delta.cuh"
 
 namespace kmb {
 namespace {
 
-template <int DKP, typename IO, bool KEEP>
-__global__ void __launch_bounds__(128, 2)
-delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int nw) {
+template <int DKP, typename IO, bool KEEP, int NU>
+__global__ void __launch_bounds__(128 * NU, 2 / NU)
+delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NPK = F32 ? 2 : 1;
     constexpr int NPO = (F32 || KEEP) ? 2 : 1;   // pieces behind o: it is rounded to bf16 unless it is kept in fp32
     using ST = DeltaStage<C, DKP, NPK, NPO>;
-    constexpr int NT = C / 8, KT = DKP / 8;
+    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;   // dk tiles, of a warp; its blocks of 16
     constexpr int PK = C * DKP * 2;              // bytes of a K or Q piece
+    using FS = FragBuf<DKP / 16, 2>;
+    using FX = FragBuf<C / 16, 2>;
+    using FO = FragBuf<C / 16, NPO>;
+    constexpr int EX = FS::BYTES + 2 * FX::BYTES + FO::BYTES;   // exchange buffers of a unit
     extern __shared__ __align__(128) unsigned char sm[];
+    __shared__ __align__(8) uint64_t full[2];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ub = (d.units + nw - 1) / nw;
-    const int u = (int)(blockIdx.x % ub) * nw + warp;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 2, w = warp & 3;
+    unsigned char* exS = sm + 2 * ST::BYTES + grp * EX;
+    unsigned char *exX = exS + FS::BYTES, *exU = exX + FX::BYTES, *exO = exU + FX::BYTES;
+    const int ub = (d.units + NU - 1) / NU;
+    const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, n = (int)(blockIdx.x / ub) / d.Hv;
-    const bool on = u < d.units;            // warps past dv only help with the copies
+    const bool on = u < d.units;                 // a unit past dv computes on zeros and stores nothing
     const int r = lane >> 2, c2 = (lane & 3) * 2;
     const int col[2] = {u * 16 + r, u * 16 + r + 8};
-    const bool cok[2] = {on && col[0] < d.dv, on && col[1] < d.dv};
+    const bool cok[2] = {col[0] < d.dv, col[1] < d.dv};
     const int ldv = (int)d.ld_v, ldo = (int)d.ld_o;
     long long start, len;
     seq_range(d, n, start, len);
     const int chunk0 = d.cu ? d.cstart[n] : n * d.nc;
     const int nch = (int)((len + C - 1) / C);
 
-    float S[KT][4];
+    float S[KTW][4];
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
 #pragma unroll
-    for (int t = 0; t < KT; t++)
+    for (int t = 0; t < KTW; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int i = t * 8 + c2 + (e & 1);
+            const int i = (w * KTW + t) * 8 + c2 + (e & 1);
             S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
-
-    if (nch > 0) ST::load(d, d.Mt, sb, chunk0, hv);
-    cp_commit();
-    for (int c = 0; c < nch; c++) {
-        if (c + 1 < nch) ST::load(d, d.Mt, sb + ((c + 1) & 1) * ST::BYTES, chunk0 + c + 1, hv);
-        cp_commit();
-        const long long tok0 = start + (long long)c * C;
-        const int cnt = (int)(len - (long long)c * C < C ? len - (long long)c * C : C);
-        // v of this chunk as accumulator tiles [16 columns][C tokens]; in flight under the first product
-        float V[NT][4];
-        {
-            const IO* pv = (const IO*)d.v + tok0 * d.ld_v + (long long)hv * d.dv + col[0];
+    // v of the warp's tokens of chunk c as accumulator tiles [16 columns][16 tokens]
+    const auto load_v = [&](int c, float (&V)[2][4]) {
+        const long long t0 = (long long)c * C + w * 16;
+        const IO* p = (const IO*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    V[t][e] = (i < cnt && cok[e >> 1]) ? ldt(pv + (long long)i * ldv, (e >> 1) * 8) : 0.0f;
-                }
-        }
-        cp_wait<1>();
-        __syncthreads();
-        const uint32_t st = sb + (c & 1) * ST::BYTES;
-        const float* tk = (const float*)(sm + (c & 1) * ST::BYTES + ST::oTok);
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        if (on) {
-            if (KEEP) {
-                float4* p = (float4*)d.Sf + fb * KT * 32 + lane;
-#pragma unroll
-                for (int t = 0; t < KT; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
-            }
-            float X[NT][4], O[NT][4], up[2], dn[2];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) X[t][e] = O[t][e] = 0.0f;
-            frag_scale(S, up, dn);
-            const float sd[2] = {dn[0], dn[1]};
-            if (KEEP) {
-                const float m = warp_down(dn);
-                if (lane == 0) d.mx[fb * MX_ROWS + MX_S] = m;
-            }
-#pragma unroll
-            for (int kk = 0; kk < DKP / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(S[2 * kk], S[2 * kk + 1], up, a);
-                const auto ldk = [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4(b, st + p * PK + wide_off<C>(t2 * 16 + lb_row(lane), kk * 16 + lb_col(lane)));
-                };
-                const auto ldq = [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4(b, st + ST::oQ + p * PK + wide_off<C>(t2 * 16 + lb_row(lane), kk * 16 + lb_col(lane)));
-                };
-                mma_row<2, NPK>(X, a, 0, C / 16, ldk);
-                mma_row<NPO, NPK>(O, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, C / 16, ldq);
-            }
-            // right-hand side v - e^gamma K S, and e^gamma Q S
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    const float eg = tk[TOK_EG * C + i] * dn[e >> 1];
-                    X[t][e] = V[t][e] - eg * tk[TOK_FK * C + i] * X[t][e];
-                    O[t][e] *= eg * tk[TOK_FQ * C + i];
-                }
-            // W^T = X M^T: row i of M reaches columns j <= i only
-            float U[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) U[t][e] = 0.0f;
-            frag_scale(X, up, dn);
-#pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(X[2 * kk], X[2 * kk + 1], up, a);
-                mma_row<2, 2>(U, a, kk, C / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4(b, st + ST::oT + p * ST::TT + tile_off<C>(t2 * 16 + lb_row(lane), kk * 16 + lb_col(lane)));
-                });
-            }
-            const float ft = tk[TOK_MISC * C], fp = tk[TOK_MISC * C + 1];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) U[t][e] *= ft * dn[e >> 1];
-            if (KEEP) {
-                float4* p = (float4*)d.Wf + fb * NT * 32 + lane;
-#pragma unroll
-                for (int t = 0; t < NT; t++) p[t * 32] = make_float4(U[t][0], U[t][1], U[t][2], U[t][3]);
-            }
-            // U = beta W
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    U[t][e] *= tk[TOK_BETA * C + t * 8 + c2 + (e & 1)];
-                    X[t][e] = 0.0f;
-                }
-            // O^T += U^T P^T
-            frag_scale(U, up, dn);
-            if (KEEP) {
-                const float m = warp_down(dn);
-                if (lane == 0) d.mx[fb * MX_ROWS + MX_U] = m;
-            }
-#pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[NPO][4];
-                frag_pieces<NPO>(U[2 * kk], U[2 * kk + 1], up, a);
-                mma_row<NPO, NPO>(X, a, kk, C / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4(b, st + ST::oP + p * ST::TT + tile_off<C>(t2 * 16 + lb_row(lane), kk * 16 + lb_col(lane)));
-                });
-            }
-            IO* po = (IO*)d.o + tok0 * d.ld_o + (long long)hv * d.dv + col[0];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    O[t][e] = d.scale * fmaf(X[t][e], fp * dn[e >> 1], O[t][e]);
-                    if (i < cnt && cok[e >> 1]) stt(po + (long long)i * ldo, (e >> 1) * 8, O[t][e]);
-                }
-                if (KEEP) *((float4*)d.Of + (fb * NT + t) * 32 + lane) = make_float4(O[t][0], O[t][1], O[t][2], O[t][3]);
-            }
-            // S^T <- e^gamma_C S^T + (G_C. U)^T K
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    U[t][e] *= tk[TOK_GC * C + i] * tk[TOK_FK * C + i];
-                }
-            // The state takes the scale of U for the product and comes back after it (powers of two).  A U below
-            // 2^-40 of the state is scaled as if it were that large, so the state does not overflow.
-            const float last = tk[TOK_EG * C + C - 1];
-            frag_scale(U, up, dn, sd[0] * last * kStateFloor, sd[1] * last * kStateFloor);
-            const float s0 = last * up[0], s1 = last * up[1];
-#pragma unroll
-            for (int t = 0; t < KT; t++) {
-                S[t][0] *= s0; S[t][1] *= s0;
-                S[t][2] *= s1; S[t][3] *= s1;
-            }
-#pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[2][4];
-                frag_pieces<2>(U[2 * kk], U[2 * kk + 1], up, a);
-                mma_row<2, NPK>(S, a, 0, DKP / 16, [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), t2 * 16 + la_col(lane)));
-                });
-            }
-#pragma unroll
-            for (int t = 0; t < KT; t++) {
-                S[t][0] *= dn[0]; S[t][1] *= dn[0];
-                S[t][2] *= dn[1]; S[t][3] *= dn[1];
-            }
-        }
-        __syncthreads();   // the stage is free for the chunk after the next
-    }
-    if (d.hT) {
-#pragma unroll
-        for (int t = 0; t < KT; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + c2 + (e & 1);
+                V[t][e] = (t0 + i < len && cok[e >> 1]) ? ldt(p + (long long)i * ldv, (e >> 1) * 8) : 0.0f;
+            }
+    };
+    float sup[2], sdn[2];
+    const auto put_state = [&]() {
+        frag_scale(S, sup, sdn);
+#pragma unroll
+        for (int b = 0; b < KBW; b++) FS::put(exS, w * KBW + b, lane, S[2 * b], S[2 * b + 1], sup, sdn);
+    };
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&full[0]), 1);
+        mbar_init(smem_u32(&full[1]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (nch > 0) ST::load(d, d.Mt, sb, smem_u32(&full[0]), chunk0, hv);
+    }
+    put_state();
+    __syncthreads();
+    float Vn[2][4];
+    if (nch > 0) load_v(0, Vn);
+    for (int c = 0; c < nch; c++) {
+        const bool got = mbar_wait(smem_u32(&full[c & 1]), (c >> 1) & 1);
+        // the state's fragments and this chunk's tiles are there; the other stage is read
+        if (!__syncthreads_and(got)) {
+            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            return;
+        }
+        if (threadIdx.x == 0 && c + 1 < nch)
+            ST::load(d, d.Mt, sb + ((c + 1) & 1) * ST::BYTES, smem_u32(&full[(c + 1) & 1]), chunk0 + c + 1, hv);
+        float V[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) V[t][e] = Vn[t][e];
+        if (c + 1 < nch) load_v(c + 1, Vn);
+        const uint32_t st = sb + (c & 1) * ST::BYTES;
+        const float* tk = (const float*)(sm + (c & 1) * ST::BYTES + ST::oTok);
+        const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
+        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+        if (KEEP && on) {
+            float4* p = (float4*)d.Sf + (fb * KT + w * KTW) * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < KTW; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
+            const float m = warp_down(sdn);
+            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = m;
+        }
+        float X[2][4], O[2][4], part[2][4], dn[2], up[2];
+        zero(X);
+        zero(O);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            float po[2][4];
+            zero(part);
+            zero(po);
+#pragma unroll
+            for (int b = 0; b < KBW; b++) {
+                const int kk = s * KBW + b;
+                uint32_t a[2][4];
+                FS::template get<2>(exS, kk, lane, a);
+                const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
+                mma_row<NPO, NPK>(po, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
+                                  [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oQ + p * PK + o); });
+            }
+            FS::scale(exS, s * KBW, lane, dn);
+            add_scaled(X, part, dn);
+            add_scaled(O, po, dn);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                const float eg = tw[TOK_EG * C + i];
+                X[t][e] = V[t][e] - eg * tw[TOK_FK * C + i] * X[t][e];
+                O[t][e] *= eg * tw[TOK_FQ * C + i];
+            }
+        frag_scale(X, up, dn);
+        FX::put(exX, w, lane, X[0], X[1], up, dn);
+        unit_bar(grp);
+        // W^T = X M^T: row i of M reaches columns j <= i only
+        float W[2][4];
+        zero(W);
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            if (kk > w) continue;
+            uint32_t a[2][4];
+            FX::template get<2>(exX, kk, lane, a);
+            FX::scale(exX, kk, lane, dn);
+            const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+            zero(part);
+            mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
+            add_scaled(W, part, dn);
+        }
+        const float fm = tk[TOK_MISC * C], fp = tk[TOK_MISC * C + 1];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) W[t][e] *= fm;
+        if (KEEP && on) {
+            float4* p = (float4*)d.Wf + (fb * (C / 8) + w * 2) * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < 2; t++) p[t * 32] = make_float4(W[t][0], W[t][1], W[t][2], W[t][3]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
+        frag_scale(W, up, dn);
+        FO::put(exO, w, lane, W[0], W[1], up, dn);
+        if (KEEP && on) {
+            const float m = warp_down(dn);
+            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_U] = m;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                W[t][e] *= tw[TOK_GC * C + i] * tw[TOK_FK * C + i];
+            }
+        frag_scale(W, up, dn);
+        FX::put(exU, w, lane, W[0], W[1], up, dn);
+        unit_bar(grp);
+        // S^T <- e^gamma_C S^T + (G_C. U)^T K
+        const float last = tk[TOK_EG * C + C - 1];
+#pragma unroll
+        for (int t = 0; t < KTW; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) S[t][e] *= last;
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            uint32_t a[2][4];
+            float ps[KTW][4];
+            FX::template get<2>(exU, kk, lane, a);
+            FX::scale(exU, kk, lane, dn);
+            zero(ps);
+            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+            });
+            add_scaled(S, ps, dn);
+        }
+        put_state();
+        // O^T += U^T P^T
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {
+            if (kk > w) continue;
+            uint32_t a[NPO][4];
+            FO::template get<NPO>(exO, kk, lane, a);
+            FO::scale(exO, kk, lane, dn);
+            dn[0] *= fp;
+            dn[1] *= fp;
+            const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+            zero(part);
+            mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });
+            add_scaled(O, part, dn);
+        }
+        const long long t0 = (long long)c * C + w * 16;
+        IO* po = (IO*)d.o + (start + t0) * d.ld_o + (long long)hv * d.dv + col[0];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + c2 + (e & 1);
+                O[t][e] *= d.scale;
+                if (t0 + i < len && cok[e >> 1]) stt(po + (long long)i * ldo, (e >> 1) * 8, O[t][e]);
+            }
+            if (KEEP && on)
+                *((float4*)d.Of + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(O[t][0], O[t][1], O[t][2], O[t][3]);
+        }
+    }
+    if (d.hT) {
+#pragma unroll
+        for (int t = 0; t < KTW; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = (w * KTW + t) * 8 + c2 + (e & 1);
                 if (i < d.dk && cok[e >> 1]) d.hT[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
             }
     }
-    cp_wait<0>();
 }
 
-template <int DKP, typename IO, bool KEEP>
+template <int DKP, typename IO, bool KEEP, int NU>
 cudaError_t go(const DeltaDesc& d, cudaStream_t st) {
-    constexpr bool F32 = sizeof(IO) == 4;
-    using ST = DeltaStage<kDeltaC, DKP, F32 ? 2 : 1, (F32 || KEEP) ? 2 : 1>;
-    const int nw = delta_warps(d);
-    auto kern = delta_chain_fwd_kernel<DKP, IO, KEEP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ST::BYTES);
+    constexpr int C = kDeltaC, NPO = (sizeof(IO) == 4 || KEEP) ? 2 : 1;
+    using ST = DeltaStage<C, DKP, sizeof(IO) == 4 ? 2 : 1, NPO>;
+    constexpr int EX = FragBuf<DKP / 16, 2>::BYTES + 2 * FragBuf<C / 16, 2>::BYTES + FragBuf<C / 16, NPO>::BYTES;
+    constexpr int SMEM = 2 * ST::BYTES + NU * EX;
+    auto kern = delta_chain_fwd_kernel<DKP, IO, KEEP, NU>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    const long long blocks = (long long)d.nseq * d.Hv * ((d.units + nw - 1) / nw);
-    kern<<<(unsigned)blocks, 32 * nw, 2 * ST::BYTES, st>>>(d, nw);
+    const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
+    kern<<<(unsigned)blocks, 128 * NU, SMEM, st>>>(d);
     return cudaGetLastError();
 }
-template <typename IO>
-cudaError_t pick(const DeltaDesc& d, int DKP, bool keep, cudaStream_t st) {
-    if (DKP == 64) return keep ? go<64, IO, true>(d, st) : go<64, IO, false>(d, st);
-    return keep ? go<128, IO, true>(d, st) : go<128, IO, false>(d, st);
+template <int DKP, typename IO>
+cudaError_t pick(const DeltaDesc& d, bool keep, cudaStream_t st) {
+    // two units with fp32 tiles of dk = 128 exceed the shared memory of a block
+    if constexpr (!(DKP == 128 && sizeof(IO) == 4)) {
+        if (delta_units(d) > 1) return keep ? go<DKP, IO, true, 2>(d, st) : go<DKP, IO, false, 2>(d, st);
+    }
+    return keep ? go<DKP, IO, true, 1>(d, st) : go<DKP, IO, false, 1>(d, st);
 }
 }  // namespace
 
 cudaError_t delta_chain_fwd(const DeltaDesc& d, int DKP, bool bf16, bool keep, cudaStream_t st) {
-    return bf16 ? pick<__nv_bfloat16>(d, DKP, keep, st) : pick<float>(d, DKP, keep, st);
+    if (bf16) return DKP == 64 ? pick<64, __nv_bfloat16>(d, keep, st) : pick<128, __nv_bfloat16>(d, keep, st);
+    return DKP == 64 ? pick<64, float>(d, keep, st) : pick<128, float>(d, keep, st);
 }
 }  // namespace kmb

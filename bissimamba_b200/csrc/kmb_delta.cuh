@@ -26,6 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include "kmb_sync.cuh"
 
 namespace kmb {
 
@@ -64,13 +65,14 @@ struct DeltaDesc {
     // kept for the backward; "fragment order": [nch][Hv][units][tiles][32 lanes][4]
     float *Sf, *Wf, *Of;         // state at the chunk's start, W, O
     float *Rf, *dSf;             // backward: dR = T^T dU, adjoint of the state at the chunk's end
-    float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units]
-    float* mx;                   // [nch][Hv][units][MX_ROWS]: down-scale of the largest entry of S, U, dO, dR, dS
+    float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units][4 warps]
+    float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: down-scale of the largest entry of S, U, dO, dR, dS
     // gradients
     const void* go;
     const float* dhT;
     void *dq, *dkk, *dvv;
     float *dg, *dbeta, *dh0;
+    int* status;
     long long ld_do, ld_dq, ld_dk, ld_dv;
 };
 
@@ -96,7 +98,7 @@ __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -248,48 +250,97 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared-memory stage of the chunk recurrences: K, Q tiles, pieces of M (or T) and P, token factors
+// ------------------------------------------------------------------ chunk recurrences
+// A unit is 16 columns of dv of one head; four warps work on it, one per SM sub-partition.  Transposed, the state
+// S^T [16][dk] is an m16 product's accumulator: warp w keeps the quarter w of dk in registers, and owns the tokens
+// 16 w .. 16 w + 15 of a chunk.  What all four need (the state, then the chunk's right-hand side, then U) goes
+// through shared memory as fp16 A fragments, 16 columns of k at a time, each with a power of two per row, so no
+// warp waits for another's row maximum: the products of a block of k are summed apart and added in fp32.
+// Three barriers a chunk.  A block holds NU units that share the staged tiles.
 template <int C, int DKP, int NPK, int NPP>
 struct DeltaStage {
     static constexpr int KQ = NPK * C * DKP * 2;   // bytes of K (and of Q)
-    static constexpr int TT = C * C * 2;           // one piece of T or P
+    static constexpr int TT = C * C * 2;           // one piece of M, T or P
     static constexpr int oQ = KQ, oT = 2 * KQ, oP = oT + 2 * TT, oTok = oP + NPP * TT;
-    static constexpr int BYTES = oTok + TOK_ROWS * C * 4;
+    static constexpr int TOK = TOK_ROWS * C * 4;
+    static constexpr int BYTES = oTok + TOK;
 
-    // copies of one chunk into the stage at `dst`, T or M from `tiles`; of it and of P only what lies on or below the diagonal blocks
-    static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t dst, int chunk,
-                                                int hv) {
+    // one thread: bulk copies of one chunk into the stage at `dst`, M or T from `tiles`
+    static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t dst, uint32_t bar,
+                                                int chunk, int hv) {
         const int hk = hv / d.grp;
-        const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
-        const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
-        for (int i = threadIdx.x; i < KQ / 16; i += blockDim.x) {
-            cp16(dst + i * 16, ks + i * 16);
-            cp16(dst + oQ + i * 16, qs + i * 16);
-        }
-        const size_t th = ((size_t)chunk * d.Hv + hv) * 2 * C * C;
-        const char *ts = (const char*)(tiles + th), *ps = (const char*)(d.Pt + th);
-        constexpr int CPR = C / 8;   // 16-byte pieces per row
-        for (int i = threadIdx.x; i < C * CPR; i += blockDim.x) {
-            const int r = i / CPR, c8 = i % CPR;
-            if (c8 > 2 * (r >> 4) + 1) continue;
-            const uint32_t o = tile_off<C>(r, c8 * 8);
-#pragma unroll
-            for (int p = 0; p < 2; p++) {
-                cp16(dst + oT + p * TT + o, ts + p * TT + o);
-                if (p < NPP) cp16(dst + oP + p * TT + o, ps + p * TT + o);
-            }
-        }
-        const char* tk = (const char*)(d.tok + ((size_t)chunk * d.Hv + hv) * TOK_ROWS * C);
-        for (int i = threadIdx.x; i < TOK_ROWS * C / 4; i += blockDim.x) cp16(dst + oTok + i * 16, tk + i * 16);
+        const size_t kh = ((size_t)chunk * d.Hk + hk) * NPK * C * DKP, vh = (size_t)chunk * d.Hv + hv;
+        mbar_expect_tx(bar, BYTES);
+        bulk(dst, d.Kt + kh, KQ, bar);
+        bulk(dst + oQ, d.Qt + kh, KQ, bar);
+        bulk(dst + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
+        bulk(dst + oP, d.Pt + vh * 2 * C * C, NPP * TT, bar);
+        bulk(dst + oTok, d.tok + vh * TOK_ROWS * C, TOK, bar);
+    }
+    static __device__ __forceinline__ void bulk(uint32_t dst, const void* src, unsigned bytes, uint32_t bar) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
     }
 };
+
+// A fragments in shared memory: [block][piece][lane] 16 bytes, and per block the 16 rows' down-scales
+template <int NBLK, int NP>
+struct FragBuf {
+    static constexpr int BYTES = NBLK * (NP * 512 + 64);
+    static __device__ __forceinline__ void put(unsigned char* base, int blk, int lane, const float (&t0)[4],
+                                               const float (&t1)[4], const float (&up)[2], const float (&dn)[2]) {
+        uint32_t a[NP][4];
+        frag_pieces<NP>(t0, t1, up, a);
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+            *(uint4*)(base + (blk * NP + p) * 512 + lane * 16) = make_uint4(a[p][0], a[p][1], a[p][2], a[p][3]);
+        if ((lane & 3) == 0) {
+            float* s = (float*)(base + NBLK * NP * 512) + blk * 16;
+            s[lane >> 2] = dn[0];
+            s[(lane >> 2) + 8] = dn[1];
+        }
+    }
+    // first N of the block's pieces
+    template <int N>
+    static __device__ __forceinline__ void get(const unsigned char* base, int blk, int lane, uint32_t (&a)[N][4]) {
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            const uint4 v = *(const uint4*)(base + (blk * NP + p) * 512 + lane * 16);
+            a[p][0] = v.x; a[p][1] = v.y; a[p][2] = v.z; a[p][3] = v.w;
+        }
+    }
+    static __device__ __forceinline__ void scale(const unsigned char* base, int blk, int lane, float (&dn)[2]) {
+        const float* s = (const float*)(base + NBLK * NP * 512) + blk * 16;
+        dn[0] = s[lane >> 2];
+        dn[1] = s[(lane >> 2) + 8];
+    }
+};
+template <int N>
+__device__ __forceinline__ void zero(float (&t)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[i][e] = 0.0f;
+}
+// acc += part * f[row]
+template <int N>
+__device__ __forceinline__ void add_scaled(float (&acc)[N][4], const float (&part)[N][4], const float (&f)[2]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[i][e] = fmaf(part[i][e], f[e >> 1], acc[i][e]);
+}
+__device__ __forceinline__ void unit_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
+
+int delta_sms();
+// Units per block: one where every SM gets a unit at most (the chain of a chunk is bound by latency), two where
+// there are more units than SMs (they share the copies of the tiles).
+inline int delta_units(const DeltaDesc& d) {
+    return d.units > 1 && (long long)d.nseq * d.Hv * d.units > delta_sms() ? 2 : 1;
+}
 
 cudaError_t delta_chain_fwd(const DeltaDesc& d, int DKP, bool bf16, bool keep, cudaStream_t st);
 cudaError_t delta_chain_bwd(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st);
 cudaError_t delta_grads(const DeltaDesc& d, int DKP, bool bf16, cudaStream_t st);
-
-// Warps per block of the chunk recurrences (each owns 16 columns of dv): four, one per SM sub-partition, share
-// the staged tiles.
-inline int delta_warps(const DeltaDesc& d) { return d.units < 4 ? d.units : 4; }
 
 }  // namespace kmb
