@@ -63,15 +63,16 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             const int i = (w * KTW + t) * 8 + c2 + (e & 1);
             S[t][e] = (d.dhT && i < d.dk && cok[e >> 1]) ? d.dhT[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
-    const auto load_t = [&](const void* base, long long ld, int ldi, int c, float (&V)[2][4]) {
+    using RT = typename RawOf<IO>::type;
+    const auto load_t = [&](const void* base, long long ld, int ldi, int c, RT (&V)[2][4]) {
         const long long t0 = (long long)c * C + w * 16;
-        const IO* p = (const IO*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
+        const RT* p = (const RT*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + c2 + (e & 1);
-                V[t][e] = (t0 + i < len && cok[e >> 1]) ? ldt(p + (long long)i * ldi, (e >> 1) * 8) : 0.0f;
+                V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldi + (e >> 1) * 8] : RT(0);
             }
     };
     float sup[2], sdn[2], up[2], dn[2];
@@ -82,7 +83,12 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     };
     float G[2][4];   // dO^T of the warp's tokens
     float gdn[2];
+    RT Gn[2][4];   // the next chunk's
     const auto put_go = [&]() {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) G[t][e] = from_raw(Gn[t][e]);
         frag_scale(G, up, gdn);
         FG::put(exG, w, lane, G[0], G[1], up, gdn);
     };
@@ -93,9 +99,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         if (nch > 0) ST::load(d, d.Tt, sb, smem_u32(&full[0]), chunk0 + nch - 1, hv);
     }
     put_state();
-    float Gn[2][4];
     if (nch > 0) {
-        load_t(d.go, d.ld_do, ldg, nch - 1, G);
+        load_t(d.go, d.ld_do, ldg, nch - 1, Gn);
         put_go();
     }
     __syncthreads();
@@ -114,7 +119,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         const float* tw = tk + w * 16 + c2;
         const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
         // what the end of the chunk reads: in flight under the products
-        float V[2][4];
+        RT V[2][4];
         float4 w4[2], o4[2];
         load_t(d.v, d.ld_v, ldv, c, V);
 #pragma unroll
@@ -255,7 +260,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                     const float dv = tw[TOK_BETA * C + t * 8 + (e & 1)] * Y[t][e];
                     bs[t][e & 1] = fmaf(Y[t][e], ww[e], bs[t][e & 1]);
                     ts[t][e & 1] = fmaf(G[t][e], oo[e], ts[t][e & 1]);
-                    ts[t][e & 1] = fmaf(-V[t][e], dv, ts[t][e & 1]);
+                    ts[t][e & 1] = fmaf(-from_raw(V[t][e]), dv, ts[t][e & 1]);
                     if (t0 + i < len && cok[e >> 1]) stt(pd + (long long)i * lddv, (e >> 1) * 8, dv);
                 }
 #pragma unroll
@@ -288,13 +293,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
             if (lane == 0) d.anchor[fb * 4 + w] = an;
         }
-        if (c > 0) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) G[t][e] = Gn[t][e];
-            put_go();
-        }
+        if (c > 0) put_go();
     }
     if (d.dh0) {
 #pragma unroll

@@ -51,15 +51,16 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
         }
     // v of the warp's tokens of chunk c as accumulator tiles [16 columns][16 tokens]
-    const auto load_v = [&](int c, float (&V)[2][4]) {
+    using RT = typename RawOf<IO>::type;
+    const auto load_v = [&](int c, RT (&V)[2][4]) {
         const long long t0 = (long long)c * C + w * 16;
-        const IO* p = (const IO*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
+        const RT* p = (const RT*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + c2 + (e & 1);
-                V[t][e] = (t0 + i < len && cok[e >> 1]) ? ldt(p + (long long)i * ldv, (e >> 1) * 8) : 0.0f;
+                V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
             }
     };
     float sup[2], sdn[2];
@@ -76,7 +77,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     }
     put_state();
     __syncthreads();
-    float Vn[2][4];
+    RT Vn[2][4];
     if (nch > 0) load_v(0, Vn);
     for (int c = 0; c < nch; c++) {
         const bool got = mbar_wait(smem_u32(&full[c & 1]), (c >> 1) & 1);
@@ -87,7 +88,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         }
         if (threadIdx.x == 0 && c + 1 < nch)
             ST::load(d, d.Mt, sb + ((c + 1) & 1) * ST::BYTES, smem_u32(&full[(c + 1) & 1]), chunk0 + c + 1, hv);
-        float V[2][4];
+        RT V[2][4];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -132,7 +133,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + (e & 1);
                 const float eg = tw[TOK_EG * C + i];
-                X[t][e] = V[t][e] - eg * tw[TOK_FK * C + i] * X[t][e];
+                X[t][e] = from_raw(V[t][e]) - eg * tw[TOK_FK * C + i] * X[t][e];
                 O[t][e] *= eg * tw[TOK_FQ * C + i];
             }
         frag_scale(X, up, dn);

@@ -203,6 +203,11 @@ __device__ __forceinline__ void mma_row(float (&acc)[N][4], const uint32_t (&a)[
 
 __device__ __forceinline__ float ldt(const float* p, long long i) { return p[i]; }
 __device__ __forceinline__ float ldt(const __nv_bfloat16* p, long long i) { return __bfloat162float(p[i]); }
+// Values as they are in memory: converted where they are used, so a load that is in flight holds nobody up.
+template <typename IO> struct RawOf { using type = float; };
+template <> struct RawOf<__nv_bfloat16> { using type = unsigned short; };
+__device__ __forceinline__ float from_raw(float v) { return v; }
+__device__ __forceinline__ float from_raw(unsigned short v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ void stt(float* p, long long i, float v) { p[i] = v; }
 __device__ __forceinline__ void stt(__nv_bfloat16* p, long long i, float v) { p[i] = __float2bfloat16_rn(v); }
 
