@@ -60,29 +60,31 @@ __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ i
 // ------------------------------------------------------------------ per-chunk matrices
 // Block = (chunk, key head), four warps of 16 rows: the chunk's K and Q as swizzled fp16 tiles (zero behind the
 // last token and behind dk), K K^T and Q K^T once per key head; then for each of its value heads the token
-// factors, T (or M, see kmb_delta.cuh) and P in two fp16 pieces.  T comes from 16 x 16 diagonal blocks by forward
-// substitution, one column per lane, merged in pairs: [[a, 0], [c, b]]^-1 = [[a^-1, 0], [-b^-1 c a^-1, b^-1]].
-// The running sums of g are 64-bit: their differences are what G needs, after a reset (g = -inf, held at -104,
-// where exp is 0 in fp32) too.  M_ij = T_ij beta_j / beta_i; a beta of 0 is 2^-100 in both: T is then the same in
-// fp32, and the quotient is the one that the limit has.
-constexpr float kBetaTiny = 7.888609052210118e-31f;
+// factors, P, and the chunk's triangular system.  With a_ij = G_ij k_i.k_j (j < i) and
+//   C = (I + a diag(beta))^-1 a:   M = I - C diag(beta),   T = I - diag(beta) C
+// (no division: both are exact where beta is 0).  By blocks of 16, diagonal blocks by forward substitution, one
+// column per lane, then row block after row block
+//   C_IJ = M_II (a_IJ - sum_{J <= K < I} a_IK diag(beta_K) C_KJ)
+// on fp16 pieces: a warp holds its rows of a as accumulators, which are A fragments, and reads the finished C_K
+// from shared memory.
 
 template <int DKP, typename IO>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 3)
 delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NPK = F32 ? 2 : 1;
     constexpr int TILE = C * DKP * 2;                     // bytes of one piece
-    constexpr int LDA = C + 1;
     constexpr int G8 = DKP / 8;                           // threads per row of the tiles
+    constexpr int TT = C * C * 2;
     extern __shared__ __align__(128) unsigned char sm[];
     const uint32_t sK = (uint32_t)__cvta_generic_to_shared(sm), sQ = sK + NPK * TILE;
-    float* Am = (float*)(sm + 2 * NPK * TILE);
-    float* X = Am + C * LDA;
-    float* W = X + C * LDA;                               // [C / 2][LDA]
+    unsigned char* Csm = sm + 2 * NPK * TILE;             // C, two pieces
     __shared__ double gam[C];
-    __shared__ float bet[C], fK[C], fQ[C], red[3][4];
+    __shared__ float rowE[C], colE[3 * 48], bet[C], fK[C], fQ[C], fC[4];
+    __shared__ float dg[4][16][17];                       // diagonal blocks, per warp
+    __shared__ __align__(128) unsigned char Ysm[2 * 16 * 128];   // the row block in work, two pieces
+    const DecaySmem dec{gam, rowE, colE};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunk = blockIdx.x, hk = blockIdx.y;
     long long tok0;
@@ -156,155 +158,199 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
         mma_row<NPK, NPK>(kk, ak, 0, C / 16, ldb);
         mma_row<NPK, NPK>(qk, aq, 0, C / 16, ldb);
     }
+    const uint32_t sC = (uint32_t)__cvta_generic_to_shared(Csm), sY = (uint32_t)__cvta_generic_to_shared(Ysm);
     for (int hh = 0; hh < d.grp; hh++) {
         const int hv = hk * d.grp + hh;
         const size_t head = (size_t)chunk * d.Hv + hv;
         float* tk = d.tok + head * TOK_ROWS * C;
         __syncthreads();   // the last head's matrices are read
-        if (warp == 0) {   // running sums: lane holds tokens lane and lane + 32
-            double carry = 0.0;
-#pragma unroll
-            for (int h = 0; h < C / 32; h++) {
-                const int i = h * 32 + lane;
-                float g = (d.g && i < cnt) ? d.g[(tok0 + i) * d.Hv + hv] : 0.0f;
-                if (g < -104.0f) g = -104.0f;
-                double s = g;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double t = __shfl_up_sync(0xffffffffu, s, o);
-                    if (lane >= o) s += t;
-                }
-                s += carry;
-                gam[i] = s;
-                carry = __shfl_sync(0xffffffffu, s, 31);
-                float b = i < cnt ? (d.beta ? d.beta[(tok0 + i) * d.Hv + hv] : 1.0f) : 0.0f;
-                tk[TOK_EG * C + i] = expf((float)s);
-                tk[TOK_BETA * C + i] = b;
-                bet[i] = fabsf(b) < kBetaTiny ? kBetaTiny : b;
-                tk[TOK_FK * C + i] = fK[i];
-                tk[TOK_FQ * C + i] = fQ[i];
-            }
-            __syncwarp();
-#pragma unroll
-            for (int h = 0; h < C / 32; h++) {
-                const int i = h * 32 + lane;
-                tk[TOK_GC * C + i] = expf((float)(gam[C - 1] - gam[i]));
-            }
+        if (warp == 0) {
+            running_sums(d, tok0, cnt, hv, lane, gam);
+        } else if (warp < 3) {
+            const int i = threadIdx.x - 32;
+            const float b = i < cnt ? (d.beta ? d.beta[(tok0 + i) * d.Hv + hv] : 1.0f) : 0.0f;
+            bet[i] = b;
+            tk[TOK_BETA * C + i] = b;
+            tk[TOK_FK * C + i] = fK[i];
+            tk[TOK_FQ * C + i] = fQ[i];
         }
-        for (int i = threadIdx.x; i < C * LDA; i += 128) X[i] = 0.0f;
         __syncthreads();
-        float pv[C / 8][4], pm = 0.0f;
+        decay_tables(dec, threadIdx.x);
+        if (threadIdx.x < C) {
+            const int i = threadIdx.x;
+            tk[TOK_EG * C + i] = expf((float)gam[i]);
+            tk[TOK_GC * C + i] = expf((float)(gam[C - 1] - gam[i]));
+        }
+        __syncthreads();
+        // rows of a and P on and below the warp's diagonal block
+        float A[C / 8][4], B[C / 8][4], pm = 0.0f;
 #pragma unroll
-        for (int t = 0; t < C / 8; t++)
+        for (int t = 0; t < C / 8; t++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) A[t][e] = B[t][e] = 0.0f;
+            if ((t >> 1) > rg) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = rg * 16 + r + (e >> 1) * 8, j = t * 8 + c2 + (e & 1);
-                const float G = j <= i ? expf((float)(gam[i] - gam[j])) * fK[j] : 0.0f;
-                pv[t][e] = j <= i ? G * fQ[i] * qk[t][e] : 0.0f;
-                pm = fmaxf(pm, fabsf(pv[t][e]));
-                Am[i * LDA + j] = j < i ? bet[i] * G * fK[i] * kk[t][e] : 0.0f;
-            }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, o));
-        if (lane == 0) red[0][warp] = pm;
-        __syncthreads();
-        if (lane < 16) {   // column `lane` of the inverse of diagonal block `warp`
-            const int b0 = warp * 16;
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float s = i == lane ? 1.0f : 0.0f;
-#pragma unroll
-                for (int j = 0; j < i; j++) s = fmaf(-Am[(b0 + i) * LDA + b0 + j], x[j], s);
-                x[i] = s;
-                X[(b0 + i) * LDA + b0 + lane] = s;
+                const float G = dec.at(i, j, (t >> 1) == rg, rg) * fK[j];
+                B[t][e] = G * fQ[i] * qk[t][e];
+                pm = fmaxf(pm, fabsf(B[t][e]));
+                A[t][e] = j < i ? G * fK[i] * kk[t][e] : 0.0f;
             }
         }
-        float pup, pdown;
-        row_scale(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), pup, pdown);
-        char* gP = (char*)(d.Pt + head * 2 * C * C);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, o));
+        float up, down;
+        row_scale(pm, up, down);
+        if (lane == 0) tk[TOK_MISC * C + 4 + rg] = down;
+        const auto put = [&](char* g, const float (&x)[C / 8][4], float s, bool shared) {
+#pragma unroll
+            for (int t = 0; t < C / 8; t++) {
+                if ((t >> 1) > rg) continue;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[2];
+                    split_pair<2>(x[t][h * 2] * s, x[t][h * 2 + 1] * s, p);
+                    const uint32_t o = tile_off<C>(rg * 16 + r + h * 8, t * 8 + c2);
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        if (shared) *(uint32_t*)(Csm + k * TT + o) = p[k];
+                        if (g) *(uint32_t*)(g + k * TT + o) = p[k];
+                    }
+                }
+            }
+        };
+        put((char*)(d.Pt + head * 2 * C * C), B, up, false);
+        // C_II: the diagonal block through shared memory, column `lane` of the solution, back as accumulator tiles
+#pragma unroll
+        for (int t = 0; t < C / 8; t++)
+            if ((t >> 1) == rg) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    dg[warp][r + (e >> 1) * 8][(t & 1) * 8 + c2 + (e & 1)] = A[t][e];
+                    A[t][e] = 0.0f;
+                }
+            }
+        __syncwarp();
+        {
+            float x[16], xb[16];   // the column, and beta times it
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float s = dg[warp][i][lane & 15];
+#pragma unroll
+                for (int j = 0; j < i; j++) s = fmaf(-dg[warp][i][j], xb[j], s);
+                x[i] = s;
+                xb[i] = s * bet[warp * 16 + i];
+            }
+            __syncwarp();
+            if (lane < 16) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) dg[warp][i][lane] = x[i];
+            }
+            __syncwarp();
+        }
+        float S[C / 8][4], md[2][4];   // the warp's rows of C; M_II
 #pragma unroll
         for (int t = 0; t < C / 8; t++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t p[2];
-                split_pair<2>(pv[t][h * 2] * pup, pv[t][h * 2 + 1] * pup, p);
-                const uint32_t o = tile_off<C>(rg * 16 + r + h * 8, t * 8 + c2);
+            for (int e = 0; e < 4; e++)
+                S[t][e] = (t >> 1) == rg ? dg[warp][r + (e >> 1) * 8][(t & 1) * 8 + c2 + (e & 1)] : 0.0f;
 #pragma unroll
-                for (int k = 0; k < 2; k++) *(uint32_t*)(gP + k * (C * C * 2) + o) = p[k];
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = r + (e >> 1) * 8, j = t * 8 + c2 + (e & 1);
+                md[t][e] = (i == j ? 1.0f : 0.0f) - dg[warp][i][j] * bet[warp * 16 + j];
             }
-        __syncthreads();
+        for (int I = 0; I < 4; I++) {
+            if (warp == I) {
+                if (I > 0) {
+                    float Y[6][4], aup[2], adn[2], part[6][4];
 #pragma unroll
-        for (int s = 16; s < C; s *= 2) {
-            // thread: one row, a run of columns, of the block below each pair of inverted blocks
-            const int pairs = C / (2 * s), run = pairs * s * s / 128;
-            const int e0 = threadIdx.x * run, pr = e0 / (s * s), i = (e0 / s) % s, j0 = e0 % s;
-            const int b0 = pr * 2 * s;
-            float acc[8];
+                    for (int t = 0; t < 6; t++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) acc[e] = 0.0f;
-            for (int m = 0; m < s; m++) {
-                const float a = Am[(b0 + s + i) * LDA + b0 + m];
+                        for (int e = 0; e < 4; e++) {
+                            Y[t][e] = A[t][e];
+                            A[t][e] *= bet[t * 8 + c2 + (e & 1)];
+                        }
+                    frag_scale(A, aup, adn);
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (e < run) acc[e] = fmaf(a, X[(b0 + m) * LDA + b0 + j0 + e], acc[e]);
+                    for (int K = 0; K < 3; K++) {
+                        if (K >= I) continue;
+                        uint32_t a[2][4];
+                        frag_pieces<2>(A[2 * K], A[2 * K + 1], aup, a);
+                        zero(part);
+                        mma_row<2, 2>(part, a, 0, K + 1, [&](int p, int t2, uint32_t (&b)[4]) {
+                            ldm4t(b, sC + p * TT + tile_off<C>(K * 16 + la_row(lane), t2 * 16 + la_col(lane)));
+                        });
+                        const float f[2] = {-adn[0] * fC[K], -adn[1] * fC[K]};
+                        add_scaled(Y, part, f);
+                    }
+                    float yup[2], ydn[2];
+                    frag_scale(Y, yup, ydn);
+                    const float ym = warp_down(ydn), yu = 1.0f / ym;
+#pragma unroll
+                    for (int t = 0; t < 6; t++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            uint32_t p[2];
+                            split_pair<2>(Y[t][h * 2] * yu, Y[t][h * 2 + 1] * yu, p);
+                            const uint32_t o = tile_off<C>(r + h * 8, t * 8 + c2);
+#pragma unroll
+                            for (int k = 0; k < 2; k++) *(uint32_t*)(Ysm + k * 2048 + o) = p[k];
+                        }
+                    __syncwarp();
+                    uint32_t a[2][4];
+                    frag_scale(md, aup, adn);
+                    frag_pieces<2>(md[0], md[1], aup, a);
+                    zero(part);
+                    mma_row<2, 2>(part, a, 0, 3, [&](int p, int t2, uint32_t (&b)[4]) {
+                        ldm4t(b, sY + p * 2048 + tile_off<C>(la_row(lane), t2 * 16 + la_col(lane)));
+                    });
+#pragma unroll
+                    for (int t = 0; t < 6; t++)
+                        if ((t >> 1) < rg) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) S[t][e] = part[t][e] * adn[e >> 1] * ym;
+                        }
+                }
+                if (I < 3) {
+                    float cup[2], cdn[2];
+                    frag_scale(S, cup, cdn);
+                    const float m = warp_down(cdn);
+                    if (lane == 0) fC[I] = m;
+                    put(nullptr, S, 1.0f / m, true);
+                }
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e < run) W[(pr * s + i) * LDA + j0 + e] = acc[e];
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 8; e++) acc[e] = 0.0f;
-            for (int m = 0; m <= i; m++) {
-                const float a = X[(b0 + s + i) * LDA + b0 + s + m];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (e < run) acc[e] = fmaf(-a, W[(pr * s + m) * LDA + j0 + e], acc[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e < run) X[(b0 + s + i) * LDA + b0 + j0 + e] = acc[e];
             __syncthreads();
         }
+        // T = I - diag(beta) C, M = I - C diag(beta): the warp's rows, one power of two each
         float tm = 0.0f, mm = 0.0f;
-        for (int i = threadIdx.x; i < C * C; i += 128) {
-            const int row = i / C, cc = i % C;
-            const float x = fabsf(X[row * LDA + cc]);
-            tm = fmaxf(tm, x);
-            mm = fmaxf(mm, x * fabsf(bet[cc] / bet[row]));
+#pragma unroll
+        for (int t = 0; t < C / 8; t++) {
+            if ((t >> 1) > rg) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = rg * 16 + r + (e >> 1) * 8, j = t * 8 + c2 + (e & 1);
+                const float one = i == j ? 1.0f : 0.0f;
+                A[t][e] = one - bet[i] * S[t][e];
+                S[t][e] = one - S[t][e] * bet[j];
+                tm = fmaxf(tm, fabsf(A[t][e]));
+                mm = fmaxf(mm, fabsf(S[t][e]));
+            }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
             mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
         }
-        if (lane == 0) {
-            red[1][warp] = tm;
-            red[2][warp] = mm;
-        }
-        __syncthreads();
-        float tup, tdown, mup, mdown;
-        row_scale(fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), tup, tdown);
-        row_scale(fmaxf(fmaxf(red[2][0], red[2][1]), fmaxf(red[2][2], red[2][3])), mup, mdown);
-        if (threadIdx.x == 0) {
-            tk[TOK_MISC * C] = mdown;
-            tk[TOK_MISC * C + 1] = pdown;
-            tk[TOK_MISC * C + 2] = tdown;
-        }
-        char* gM = (char*)(d.Mt + head * 2 * C * C);
-        char* gT = (char*)(d.Tt + head * 2 * C * C);
-        for (int i = threadIdx.x; i < C * C / 2; i += 128) {
-            const int row = i / (C / 2), cc = i % (C / 2) * 2;
-            const float x = X[row * LDA + cc], y = X[row * LDA + cc + 1];
-            uint32_t p[2];
-            const uint32_t o = tile_off<C>(row, cc);
-            split_pair<2>(x * (bet[cc] / bet[row]) * mup, y * (bet[cc + 1] / bet[row]) * mup, p);
-#pragma unroll
-            for (int k = 0; k < 2; k++) *(uint32_t*)(gM + k * (C * C * 2) + o) = p[k];
-            if (!train) continue;
-            split_pair<2>(x * tup, y * tup, p);
-#pragma unroll
-            for (int k = 0; k < 2; k++) *(uint32_t*)(gT + k * (C * C * 2) + o) = p[k];
+        row_scale(mm, up, down);
+        if (lane == 0) tk[TOK_MISC * C + rg] = down;
+        put((char*)(d.Mt + head * 2 * C * C), S, up, false);
+        if (train) {
+            row_scale(tm, up, down);
+            if (lane == 0) tk[TOK_MISC * C + 8 + rg] = down;
+            put((char*)(d.Tt + head * 2 * C * C), A, up, false);
         }
     }
 }
@@ -312,7 +358,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
 template <int DKP, typename IO>
 cudaError_t prep_go(const DeltaDesc& d, int train, cudaStream_t st) {
     constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
-    const int sm = 2 * NPK * C * DKP * 2 + (2 * C + C / 2) * (C + 1) * 4;
+    const int sm = 2 * NPK * C * DKP * 2 + 2 * C * C * 2;
     auto kern = delta_prep_kernel<DKP, IO>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm);
     if (e != cudaSuccess) return e;
@@ -513,13 +559,14 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     d.Pt = (__half*)take(cv * 2 * C * C * 2);
     d.tok = (float*)take(cv * TOK_ROWS * C * 4);
     if (train) {
-        const size_t f = cv * d.units * 32 * 4 * 4;   // one 16-byte piece per lane and unit
-        d.Sf = (float*)take(f * (DKP / 8));
-        d.dSf = (float*)take(f * (DKP / 8));
+        const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
         d.Tt = (__half*)take(cv * 2 * C * C * 2);
-        d.Wf = (float*)take(f * (C / 8));
-        d.Of = (float*)take(f * (C / 8));
-        d.Rf = (float*)take(f * (C / 8));
+        d.Sh = (__half*)take(u * 2 * DKP);
+        d.Wh = (__half*)take(u * 2 * C);
+        d.Of = (float*)take(u * 2 * C);
+        d.Gh = (__half*)take(u * NPK * C);
+        d.Rh = (__half*)take(u * NPK * C);
+        d.dSh = (__half*)take(u * NPK * DKP);
         d.part = (float*)take(cv * d.units * 2 * C * 4);
         d.anchor = (float*)take(cv * d.units * 4 * 4);
         d.mx = (float*)take(cv * d.units * 4 * MX_ROWS * 4);

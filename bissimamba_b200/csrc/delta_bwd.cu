@@ -120,23 +120,30 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
         // what the end of the chunk reads: in flight under the products
         RT V[2][4];
-        float4 w4[2], o4[2];
+        uint32_t wr[2][2][2];
+        float4 o4[2];
         load_t(d.v, d.ld_v, ldv, c, V);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const size_t at = (fb * (C / 8) + w * 2 + t) * 32 + lane;
-            w4[t] = on ? ((const float4*)d.Wf)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             o4[t] = on ? ((const float4*)d.Of)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (on) get_tile<64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, wr[t]);
+            else wr[t][0][0] = wr[t][0][1] = wr[t][1][0] = wr[t][1][1] = 0;
         }
+        float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
+        const float fw = on ? mx[MX_W] : 0.0f, fs = on ? mx[MX_S] : 0.0f;
         if (on) {
-            float4* p = (float4*)d.dSf + (fb * KT + w * KTW) * 32 + lane;
-#pragma unroll
-            for (int t = 0; t < KTW; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
             const float m = warp_down(sdn), mg = warp_down(gdn);
             if (lane == 0) {
-                d.mx[(fb * 4 + w) * MX_ROWS + MX_DS] = m;
-                d.mx[(fb * 4 + w) * MX_ROWS + MX_DO] = mg;
+                mx[MX_DS] = m;
+                mx[MX_DO] = mg;
             }
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+                put_tile<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, S[t], 1.0f / m);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                put_tile<NPK, 64>(d.Gh + fb * NPK * 16 * C, 16 * C, lane, (w * 2 + t) * 8, G[t], 1.0f / mg);
         }
         // K dS_C
         float X[2][4], Y[2][4], part[2][4];
@@ -163,18 +170,20 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             uint32_t a[NPK][4];
             FG::template get<NPK>(exG, kk, lane, a);
             FG::scale(exG, kk, lane, dn);
+            const float fp = tk[TOK_MISC * C + 4 + kk];
+            dn[0] *= fp;
+            dn[1] *= fp;
             const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
             zero(part);
             mma_row<NPK, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
             add_scaled(Y, part, dn);
         }
-        const float ft = tk[TOK_MISC * C + 2], fp = tk[TOK_MISC * C + 1] * d.scale;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + (e & 1);
-                X[t][e] = fmaf(Y[t][e], fp, X[t][e] * (tw[TOK_GC * C + i] * tw[TOK_FK * C + i]));
+                X[t][e] = fmaf(Y[t][e], d.scale, X[t][e] * (tw[TOK_GC * C + i] * tw[TOK_FK * C + i]));
                 Y[t][e] = 0.0f;
             }
         frag_scale(X, up, dn);
@@ -197,6 +206,9 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             uint32_t a[2][4];
             FX::template get<2>(exX, kk, lane, a);
             FX::scale(exX, kk, lane, dn);
+            const float ft = tk[TOK_MISC * C + 8 + kk];
+            dn[0] *= ft;
+            dn[1] *= ft;
             const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
             zero(part);
             mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oT + p * ST::TT + o); });
@@ -207,12 +219,17 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = t * 8 + (e & 1);
-                Y[t][e] *= ft;
                 X[t][e] = Y[t][e] * -(tw[TOK_BETA * C + i] * tw[TOK_EG * C + i] * tw[TOK_FK * C + i]);
             }
         frag_scale(X, up, dn);
         FX::put(exF, w, lane, X[0], X[1], up, dn);
         unit_bar(grp);
+        uint32_t sr[KTW][2][2];   // S_0, in flight under the product
+        if (on) {
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+                get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, sr[t]);
+        }
         // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q - (beta e^gamma dR)^T K
         const float last = tk[TOK_EG * C + C - 1];
 #pragma unroll
@@ -244,15 +261,15 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         frag_scale(Y, up, dn);
         {
             const float m = warp_down(dn);
-            if (on && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_R] = m;
+            if (on && lane == 0) mx[MX_R] = m;
             const long long t0 = (long long)c * C + w * 16;
             IO* pd = (IO*)d.dvv + (start + t0) * d.ld_dv + (long long)hv * d.dv + col[0];
             float ts[2][2], bs[2][2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                if (on)
-                    *((float4*)d.Rf + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(Y[t][0], Y[t][1], Y[t][2], Y[t][3]);
-                const float ww[4] = {w4[t].x, w4[t].y, w4[t].z, w4[t].w}, oo[4] = {o4[t].x, o4[t].y, o4[t].z, o4[t].w};
+                if (on) put_tile<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, (w * 2 + t) * 8, Y[t], 1.0f / m);
+                const float2 wa = join(wr[t][0][0], wr[t][0][1]), wb = join(wr[t][1][0], wr[t][1][1]);
+                const float ww[4] = {wa.x, wa.y, wb.x, wb.y}, oo[4] = {o4[t].x, o4[t].y, o4[t].z, o4[t].w};
                 ts[t][0] = ts[t][1] = bs[t][0] = bs[t][1] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -273,22 +290,22 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 if (on && r == t) {
                     float* pp = d.part + fb * 2 * C + w * 16 + t * 8 + c2;
                     *(float2*)pp = make_float2(ts[t][0], ts[t][1]);
-                    *(float2*)(pp + C) = make_float2(bs[t][0], bs[t][1]);
+                    *(float2*)(pp + C) = make_float2(bs[t][0] * fw, bs[t][1] * fw);
                 }
             }
         }
         // <S_0, dS_0> over the warp's entries
         if (on) {
             float an = 0.0f;
-            const float4* ps = (const float4*)d.Sf + (fb * KT + w * KTW) * 32 + lane;
 #pragma unroll
             for (int t = 0; t < KTW; t++) {
-                const float4 x = ps[t * 32];
+                const float2 x = join(sr[t][0][0], sr[t][0][1]), y = join(sr[t][1][0], sr[t][1][1]);
                 an = fmaf(S[t][0], x.x, an);
                 an = fmaf(S[t][1], x.y, an);
-                an = fmaf(S[t][2], x.z, an);
-                an = fmaf(S[t][3], x.w, an);
+                an = fmaf(S[t][2], y.x, an);
+                an = fmaf(S[t][3], y.y, an);
             }
+            an *= fs;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
             if (lane == 0) d.anchor[fb * 4 + w] = an;
@@ -308,43 +325,39 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
 
 // ------------------------------------------------------------------ gradients without recurrence
 // Eight warps: 16 token rows x half of dk (and half of the 64 columns of dP, dA) each.  dv is walked in slices of
-// 64, staged as fp16 tiles in one piece (bf16 results: 11 bits are enough before the rounding) or two (fp32); a
-// tile has one power of two, from the largest entry that the recurrences recorded.
+// four units, whose fp16 tiles come as the recurrences left them: one piece for bf16 results (11 bits are enough
+// before the rounding), two for fp32.  A unit is one step of 16 in the products over dv, so its powers of two are
+// applied when the step's products are added to the fp32 sums.
 template <int DKP, int NP>
 struct GradSmem {
-    static constexpr int C = kDeltaC;
-    static constexpr int KQ = NP * C * DKP * 2, T64 = 64 * C * 2, SD = 64 * DKP * 2;
-    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oU = oG + NP * T64, oR = oU + NP * T64, oS = oR + NP * T64,
+    static constexpr int C = kDeltaC, NH = DKP / 64;
+    static constexpr int KQ = NP * C * DKP * 2, T64 = 64 * C * 2, SD = NH * 64 * 128;
+    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oW = oG + NP * T64, oR = oW + NP * T64, oS = oR + NP * T64,
                          oD = oS + NP * SD, oEnd = oD + NP * SD;
     // the four weighted matrices take the place of the slices
     static constexpr int oE = oG, TE = C * C * 2;
     static constexpr int oTok = (oE + 4 * NP * TE > oEnd ? oE + 4 * NP * TE : oEnd);
-    static constexpr int oGam = oTok + TOK_ROWS * C * 4;
-    static constexpr int BYTES = oGam + C * 8;
+    static constexpr int oMx = oTok + TOK_ROWS * C * 4;
+    static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
+    static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
+    static constexpr int BYTES = oCol + 3 * 48 * 4;
 };
 
-// 2^14-based scale of the largest of the units' records
-__device__ __forceinline__ void units_scale(const float* mx, int units, int which, float& up, float& down) {
-    float m = 0.0f;
-    for (int i = 0; i < units; i++) m = fmaxf(m, mx[i * MX_ROWS + which]);
-    down = m;
-    up = 1.0f / m;   // a power of two, at least 2^-126
-}
-
 template <int DKP, typename IO>
-__global__ void __launch_bounds__(256, 1)
-delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
+__global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1)
+delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NP = F32 ? 2 : 1;
     using SM = GradSmem<DKP, NP>;
-    constexpr int HN = DKP / 2, HT = HN / 8, KT = DKP / 8, NT = C / 8;
+    constexpr int HN = DKP / 2, HT = HN / 8;
     constexpr int PK = C * DKP * 2;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ float red[4][8];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     float* tk = (float*)(sm + SM::oTok);
-    double* gam = (double*)(sm + SM::oGam);
+    float* mx = (float*)(sm + SM::oMx);
+    DecaySmem dec{(double*)(sm + SM::oGam), (float*)(sm + SM::oRow), (float*)(sm + SM::oCol)};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rg = warp & 3, ch = warp >> 2;
     const int r = lane >> 2, c2 = (lane & 3) * 2;
@@ -362,33 +375,40 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         cp_commit();
     }
     float dQ[HT][4], dK[HT][4];
-#pragma unroll
-    for (int t = 0; t < HT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) dQ[t][e] = dK[t][e] = 0.0f;
+    zero(dQ);
+    zero(dK);
 
     for (int hh = 0; hh < d.grp; hh++) {
         const int hv = hk * d.grp + hh;
         const size_t head = (size_t)chunk * d.Hv + hv;
-        __syncthreads();
-        for (int i = tid; i < TOK_ROWS * C; i += 256) tk[i] = d.tok[head * TOK_ROWS * C + i];
-        if (warp == 0) {
-            double carry = 0.0;
-#pragma unroll
-            for (int h = 0; h < C / 32; h++) {
-                const int i = h * 32 + lane;
-                float g = (d.g && i < cnt) ? d.g[(tok0 + i) * d.Hv + hv] : 0.0f;
-                if (g < -104.0f) g = -104.0f;
-                double s = g;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double t = __shfl_up_sync(0xffffffffu, s, o);
-                    if (lane >= o) s += t;
-                }
-                s += carry;
-                gam[i] = s;
-                carry = __shfl_sync(0xffffffffu, s, 31);
+        // tiles of units u0 .. u0 + 3
+        const auto slice = [&](int u0) {
+            const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
+            for (int i = tid; i < nx * NP * 128; i += 256) {
+                const int x = i / (NP * 128), p = i / 128 % NP, o = (i & 127) * 16;
+                const size_t g = ((head * d.units + u0 + x) * NP + p) * 2048 + o;
+                const size_t gw = ((head * d.units + u0 + x) * 2 + p) * 2048 + o;   // W keeps both pieces
+                const uint32_t s = sb + p * SM::T64 + x * 2048 + o;
+                cp16(s + SM::oG, (const char*)d.Gh + g);
+                cp16(s + SM::oR, (const char*)d.Rh + g);
+                cp16(s + SM::oW, (const char*)d.Wh + gw);
             }
+            for (int i = tid; i < nx * NP * SM::NH * 128; i += 256) {
+                const int x = i / (NP * SM::NH * 128), p = i / (SM::NH * 128) % NP, h = i / 128 % SM::NH, o = (i & 127) * 16;
+                const size_t g = (((head * d.units + u0 + x) * NP + p) * SM::NH + h) * 2048 + o;
+                const size_t gs = (((head * d.units + u0 + x) * 2 + p) * SM::NH + h) * 2048 + o;
+                const uint32_t s = sb + p * SM::SD + h * 8192 + x * 2048 + o;
+                cp16(s + SM::oD, (const char*)d.dSh + g);
+                cp16(s + SM::oS, (const char*)d.Sh + gs);
+            }
+            cp_commit();
+        };
+        __syncthreads();
+        slice(0);
+        for (int i = tid; i < TOK_ROWS * C; i += 256) tk[i] = d.tok[head * TOK_ROWS * C + i];
+        for (int i = tid; i < d.units * 4 * MX_ROWS; i += 256) mx[i] = d.mx[head * d.units * 4 * MX_ROWS + i];
+        if (warp == 0) {
+            running_sums(d, tok0, cnt, hv, lane, dec.gam);
         } else if (warp == 1 && (d.dg || d.dbeta)) {
             // gates: tokens lane and lane + 32
             double before = 0.0, anchor = 0.0;
@@ -418,168 +438,117 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 before += __shfl_sync(0xffffffffu, s, 31);
             }
         }
-        const float* mx = d.mx + head * d.units * 4 * MX_ROWS;
-        float uS, sS, uU, sU, uG, sG, uR, sR, uD, sD;
-        units_scale(mx, d.units * 4, MX_S, uS, sS);
-        units_scale(mx, d.units * 4, MX_U, uU, sU);
-        units_scale(mx, d.units * 4, MX_DO, uG, sG);
-        units_scale(mx, d.units * 4, MX_R, uR, sR);
-        units_scale(mx, d.units * 4, MX_DS, uD, sD);
+        __syncthreads();
+        decay_tables(dec, tid);
 
-        float dP[4][4], dA[4][4], q1[HT][4], z1[HT][4], k1[HT][4];
+        float dP[4][4], dA[4][4];
+        zero(dP);
+        zero(dA);
+        float fq[2], fz[2], fu[2];   // row factors of the products with the states
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) dP[t][e] = dA[t][e] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < HT; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) q1[t][e] = z1[t][e] = k1[t][e] = 0.0f;
-
+        for (int h = 0; h < 2; h++) {
+            const int i = rg * 16 + r + h * 8;
+            const float eg = tk[TOK_EG * C + i], be = tk[TOK_BETA * C + i];
+            fq[h] = d.scale * eg;
+            fz[h] = -be * eg;
+            fu[h] = tk[TOK_GC * C + i] * be;
+        }
         for (int u0 = 0; u0 < d.units; u0 += 4) {
+            if (u0) {
+                __syncthreads();
+                slice(u0);
+            }
+            cp_wait<0>();
             __syncthreads();
-            // dO: [tokens][64 columns]
-            for (int i = tid; i < C * 8; i += 256) {
-                const int row = i >> 3, c8 = (i & 7) * 8, cc = u0 * 16 + c8;
-                const IO* src = (const IO*)d.go + (tok0 + row) * d.ld_do + (long long)hv * d.dv + cc;
-                float x[8];
-                if (vec && row < cnt && cc + 8 <= d.dv) {
-                    if constexpr (F32) {
-                        const float4 a = *(const float4*)src, b = *(const float4*)(src + 4);
-                        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                    } else {
-                        const uint4 a = *(const uint4*)src;
-                        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[2 * e] = __uint_as_float(w[e] << 16);
-                            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = row < cnt && cc + e < d.dv ? ldt(src, e) : 0.0f;
-                }
-                uint32_t w[4][NP];
-#pragma unroll
-                for (int e = 0; e < 4; e++) split_pair<NP>(x[2 * e] * uG, x[2 * e + 1] * uG, w[e]);
-#pragma unroll
-                for (int k = 0; k < NP; k++)
-                    *(uint4*)(sm + SM::oG + k * SM::T64 + tile_off<64>(row, c8)) =
-                        make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
-            }
-            // U, dR: [64 columns of dv][tokens]
-            for (int i = tid; i < 4 * NT * 32; i += 256) {
-                const int x = i / (NT * 32), t = i / 32 % NT, l = i & 31;
-                float4 uu = make_float4(0.0f, 0.0f, 0.0f, 0.0f), rr = uu;
-                if (u0 + x < d.units) {
-                    const size_t at = ((head * d.units + u0 + x) * NT + t) * 32 + l;
-                    uu = ((const float4*)d.Wf)[at];
-                    rr = ((const float4*)d.Rf)[at];
-                }
-                const int tok = t * 8 + (l & 3) * 2, row = x * 16 + (l >> 2);
-                const float a0 = tk[TOK_BETA * C + tok] * uU, a1 = tk[TOK_BETA * C + tok + 1] * uU;
-                uint32_t p[NP], q[NP];
-                const uint32_t o0 = tile_off<64>(row, tok), o1 = tile_off<64>(row + 8, tok);
-                split_pair<NP>(uu.x * a0, uu.y * a1, p);
-                split_pair<NP>(rr.x * uR, rr.y * uR, q);
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    *(uint32_t*)(sm + SM::oU + k * SM::T64 + o0) = p[k];
-                    *(uint32_t*)(sm + SM::oR + k * SM::T64 + o0) = q[k];
-                }
-                split_pair<NP>(uu.z * a0, uu.w * a1, p);
-                split_pair<NP>(rr.z * uR, rr.w * uR, q);
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    *(uint32_t*)(sm + SM::oU + k * SM::T64 + o1) = p[k];
-                    *(uint32_t*)(sm + SM::oR + k * SM::T64 + o1) = q[k];
-                }
-            }
-            // S_0, dS_C: [64 columns of dv][dk]
-            for (int i = tid; i < 4 * KT * 32; i += 256) {
-                const int x = i / (KT * 32), t = i / 32 % KT, l = i & 31;
-                float4 ss = make_float4(0.0f, 0.0f, 0.0f, 0.0f), dd = ss;
-                if (u0 + x < d.units) {
-                    const size_t at = ((head * d.units + u0 + x) * KT + t) * 32 + l;
-                    ss = ((const float4*)d.Sf)[at];
-                    dd = ((const float4*)d.dSf)[at];
-                }
-                const int kc = t * 8 + (l & 3) * 2, row = x * 16 + (l >> 2);
-                uint32_t p[NP], q[NP];
-                const uint32_t o0 = wide_off<64>(row, kc), o1 = wide_off<64>(row + 8, kc);
-                split_pair<NP>(ss.x * uS, ss.y * uS, p);
-                split_pair<NP>(dd.x * uD, dd.y * uD, q);
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    *(uint32_t*)(sm + SM::oS + k * SM::SD + o0) = p[k];
-                    *(uint32_t*)(sm + SM::oD + k * SM::SD + o0) = q[k];
-                }
-                split_pair<NP>(ss.z * uS, ss.w * uS, p);
-                split_pair<NP>(dd.z * uD, dd.w * uD, q);
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    *(uint32_t*)(sm + SM::oS + k * SM::SD + o1) = p[k];
-                    *(uint32_t*)(sm + SM::oD + k * SM::SD + o1) = q[k];
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                uint32_t aG[NP][4], aR[NP][4], aU[NP][4];
+            const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
+            for (int kk = 0; kk < nx; kk++) {
+                const float* m4 = mx + (u0 + kk) * 4 * MX_ROWS;
+                const float sG = m4[rg * MX_ROWS + MX_DO], sR = m4[rg * MX_ROWS + MX_R], sW = m4[rg * MX_ROWS + MX_W];
+                uint32_t aG[NP][4], aR[NP][4], aW[NP][4];
+                const uint32_t oa = tile_off<64>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane));
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
-                    ldm4(aG[p], sb + SM::oG + p * SM::T64 + tile_off<64>(rg * 16 + la_row(lane), kk * 16 + la_col(lane)));
-                    ldm4t(aR[p], sb + SM::oR + p * SM::T64 + tile_off<64>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane)));
-                    ldm4t(aU[p], sb + SM::oU + p * SM::T64 + tile_off<64>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane)));
+                    ldm4t(aG[p], sb + SM::oG + p * SM::T64 + oa);
+                    ldm4t(aR[p], sb + SM::oR + p * SM::T64 + oa);
+                    ldm4t(aW[p], sb + SM::oW + p * SM::T64 + oa);
                 }
-                const auto ldu = [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, sb + SM::oU + p * SM::T64 +
-                                 tile_off<64>(kk * 16 + la_row(lane), ch * 32 + t2 * 16 + la_col(lane)));
-                };
-                if (ch * 2 <= rg) {   // columns above the diagonal blocks are not needed
-                    mma_row<NP, NP>(dP, aG, 0, 2, ldu);
-                    mma_row<NP, NP>(dA, aR, 0, 2, ldu);
+                // dO W^T and dR W^T, columns up to the diagonal block
+#pragma unroll
+                for (int t2 = 0; t2 < 2; t2++) {
+                    if (ch * 2 + t2 > rg) continue;
+                    const float sw = m4[(ch * 2 + t2) * MX_ROWS + MX_W];
+                    const auto ldw = [&](int p, int, uint32_t (&b)[4]) {
+                        ldm4t(b, sb + SM::oW + p * SM::T64 + tile_off<64>(kk * 16 + la_row(lane), ch * 32 + t2 * 16 + la_col(lane)));
+                    };
+                    float part[2][4], par2[2][4];
+                    zero(part);
+                    zero(par2);
+                    mma_row<NP, NP>(part, aG, 0, 1, ldw);
+                    mma_row<NP, NP>(par2, aR, 0, 1, ldw);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            dP[t2 * 2 + t][e] = fmaf(part[t][e], sG * sw, dP[t2 * 2 + t][e]);
+                            dA[t2 * 2 + t][e] = fmaf(par2[t][e], sR * sw, dA[t2 * 2 + t][e]);
+                        }
                 }
-                const auto lds = [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, sb + SM::oS + p * SM::SD +
-                                 wide_off<64>(kk * 16 + la_row(lane), ch * HN + t2 * 16 + la_col(lane)));
-                };
-                const auto ldd = [&](int p, int t2, uint32_t (&b)[4]) {
-                    ldm4t(b, sb + SM::oD + p * SM::SD +
-                                 wide_off<64>(kk * 16 + la_row(lane), ch * HN + t2 * 16 + la_col(lane)));
-                };
-                mma_row<NP, NP>(q1, aG, 0, HN / 16, lds);
-                mma_row<NP, NP>(z1, aR, 0, HN / 16, lds);
-                mma_row<NP, NP>(k1, aU, 0, HN / 16, ldd);
+                // dO S_0^T, dR S_0^T, W dS_C^T: columns in quarters of dk, two of them this warp's
+#pragma unroll
+                for (int qd = 0; qd < 2; qd++) {
+                    constexpr int QT = DKP / 32;   // tiles of a quarter
+                    const float* mq = m4 + (ch * 2 + qd) * MX_ROWS;
+                    const float sS = mq[MX_S], sD = mq[MX_DS];
+                    float part[QT][4];
+                    const auto ld_at = [&](int base, int p, int t2, uint32_t (&b)[4]) {
+                        ldm4t(b, sb + base + p * SM::SD +
+                                     wide_off<64>(kk * 16 + la_row(lane), ch * HN + qd * QT * 8 + t2 * 16 + la_col(lane)));
+                    };
+                    const auto lds = [&](int p, int t2, uint32_t (&b)[4]) { ld_at(SM::oS, p, t2, b); };
+                    const auto ldd = [&](int p, int t2, uint32_t (&b)[4]) { ld_at(SM::oD, p, t2, b); };
+                    const auto add = [&](float (&to)[HT][4], const float (&f)[2], float s) {
+#pragma unroll
+                        for (int t = 0; t < QT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) to[qd * QT + t][e] = fmaf(part[t][e], f[e >> 1] * s, to[qd * QT + t][e]);
+                    };
+                    zero(part);
+                    mma_row<NP, NP>(part, aG, 0, QT / 2, lds);
+                    add(dQ, fq, sG * sS);
+                    zero(part);
+                    mma_row<NP, NP>(part, aR, 0, QT / 2, lds);
+                    add(dK, fz, sR * sS);
+                    zero(part);
+                    mma_row<NP, NP>(part, aW, 0, QT / 2, ldd);
+                    add(dK, fu, sW * sD);
+                }
             }
         }
         // weighted matrices: E = scale G dO U^T with the key's and with the query's tile scale, F = -beta G dR U^T
         // with the key's of either side
         float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float wP = d.scale * sG * sU, wA = -sR * sU;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < 4; t++) {
+            if (ch * 2 + (t >> 1) > rg) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = rg * 16 + r + (e >> 1) * 8, j = ch * 32 + t * 8 + c2 + (e & 1);
-                const float g = j <= i ? expf((float)(gam[i] - gam[j])) : 0.0f;
-                dP[t][e] = j <= i ? g * wP * dP[t][e] : 0.0f;
-                dA[t][e] = j < i ? g * wA * tk[TOK_BETA * C + i] * dA[t][e] : 0.0f;
+                const float g = dec.at(i, j, ch * 2 + (t >> 1) == rg, rg) * tk[TOK_BETA * C + j];
+                dP[t][e] = j <= i ? g * d.scale * dP[t][e] : 0.0f;
+                dA[t][e] = j < i ? -g * tk[TOK_BETA * C + i] * dA[t][e] : 0.0f;
                 m[0] = fmaxf(m[0], fabsf(dP[t][e] * tk[TOK_FK * C + j]));
                 m[1] = fmaxf(m[1], fabsf(dP[t][e] * tk[TOK_FQ * C + i]));
                 m[2] = fmaxf(m[2], fabsf(dA[t][e] * tk[TOK_FK * C + j]));
                 m[3] = fmaxf(m[3], fabsf(dA[t][e] * tk[TOK_FK * C + i]));
             }
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
 #pragma unroll
             for (int o = 16; o; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
             if (lane == 0) red[k][warp] = m[k];
         }
-        cp_wait<0>();
-        __syncthreads();   // the slices are read, K and Q have arrived
+        __syncthreads();   // the slices are read
         float eu[4], ed[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -589,7 +558,8 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             row_scale(x, eu[k], ed[k]);
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < 4; t++) {
+            if (ch * 2 + (t >> 1) > rg) continue;   // blocks above the diagonal are never read
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int i = rg * 16 + r + h * 8, j = ch * 32 + t * 8 + c2;
@@ -606,33 +576,14 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     for (int x = 0; x < NP; x++) *(uint32_t*)(sm + SM::oE + (k * NP + x) * SM::TE + o) = p[x];
                 }
             }
-        __syncthreads();
-        // fold the products over dv into the sums, then the four products over tokens
-        float fq[2], fz[2], fu[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int i = rg * 16 + r + h * 8;
-            const float eg = tk[TOK_EG * C + i];
-            fq[h] = d.scale * eg * sG * sS;
-            fz[h] = -tk[TOK_BETA * C + i] * eg * sR * sS;
-            fu[h] = tk[TOK_GC * C + i] * sU * sD;
         }
-#pragma unroll
-        for (int t = 0; t < HT; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                dQ[t][e] = fmaf(fq[e >> 1], q1[t][e], dQ[t][e]);
-                dK[t][e] = fmaf(fz[e >> 1], z1[t][e], dK[t][e]);
-                dK[t][e] = fmaf(fu[e >> 1], k1[t][e], dK[t][e]);
-            }
+        __syncthreads();
+        // the four products over tokens
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             // k: 0 E K -> dQ, 2 F K -> dK (rows i, sum over j <= i); 1 E^T Q, 3 F^T K -> dK (rows j, sum over i >= j)
             float acc[HT][4];
-#pragma unroll
-            for (int t = 0; t < HT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[t][e] = 0.0f;
+            zero(acc);
 #pragma unroll
             for (int kk = 0; kk < C / 16; kk++) {
                 if ((k & 1) ? kk < rg : kk > rg) continue;
@@ -702,9 +653,7 @@ cudaError_t grads_go(const DeltaDesc& d, cudaStream_t st) {
     auto kern = delta_grads_kernel<DKP, IO>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES);
     if (e != cudaSuccess) return e;
-    const int V = 16 / (int)sizeof(IO);
-    const int vec = d.dv % V == 0 && d.ld_do % V == 0 && ((uintptr_t)d.go & 15) == 0;
-    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 256, SM::BYTES, st>>>(d, vec);
+    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 256, SM::BYTES, st>>>(d);
     return cudaGetLastError();
 }
 }  // namespace

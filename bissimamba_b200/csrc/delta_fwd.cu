@@ -99,11 +99,11 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
         const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
         if (KEEP && on) {
-            float4* p = (float4*)d.Sf + (fb * KT + w * KTW) * 32 + lane;
-#pragma unroll
-            for (int t = 0; t < KTW; t++) p[t * 32] = make_float4(S[t][0], S[t][1], S[t][2], S[t][3]);
             const float m = warp_down(sdn);
             if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = m;
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+                put_tile<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, S[t], 1.0f / m);
         }
         float X[2][4], O[2][4], part[2][4], dn[2], up[2];
         zero(X);
@@ -153,15 +153,18 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
             add_scaled(W, part, dn);
         }
-        const float fm = tk[TOK_MISC * C], fp = tk[TOK_MISC * C + 1];
+        const float fm = tk[TOK_MISC * C + w], fp = tk[TOK_MISC * C + 4 + w];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) W[t][e] *= fm;
         if (KEEP && on) {
-            float4* p = (float4*)d.Wf + (fb * (C / 8) + w * 2) * 32 + lane;
+            frag_scale(W, up, dn);
+            const float m = warp_down(dn);
+            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = m;
 #pragma unroll
-            for (int t = 0; t < 2; t++) p[t * 32] = make_float4(W[t][0], W[t][1], W[t][2], W[t][3]);
+            for (int t = 0; t < 2; t++)
+                put_tile<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, W[t], 1.0f / m);
         }
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -169,10 +172,6 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
         frag_scale(W, up, dn);
         FO::put(exO, w, lane, W[0], W[1], up, dn);
-        if (KEEP && on) {
-            const float m = warp_down(dn);
-            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_U] = m;
-        }
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll

@@ -7,8 +7,8 @@
 //   O = scale (diag(e^gamma) Q S_0 + P U),   P_ij = G_ij q_i.k_j (j <= i)
 //   S_C = e^gamma_C S_0 + sum_j G_Cj k_j u_j^T
 // With a_ij = G_ij k_i.k_j (j < i):  W = M (V - diag(e^gamma) K S_0), M = (I + a diag(beta))^-1,
-// and the adjoint of U is T^T dU, T = (I + diag(beta) a)^-1 = diag(beta) M diag(beta)^-1.  W and T^T dU exist where
-// beta is 0, and their product is beta's gradient, so the forward takes M and the backward T.
+// and the adjoint of U is T^T dU, T = (I + diag(beta) a)^-1.  W and T^T dU are full where beta is 0, and their product
+// is beta's gradient, so the forward takes M and the backward T.
 // M, T and P depend on no state: a first kernel computes them for all chunks at
 // once; the recurrence over chunks then is three products a chunk.
 //
@@ -37,10 +37,10 @@ enum {
     TOK_BETA = 2,  // beta, 0 behind the last token
     TOK_FK = 3,    // k_i = FK_i * row i of the K tile
     TOK_FQ = 4,
-    TOK_MISC = 5,  // [0], [1], [2]: M, P and T = that factor times their tiles
+    TOK_MISC = 5,  // [b], [4 + b], [8 + b]: rows 16 b .. 16 b + 15 of M, P, T = that factor times their tiles
     TOK_ROWS = 6
 };
-enum { MX_S = 0, MX_U = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
+enum { MX_S = 0, MX_W = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
 constexpr int kDeltaC = 64;      // tokens per chunk
 constexpr float kStateFloor = 2.98023223876953125e-08f;   // 2^-25: times a row's `down` (its largest entry / 2^14) = 2^-39..-40 of it
 
@@ -60,13 +60,15 @@ struct DeltaDesc {
     long long ld_q, ld_k, ld_v, ld_o;
     // workspace
     __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
-    __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], scaled as a whole; Tt for training only
+    __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], on and below the diagonal blocks; Tt for training only
     float* tok;                  // [nch][Hv][TOK_ROWS][C], see TOK_*
-    // kept for the backward; "fragment order": [nch][Hv][units][tiles][32 lanes][4]
-    float *Sf, *Wf, *Of;         // state at the chunk's start, W, O
-    float *Rf, *dSf;             // backward: dR = T^T dU, adjoint of the state at the chunk's end
+    // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
+    // scaled by a power of two (mx)
+    __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [2][16 * C]
+    float* Of;                   // O, in accumulator order [C / 8 tiles][32 lanes][4]
+    __half *Gh, *Rh, *dSh;       // backward: dO, dR = T^T dU [pieces][16 * C], adjoint of the state at the chunk's end
     float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units][4 warps]
-    float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: down-scale of the largest entry of S, U, dO, dR, dS
+    float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: what the tiles of S, W, dO, dR, dS are times
     // gradients
     const void* go;
     const float* dhT;
@@ -246,6 +248,47 @@ __device__ __forceinline__ bool chunk_range(const DeltaDesc& d, int chunk, long 
     return true;
 }
 
+// ------------------------------------------------------------------ decays inside a chunk
+// Running sums of g in 64 bits (lane holds tokens lane and lane + 32), -104 for anything below it: exp is 0 in fp32
+// there, and differences of the sums stay what G needs after a reset (g = -inf) too.
+__device__ __forceinline__ void running_sums(const DeltaDesc& d, long long tok0, int cnt, int hv, int lane,
+                                             double* gam) {
+    double carry = 0.0;
+#pragma unroll
+    for (int h = 0; h < kDeltaC / 32; h++) {
+        const int i = h * 32 + lane;
+        float g = (d.g && i < cnt) ? d.g[(tok0 + i) * d.Hv + hv] : 0.0f;
+        if (g < -104.0f) g = -104.0f;
+        double s = g;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += t;
+        }
+        s += carry;
+        gam[i] = s;
+        carry = __shfl_sync(0xffffffffu, s, 31);
+    }
+}
+// G_ij = exp(gamma_i - gamma_j), j <= i.  Between blocks of 16 tokens it is the product of two decays that meet at
+// the end of the block before i's (both at most e^0 where g <= 0, so nothing overflows on the way).
+struct DecaySmem {
+    double* gam;   // [C]
+    float* row;    // [C]: exp(gamma_i - gamma at the end of the block before)
+    float* col;    // [3][48]: exp(gamma at the end of block b - gamma_j), j <= 16 b + 15
+    __device__ __forceinline__ float at(int i, int j, bool same_block, int block_i) const {
+        if (same_block) return j <= i ? expf((float)(gam[i] - gam[j])) : 0.0f;
+        return row[i] * col[(block_i - 1) * 48 + j];
+    }
+};
+__device__ __forceinline__ void decay_tables(const DecaySmem& s, int tid) {   // gam is there; a barrier follows
+    if (tid < kDeltaC && tid >= 16) s.row[tid] = expf((float)(s.gam[tid] - s.gam[(tid & ~15) - 1]));
+    if (tid < 96) {
+        const int b = tid < 16 ? 0 : tid < 48 ? 1 : 2, j = tid < 16 ? tid : tid < 48 ? tid - 16 : tid - 48;
+        s.col[b * 48 + j] = expf((float)(s.gam[16 * b + 15] - s.gam[j]));
+    }
+}
+
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -320,6 +363,37 @@ struct FragBuf {
         dn[1] = s[(lane >> 2) + 8];
     }
 };
+// Entries (r, c) (r, c + 1) and (r + 8, ...) of an accumulator tile at column `col` of a 16-row tile in global memory,
+// W columns wide, NP pieces `piece` halves apart
+template <int NP, int W>
+__device__ __forceinline__ void put_tile(__half* base, size_t piece, int lane, int col, const float (&t)[4], float up) {
+    const int c = col + (lane & 3) * 2;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint32_t p[NP];
+        split_pair<NP>(t[2 * h] * up, t[2 * h + 1] * up, p);
+        const uint32_t o = W == 64 ? tile_off<64>((lane >> 2) + 8 * h, c) : wide_off<16>((lane >> 2) + 8 * h, c);
+#pragma unroll
+        for (int k = 0; k < NP; k++) *(uint32_t*)((char*)(base + k * piece) + o) = p[k];
+    }
+}
+// the same entries, both pieces as they are
+template <int W>
+__device__ __forceinline__ void get_tile(const __half* base, size_t piece, int lane, int col, uint32_t (&v)[2][2]) {
+    const int c = col + (lane & 3) * 2;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t o = W == 64 ? tile_off<64>((lane >> 2) + 8 * h, c) : wide_off<16>((lane >> 2) + 8 * h, c);
+#pragma unroll
+        for (int k = 0; k < 2; k++) v[h][k] = *(const uint32_t*)((const char*)(base + k * piece) + o);
+    }
+}
+// x, y of a pair of pieces
+__device__ __forceinline__ float2 join(uint32_t hi, uint32_t lo) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    return make_float2(a.x + b.x, a.y + b.y);
+}
 template <int N>
 __device__ __forceinline__ void zero(float (&t)[N][4]) {
 #pragma unroll
