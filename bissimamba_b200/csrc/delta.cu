@@ -93,47 +93,71 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
 
     char* gK = (char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
     char* gQ = (char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
-    for (int i = threadIdx.x; i < 2 * C * G8; i += 128) {
-        const bool isq = i >= C * G8;
-        const int j = isq ? i - C * G8 : i;
-        const int row = j / G8, c8 = j % G8 * 8;
-        const IO* src = isq ? (const IO*)d.q + (tok0 + row) * d.ld_q + (long long)hk * d.dk
-                            : (const IO*)d.k + (tok0 + row) * d.ld_k + (long long)hk * d.dk;
-        float x[8];
-        if (vec && row < cnt && c8 + 8 <= d.dk) {
-            if constexpr (F32) {
-                const float4 a = *(const float4*)(src + c8), b = *(const float4*)(src + c8 + 4);
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-            } else {
-                const uint4 a = *(const uint4*)(src + c8);
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    // all loads of a batch are in flight before the first is used
+    constexpr int NIT = 2 * C * G8 / 128, BATCH = F32 ? 4 : 8, V4 = F32 ? 2 : 1;
+    for (int it0 = 0; it0 < NIT; it0 += BATCH) {
+        uint4 raw[BATCH][V4];
+        const auto place = [&](int it, bool& isq, int& row, int& c8) {
+            const int i = it * 128 + threadIdx.x;
+            isq = i >= C * G8;
+            const int j = isq ? i - C * G8 : i;
+            row = j / G8;
+            c8 = j % G8 * 8;
+            return isq ? (const IO*)d.q + (tok0 + row) * d.ld_q + (long long)hk * d.dk
+                       : (const IO*)d.k + (tok0 + row) * d.ld_k + (long long)hk * d.dk;
+        };
+        if (vec) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[2 * e] = __uint_as_float(w[e] << 16);
-                    x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                }
+            for (int b = 0; b < BATCH; b++) {
+                bool isq;
+                int row, c8;
+                const IO* src = place(it0 + b, isq, row, c8);
+#pragma unroll
+                for (int x = 0; x < V4; x++)
+                    raw[b][x] = row < cnt && c8 + 8 <= d.dk ? *(const uint4*)(src + c8 + x * 4) : make_uint4(0, 0, 0, 0);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = row < cnt && c8 + e < d.dk ? ldt(src, c8 + e) : 0.0f;
         }
-        float m = 0.0f, up, down;
 #pragma unroll
-        for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]));
+        for (int b = 0; b < BATCH; b++) {
+            bool isq;
+            int row, c8;
+            const IO* src = place(it0 + b, isq, row, c8);
+            float x[8];
+            if (vec && (c8 + 8 <= d.dk || c8 >= d.dk)) {
 #pragma unroll
-        for (int o = 1; o < G8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        row_scale(m, up, down);
-        if (c8 == 0) (isq ? fQ : fK)[row] = down;
-        uint32_t w[4][NPK];
+                for (int v = 0; v < V4; v++) {
+                    const uint32_t w[4] = {raw[b][v].x, raw[b][v].y, raw[b][v].z, raw[b][v].w};
 #pragma unroll
-        for (int e = 0; e < 4; e++) split_pair<NPK>(x[2 * e] * up, x[2 * e + 1] * up, w[e]);
-        const uint32_t o = wide_off<C>(row, c8);
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (F32) {
+                            x[v * 4 + e] = __uint_as_float(w[e]);
+                        } else {
+                            x[2 * e] = __uint_as_float(w[e] << 16);
+                            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                        }
+                    }
+                }
+            } else {
 #pragma unroll
-        for (int k = 0; k < NPK; k++) {
-            const uint4 p = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
-            *(uint4*)(sm + (isq ? NPK * TILE : 0) + k * TILE + o) = p;
-            *(uint4*)((isq ? gQ : gK) + k * TILE + o) = p;
+                for (int e = 0; e < 8; e++) x[e] = row < cnt && c8 + e < d.dk ? ldt(src, c8 + e) : 0.0f;
+            }
+            float m = 0.0f, up, down;
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]));
+#pragma unroll
+            for (int o = 1; o < G8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            row_scale(m, up, down);
+            if (c8 == 0) (isq ? fQ : fK)[row] = down;
+            uint32_t w[4][NPK];
+#pragma unroll
+            for (int e = 0; e < 4; e++) split_pair<NPK>(x[2 * e] * up, x[2 * e + 1] * up, w[e]);
+            const uint32_t o = wide_off<C>(row, c8);
+#pragma unroll
+            for (int k = 0; k < NPK; k++) {
+                const uint4 p = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
+                *(uint4*)(sm + (isq ? NPK * TILE : 0) + k * TILE + o) = p;
+                *(uint4*)((isq ? gQ : gK) + k * TILE + o) = p;
+            }
         }
     }
     __syncthreads();
@@ -198,10 +222,8 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
                 A[t][e] = j < i ? G * fK[i] * kk[t][e] : 0.0f;
             }
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, o));
         float up, down;
-        row_scale(pm, up, down);
+        warp_scale(pm, up, down);
         if (lane == 0) tk[TOK_MISC * C + 4 + rg] = down;
         const auto put = [&](char* g, const float (&x)[C / 8][4], float s, bool shared) {
 #pragma unroll
@@ -265,7 +287,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
         for (int I = 0; I < 4; I++) {
             if (warp == I) {
                 if (I > 0) {
-                    float Y[6][4], aup[2], adn[2], part[6][4];
+                    float Y[6][4], aup, adn, part[6][4];
 #pragma unroll
                     for (int t = 0; t < 6; t++)
 #pragma unroll
@@ -283,12 +305,10 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
                         mma_row<2, 2>(part, a, 0, K + 1, [&](int p, int t2, uint32_t (&b)[4]) {
                             ldm4t(b, sC + p * TT + tile_off<C>(K * 16 + la_row(lane), t2 * 16 + la_col(lane)));
                         });
-                        const float f[2] = {-adn[0] * fC[K], -adn[1] * fC[K]};
-                        add_scaled(Y, part, f);
+                        add_scaled(Y, part, -adn * fC[K]);
                     }
-                    float yup[2], ydn[2];
-                    frag_scale(Y, yup, ydn);
-                    const float ym = warp_down(ydn), yu = 1.0f / ym;
+                    float yu, ym;
+                    frag_scale(Y, yu, ym);
 #pragma unroll
                     for (int t = 0; t < 6; t++)
 #pragma unroll
@@ -311,15 +331,14 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
                     for (int t = 0; t < 6; t++)
                         if ((t >> 1) < rg) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) S[t][e] = part[t][e] * adn[e >> 1] * ym;
+                            for (int e = 0; e < 4; e++) S[t][e] = part[t][e] * (adn * ym);
                         }
                 }
                 if (I < 3) {
-                    float cup[2], cdn[2];
-                    frag_scale(S, cup, cdn);
-                    const float m = warp_down(cdn);
-                    if (lane == 0) fC[I] = m;
-                    put(nullptr, S, 1.0f / m, true);
+                    float cu, cm;
+                    frag_scale(S, cu, cm);
+                    if (lane == 0) fC[I] = cm;
+                    put(nullptr, S, cu, true);
                 }
             }
             __syncthreads();
@@ -339,16 +358,11 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
                 mm = fmaxf(mm, fabsf(S[t][e]));
             }
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-        }
-        row_scale(mm, up, down);
+        warp_scale(mm, up, down);
         if (lane == 0) tk[TOK_MISC * C + rg] = down;
         put((char*)(d.Mt + head * 2 * C * C), S, up, false);
         if (train) {
-            row_scale(tm, up, down);
+            warp_scale(tm, up, down);
             if (lane == 0) tk[TOK_MISC * C + 8 + rg] = down;
             put((char*)(d.Tt + head * 2 * C * C), A, up, false);
         }

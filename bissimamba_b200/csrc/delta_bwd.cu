@@ -75,22 +75,37 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldi + (e >> 1) * 8] : RT(0);
             }
     };
-    float sup[2], sdn[2], up[2], dn[2];
-    const auto put_state = [&]() {
-        frag_scale(S, sup, sdn);
+    float up, dn;
+    // fragments of dS_C and of dO for chunk c, kept too
+    const auto put_state = [&](int c) {
+        frag_scale(S, up, dn);
+        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+        const bool keep = on && c >= 0;
+        if (keep && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_DS] = dn;
 #pragma unroll
-        for (int b = 0; b < KBW; b++) FS::put(exS, w * KBW + b, lane, S[2 * b], S[2 * b + 1], sup, sdn);
+        for (int b = 0; b < KBW; b++) {
+            uint32_t a[2][4];
+            frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
+            FS::put(exS, w * KBW + b, lane, a, dn);
+            if (keep) put_frag<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
+        }
     };
     float G[2][4];   // dO^T of the warp's tokens
-    float gdn[2];
-    RT Gn[2][4];   // the next chunk's
-    const auto put_go = [&]() {
+    RT Gn[2][4];     // the next chunk's
+    const auto put_go = [&](int c) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) G[t][e] = from_raw(Gn[t][e]);
-        frag_scale(G, up, gdn);
-        FG::put(exG, w, lane, G[0], G[1], up, gdn);
+        frag_scale(G, up, dn);
+        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+        uint32_t a[NPK][4];
+        frag_pieces<NPK>(G[0], G[1], up, a);
+        FG::put(exG, w, lane, a, dn);
+        if (on) {
+            put_frag<NPK, 64>(d.Gh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_DO] = dn;
+        }
     };
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&full[0]), 1);
@@ -98,10 +113,10 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (nch > 0) ST::load(d, d.Tt, sb, smem_u32(&full[0]), chunk0 + nch - 1, hv);
     }
-    put_state();
+    put_state(nch - 1);
     if (nch > 0) {
         load_t(d.go, d.ld_do, ldg, nch - 1, Gn);
-        put_go();
+        put_go(nch - 1);
     }
     __syncthreads();
     for (int it = 0; it < nch; it++) {
@@ -132,18 +147,11 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         }
         float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
         const float fw = on ? mx[MX_W] : 0.0f, fs = on ? mx[MX_S] : 0.0f;
+        uint32_t sr[KTW][2][2];   // S_0
         if (on) {
-            const float m = warp_down(sdn), mg = warp_down(gdn);
-            if (lane == 0) {
-                mx[MX_DS] = m;
-                mx[MX_DO] = mg;
-            }
 #pragma unroll
             for (int t = 0; t < KTW; t++)
-                put_tile<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, S[t], 1.0f / m);
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-                put_tile<NPK, 64>(d.Gh + fb * NPK * 16 * C, 16 * C, lane, (w * 2 + t) * 8, G[t], 1.0f / mg);
+                get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, sr[t]);
         }
         // K dS_C
         float X[2][4], Y[2][4], part[2][4];
@@ -160,7 +168,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                 mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
             }
-            FS::scale(exS, s * KBW, lane, dn);
+            dn = FS::scale(exS, s * KBW);
             add_scaled(X, part, dn);
         }
         // P^T dO: column j of P has rows i >= j only
@@ -169,10 +177,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             if (kk < w) continue;
             uint32_t a[NPK][4];
             FG::template get<NPK>(exG, kk, lane, a);
-            FG::scale(exG, kk, lane, dn);
-            const float fp = tk[TOK_MISC * C + 4 + kk];
-            dn[0] *= fp;
-            dn[1] *= fp;
+            dn = FG::scale(exG, kk) * tk[TOK_MISC * C + 4 + kk];
             const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
             zero(part);
             mma_row<NPK, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
@@ -187,7 +192,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 Y[t][e] = 0.0f;
             }
         frag_scale(X, up, dn);
-        FX::put(exX, w, lane, X[0], X[1], up, dn);
+        FX::put(exX, w, lane, X, up, dn);
         // dO with the factors of the state's product
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -197,7 +202,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 X[t][e] = G[t][e] * (d.scale * tw[TOK_EG * C + i] * tw[TOK_FQ * C + i]);
             }
         frag_scale(X, up, dn);
-        FX::put(exE, w, lane, X[0], X[1], up, dn);
+        FX::put(exE, w, lane, X, up, dn);
         unit_bar(grp);
         // dR^T = dU^T T
 #pragma unroll
@@ -205,10 +210,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             if (kk < w) continue;
             uint32_t a[2][4];
             FX::template get<2>(exX, kk, lane, a);
-            FX::scale(exX, kk, lane, dn);
-            const float ft = tk[TOK_MISC * C + 8 + kk];
-            dn[0] *= ft;
-            dn[1] *= ft;
+            dn = FX::scale(exX, kk) * tk[TOK_MISC * C + 8 + kk];
             const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
             zero(part);
             mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oT + p * ST::TT + o); });
@@ -222,14 +224,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 X[t][e] = Y[t][e] * -(tw[TOK_BETA * C + i] * tw[TOK_EG * C + i] * tw[TOK_FK * C + i]);
             }
         frag_scale(X, up, dn);
-        FX::put(exF, w, lane, X[0], X[1], up, dn);
+        FX::put(exF, w, lane, X, up, dn);
         unit_bar(grp);
-        uint32_t sr[KTW][2][2];   // S_0, in flight under the product
-        if (on) {
-#pragma unroll
-            for (int t = 0; t < KTW; t++)
-                get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, sr[t]);
-        }
         // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q - (beta e^gamma dR)^T K
         const float last = tk[TOK_EG * C + C - 1];
 #pragma unroll
@@ -241,7 +237,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             uint32_t a[2][4];
             float ps[KTW][4];
             FX::template get<2>(exE, kk, lane, a);
-            FX::scale(exE, kk, lane, dn);
+            dn = FX::scale(exE, kk);
             zero(ps);
             mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
                 ldm4t(f, st + ST::oQ + p * PK +
@@ -249,25 +245,28 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             });
             add_scaled(S, ps, dn);
             FX::template get<2>(exF, kk, lane, a);
-            FX::scale(exF, kk, lane, dn);
+            dn = FX::scale(exF, kk);
             zero(ps);
             mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
                 ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
             });
             add_scaled(S, ps, dn);
         }
-        put_state();
+        put_state(c - 1);
         // dV, and what the gates' gradients sum over dv
         frag_scale(Y, up, dn);
+        if (on) {
+            uint32_t a[NPK][4];
+            frag_pieces<NPK>(Y[0], Y[1], up, a);
+            put_frag<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+            if (lane == 0) mx[MX_R] = dn;
+        }
         {
-            const float m = warp_down(dn);
-            if (on && lane == 0) mx[MX_R] = m;
             const long long t0 = (long long)c * C + w * 16;
             IO* pd = (IO*)d.dvv + (start + t0) * d.ld_dv + (long long)hv * d.dv + col[0];
             float ts[2][2], bs[2][2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                if (on) put_tile<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, (w * 2 + t) * 8, Y[t], 1.0f / m);
                 const float2 wa = join(wr[t][0][0], wr[t][0][1]), wb = join(wr[t][1][0], wr[t][1][1]);
                 const float ww[4] = {wa.x, wa.y, wb.x, wb.y}, oo[4] = {o4[t].x, o4[t].y, o4[t].z, o4[t].w};
                 ts[t][0] = ts[t][1] = bs[t][0] = bs[t][1] = 0.0f;
@@ -310,7 +309,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
             if (lane == 0) d.anchor[fb * 4 + w] = an;
         }
-        if (c > 0) put_go();
+        if (c > 0) put_go(c - 1);
     }
     if (d.dh0) {
 #pragma unroll

@@ -63,11 +63,20 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
             }
     };
-    float sup[2], sdn[2];
-    const auto put_state = [&]() {
-        frag_scale(S, sup, sdn);
+    // the state's fragments for chunk c, kept too
+    const auto put_state = [&](int c) {
+        float up, dn;
+        frag_scale(S, up, dn);
+        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+        const bool keep = KEEP && on && c < nch;
+        if (keep && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = dn;
 #pragma unroll
-        for (int b = 0; b < KBW; b++) FS::put(exS, w * KBW + b, lane, S[2 * b], S[2 * b + 1], sup, sdn);
+        for (int b = 0; b < KBW; b++) {
+            uint32_t a[2][4];
+            frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
+            FS::put(exS, w * KBW + b, lane, a, dn);
+            if (keep) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
+        }
     };
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&full[0]), 1);
@@ -75,7 +84,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (nch > 0) ST::load(d, d.Mt, sb, smem_u32(&full[0]), chunk0, hv);
     }
-    put_state();
+    put_state(0);
     __syncthreads();
     RT Vn[2][4];
     if (nch > 0) load_v(0, Vn);
@@ -98,14 +107,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         const float* tk = (const float*)(sm + (c & 1) * ST::BYTES + ST::oTok);
         const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
         const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        if (KEEP && on) {
-            const float m = warp_down(sdn);
-            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = m;
-#pragma unroll
-            for (int t = 0; t < KTW; t++)
-                put_tile<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, S[t], 1.0f / m);
-        }
-        float X[2][4], O[2][4], part[2][4], dn[2], up[2];
+        float X[2][4], O[2][4], part[2][4], dn, up;
         zero(X);
         zero(O);
 #pragma unroll
@@ -123,7 +125,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 mma_row<NPO, NPK>(po, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
                                   [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oQ + p * PK + o); });
             }
-            FS::scale(exS, s * KBW, lane, dn);
+            dn = FS::scale(exS, s * KBW);
             add_scaled(X, part, dn);
             add_scaled(O, po, dn);
         }
@@ -137,7 +139,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 O[t][e] *= eg * tw[TOK_FQ * C + i];
             }
         frag_scale(X, up, dn);
-        FX::put(exX, w, lane, X[0], X[1], up, dn);
+        FX::put(exX, w, lane, X, up, dn);
         unit_bar(grp);
         // W^T = X M^T: row i of M reaches columns j <= i only
         float W[2][4];
@@ -147,7 +149,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             if (kk > w) continue;
             uint32_t a[2][4];
             FX::template get<2>(exX, kk, lane, a);
-            FX::scale(exX, kk, lane, dn);
+            dn = FX::scale(exX, kk);
             const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
             zero(part);
             mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
@@ -159,19 +161,18 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
 #pragma unroll
             for (int e = 0; e < 4; e++) W[t][e] *= fm;
         if (KEEP && on) {
+            uint32_t a[2][4];
             frag_scale(W, up, dn);
-            const float m = warp_down(dn);
-            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = m;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-                put_tile<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, W[t], 1.0f / m);
+            frag_pieces<2>(W[0], W[1], up, a);
+            put_frag<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
+            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = dn;
         }
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
         frag_scale(W, up, dn);
-        FO::put(exO, w, lane, W[0], W[1], up, dn);
+        FO::put(exO, w, lane, W, up, dn);
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -180,7 +181,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 W[t][e] *= tw[TOK_GC * C + i] * tw[TOK_FK * C + i];
             }
         frag_scale(W, up, dn);
-        FX::put(exU, w, lane, W[0], W[1], up, dn);
+        FX::put(exU, w, lane, W, up, dn);
         unit_bar(grp);
         // S^T <- e^gamma_C S^T + (G_C. U)^T K
         const float last = tk[TOK_EG * C + C - 1];
@@ -193,23 +194,21 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             uint32_t a[2][4];
             float ps[KTW][4];
             FX::template get<2>(exU, kk, lane, a);
-            FX::scale(exU, kk, lane, dn);
+            dn = FX::scale(exU, kk);
             zero(ps);
             mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
                 ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
             });
             add_scaled(S, ps, dn);
         }
-        put_state();
+        put_state(c + 1);
         // O^T += U^T P^T
 #pragma unroll
         for (int kk = 0; kk < C / 16; kk++) {
             if (kk > w) continue;
             uint32_t a[NPO][4];
             FO::template get<NPO>(exO, kk, lane, a);
-            FO::scale(exO, kk, lane, dn);
-            dn[0] *= fp;
-            dn[1] *= fp;
+            dn = FO::scale(exO, kk) * fp;
             const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
             zero(part);
             mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });

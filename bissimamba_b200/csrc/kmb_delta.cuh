@@ -12,12 +12,12 @@
 // M, T and P depend on no state: a first kernel computes them for all chunks at
 // once; the recurrence over chunks then is three products a chunk.
 //
-// Products run on mma.sync (fp16 factors, fp32 accumulation).  A row of an fp32
-// factor is scaled by a power of two to a largest entry in [2^14, 2^15) and cut
-// into two fp16 pieces x = x0 + x1, each rounded to nearest: 22 bits, and an
-// absolute floor 2^-40 below the row's largest entry, so it holds what an fp32
-// product needs.  The three products x0 y0, x0 y1, x1 y0 are summed; a bf16 row
-// is a single piece (8 bits fit in 11).  Where a sum is rounded to bf16 right
+// Products run on mma.sync (fp16 factors, fp32 accumulation).  A row or a block of
+// 16 of an fp32 factor is scaled by a power of two to a largest entry in
+// [2^14, 2^15) and cut into two fp16 pieces x = x0 + x1, each rounded to nearest:
+// 22 bits down to 2^-18 of the largest entry, and an absolute floor 2^-40 below
+// it, so it holds what an fp32 product needs.  The three products x0 y0, x0 y1,
+// x1 y0 are summed; a bf16 row is a single piece (8 bits fit in 11).  Where a sum is rounded to bf16 right
 // after, one piece of each factor (11 bits) serves.  Three bf16 pieces would take
 // six products for the same accuracy.  The powers of two are undone in the fp32
 // factors that multiply the accumulators anyway.
@@ -42,7 +42,6 @@ enum {
 };
 enum { MX_S = 0, MX_W = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
 constexpr int kDeltaC = 64;      // tokens per chunk
-constexpr float kStateFloor = 2.98023223876953125e-08f;   // 2^-25: times a row's `down` (its largest entry / 2^14) = 2^-39..-40 of it
 
 struct DeltaDesc {
     long long T, total;          // tokens per sequence (fixed length), tokens in all
@@ -133,43 +132,35 @@ __device__ __forceinline__ void row_scale(float m, float& up, float& down) {
     up = __uint_as_float((uint32_t)(268 - e) << 23);
     down = __uint_as_float((uint32_t)(e - 14) << 23);
 }
-// of the two rows (lane / 4, lane / 4 + 8) of accumulator tiles; m0, m1: least magnitudes to assume
+// of all entries of the warp's accumulator tiles: one warp-wide maximum (of the bits: magnitudes order as integers)
 template <int N>
-__device__ __forceinline__ void frag_scale(const float (&t)[N][4], float (&up)[2], float (&down)[2],
-                                           float m0 = 0.0f, float m1 = 0.0f) {
+__device__ __forceinline__ float frag_max(const float (&t)[N][4]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        m0 = fmaxf(m0, fmaxf(fabsf(t[i][0]), fabsf(t[i][1])));
-        m1 = fmaxf(m1, fmaxf(fabsf(t[i][2]), fabsf(t[i][3])));
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-    }
-    row_scale(m0, up[0], down[0]);
-    row_scale(m1, up[1], down[1]);
+    for (int i = 0; i < N; i++)
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(t[i][0]), fabsf(t[i][1])), fmaxf(fabsf(t[i][2]), fabsf(t[i][3]))));
+    return m;
 }
-// A fragment pieces of 16 k columns of two accumulator tiles, rows scaled by up (an accumulator is laid out as
+__device__ __forceinline__ void warp_scale(float m, float& up, float& down) {
+    row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))), up, down);
+}
+template <int N>
+__device__ __forceinline__ void frag_scale(const float (&t)[N][4], float& up, float& down) {
+    warp_scale(frag_max(t), up, down);
+}
+// A fragment pieces of 16 k columns of two accumulator tiles, scaled by up (an accumulator is laid out as
 // an A fragment: no data moves between lanes)
 template <int NP>
-__device__ __forceinline__ void frag_pieces(const float (&t0)[4], const float (&t1)[4], const float (&up)[2],
+__device__ __forceinline__ void frag_pieces(const float (&t0)[4], const float (&t1)[4], float up,
                                             uint32_t (&a)[NP][4]) {
     uint32_t p[NP];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float* t = i < 2 ? t0 : t1;
-        split_pair<NP>(t[(i & 1) * 2] * up[i & 1], t[(i & 1) * 2 + 1] * up[i & 1], p);
+        split_pair<NP>(t[(i & 1) * 2] * up, t[(i & 1) * 2 + 1] * up, p);
 #pragma unroll
         for (int k = 0; k < NP; k++) a[k][i] = p[k];
     }
-}
-// the larger of the two rows' down-scales, over the warp's 16 rows
-__device__ __forceinline__ float warp_down(const float (&down)[2]) {
-    float m = fmaxf(down[0], down[1]);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
 }
 // acc[t] += sum over pieces of a * B for the column blocks t2 (16 columns) in [from, to): B fragments by
 // load(piece, t2, regs).  Two blocks at a time keep four accumulators in turn; smaller products first.
@@ -302,8 +293,8 @@ __device__ __forceinline__ void cp_wait() {
 // A unit is 16 columns of dv of one head; four warps work on it, one per SM sub-partition.  Transposed, the state
 // S^T [16][dk] is an m16 product's accumulator: warp w keeps the quarter w of dk in registers, and owns the tokens
 // 16 w .. 16 w + 15 of a chunk.  What all four need (the state, then the chunk's right-hand side, then U) goes
-// through shared memory as fp16 A fragments, 16 columns of k at a time, each with a power of two per row, so no
-// warp waits for another's row maximum: the products of a block of k are summed apart and added in fp32.
+// through shared memory as fp16 A fragments, each warp's with a power of two of its own, so no warp waits for
+// another's largest entry: the products of a block of k are summed apart and added in fp32.
 // Three barriers a chunk.  A block holds NU units that share the staged tiles.
 template <int C, int DKP, int NPK, int NPP>
 struct DeltaStage {
@@ -331,22 +322,22 @@ struct DeltaStage {
     }
 };
 
-// A fragments in shared memory: [block][piece][lane] 16 bytes, and per block the 16 rows' down-scales
+// A fragments in shared memory: [block][piece][lane] 16 bytes, and per block what they are times
 template <int NBLK, int NP>
 struct FragBuf {
-    static constexpr int BYTES = NBLK * (NP * 512 + 64);
-    static __device__ __forceinline__ void put(unsigned char* base, int blk, int lane, const float (&t0)[4],
-                                               const float (&t1)[4], const float (&up)[2], const float (&dn)[2]) {
-        uint32_t a[NP][4];
-        frag_pieces<NP>(t0, t1, up, a);
+    static constexpr int BYTES = NBLK * NP * 512 + 64;
+    static __device__ __forceinline__ void put(unsigned char* base, int blk, int lane, const uint32_t (*a)[4],
+                                               float down) {
 #pragma unroll
         for (int p = 0; p < NP; p++)
             *(uint4*)(base + (blk * NP + p) * 512 + lane * 16) = make_uint4(a[p][0], a[p][1], a[p][2], a[p][3]);
-        if ((lane & 3) == 0) {
-            float* s = (float*)(base + NBLK * NP * 512) + blk * 16;
-            s[lane >> 2] = dn[0];
-            s[(lane >> 2) + 8] = dn[1];
-        }
+        if (lane == 0) ((float*)(base + NBLK * NP * 512))[blk] = down;
+    }
+    static __device__ __forceinline__ void put(unsigned char* base, int blk, int lane, const float (&t)[2][4],
+                                               float up, float down) {
+        uint32_t a[NP][4];
+        frag_pieces<NP>(t[0], t[1], up, a);
+        put(base, blk, lane, a, down);
     }
     // first N of the block's pieces
     template <int N>
@@ -357,27 +348,22 @@ struct FragBuf {
             a[p][0] = v.x; a[p][1] = v.y; a[p][2] = v.z; a[p][3] = v.w;
         }
     }
-    static __device__ __forceinline__ void scale(const unsigned char* base, int blk, int lane, float (&dn)[2]) {
-        const float* s = (const float*)(base + NBLK * NP * 512) + blk * 16;
-        dn[0] = s[lane >> 2];
-        dn[1] = s[(lane >> 2) + 8];
+    static __device__ __forceinline__ float scale(const unsigned char* base, int blk) {
+        return ((const float*)(base + NBLK * NP * 512))[blk];
     }
 };
-// Entries (r, c) (r, c + 1) and (r + 8, ...) of an accumulator tile at column `col` of a 16-row tile in global memory,
-// W columns wide, NP pieces `piece` halves apart
+// A fragment pieces of one block as rows of a 16-row tile in global memory (columns col .. col + 15), W columns wide
 template <int NP, int W>
-__device__ __forceinline__ void put_tile(__half* base, size_t piece, int lane, int col, const float (&t)[4], float up) {
-    const int c = col + (lane & 3) * 2;
+__device__ __forceinline__ void put_frag(__half* base, size_t piece, int lane, int col, const uint32_t (*a)[4]) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        uint32_t p[NP];
-        split_pair<NP>(t[2 * h] * up, t[2 * h + 1] * up, p);
-        const uint32_t o = W == 64 ? tile_off<64>((lane >> 2) + 8 * h, c) : wide_off<16>((lane >> 2) + 8 * h, c);
+    for (int i = 0; i < 4; i++) {
+        const int row = (lane >> 2) + 8 * (i & 1), c = col + 8 * (i >> 1) + (lane & 3) * 2;
+        const uint32_t o = W == 64 ? tile_off<64>(row, c) : wide_off<16>(row, c);
 #pragma unroll
-        for (int k = 0; k < NP; k++) *(uint32_t*)((char*)(base + k * piece) + o) = p[k];
+        for (int k = 0; k < NP; k++) *(uint32_t*)((char*)(base + k * piece) + o) = a[k][i];
     }
 }
-// the same entries, both pieces as they are
+// entries (r, c) (r, c + 1) and (r + 8, ...) of an accumulator tile, both pieces as they are
 template <int W>
 __device__ __forceinline__ void get_tile(const __half* base, size_t piece, int lane, int col, uint32_t (&v)[2][2]) {
     const int c = col + (lane & 3) * 2;
@@ -401,13 +387,13 @@ __device__ __forceinline__ void zero(float (&t)[N][4]) {
 #pragma unroll
         for (int e = 0; e < 4; e++) t[i][e] = 0.0f;
 }
-// acc += part * f[row]
+// acc += f part
 template <int N>
-__device__ __forceinline__ void add_scaled(float (&acc)[N][4], const float (&part)[N][4], const float (&f)[2]) {
+__device__ __forceinline__ void add_scaled(float (&acc)[N][4], const float (&part)[N][4], float f) {
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[i][e] = fmaf(part[i][e], f[e >> 1], acc[i][e]);
+        for (int e = 0; e < 4; e++) acc[i][e] = fmaf(part[i][e], f, acc[i][e]);
 }
 __device__ __forceinline__ void unit_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
 
