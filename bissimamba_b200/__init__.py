@@ -528,6 +528,7 @@ def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=No
     p.h0, p.hT = _ptr(h0), _ptr(hT)
     p.ld_q, p.ld_k, p.ld_v, p.ld_o = (_rows_ld(t, 2, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
     p._keep = (q, k, v, g, beta, o, h0, hT, cu_seqlens)
+    p._entry = Hv * dk * dv
     return p
 
 
@@ -556,18 +557,22 @@ def delta_grads(p, do, dq, dk, dv, dg=None, dbeta=None, dh0=None, dhT=None):
 
 def delta_forward(p, ws, keep=False, stream=None):
     """Chunked gated delta rule; keep=True leaves in ws (a training workspace) what delta_backward reads."""
-    check(lib().kmb_delta_forward(C.byref(p), ws.data_ptr(), int(bool(keep)), stream), "kmb_delta_forward")
+    if (_lib or lib()).kmb_delta_forward(p, ws.data_ptr(), 1 if keep else 0, stream):
+        check(-1, "kmb_delta_forward")
 
 
 def delta_backward(p, grads, ws, stream=None):
-    check(lib().kmb_delta_backward(C.byref(p), C.byref(grads), ws.data_ptr(), stream), "kmb_delta_backward")
+    if (_lib or lib()).kmb_delta_backward(p, grads, ws.data_ptr(), stream):
+        check(-1, "kmb_delta_backward")
 
 
 def delta_step(p, pool, slots=None, stream=None):
     """Recurrent form: the T tokens of each row against its state in pool [entries, Hv, dk, dv], updated in place."""
-    if pool.shape[1:] != (p.Hv, p.dk, p.dv) or not pool.is_contiguous():
+    n = len(pool)
+    if pool.numel() != n * p._entry or not pool.is_contiguous():
         raise ValueError("pool: a contiguous [entries, Hv, dk, dv] tensor is expected")
-    check(lib().kmb_delta_step(C.byref(p), pool.data_ptr(), pool.shape[0], _ptr(slots), stream), "kmb_delta_step")
+    if (_lib or lib()).kmb_delta_step(p, pool.data_ptr(), n, None if slots is None else slots.data_ptr(), stream):
+        check(-1, "kmb_delta_step")
 
 
 def norm_params(x, w, b, y, eps=1e-5, residual=None, total=None, stats=None):
@@ -612,11 +617,13 @@ def norm_workspace_floats(p):
 
 
 def norm_forward(p, stream=None):
-    check(lib().kmb_layernorm_forward(C.byref(p), stream), "kmb_layernorm_forward")
+    if (_lib or lib()).kmb_layernorm_forward(p, stream):
+        check(-1, "kmb_layernorm_forward")
 
 
 def norm_backward(p, grads, ws=None, stream=None):
-    check(lib().kmb_layernorm_backward(C.byref(p), C.byref(grads), _ptr(ws), stream), "kmb_layernorm_backward")
+    if (_lib or lib()).kmb_layernorm_backward(p, grads, _ptr(ws), stream):
+        check(-1, "kmb_layernorm_backward")
 
 
 def grad_list(grads, outs=None):
@@ -639,7 +646,8 @@ def grad_clip_workspace_floats(lst):
 
 def grad_clip(lst, max_norm, result, ws, stream=None):
     """Global norm of a grad_list and clipping by it; result: float32 [2], norm and coefficient."""
-    check(lib().kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream), "kmb_grad_clip")
+    if (_lib or lib()).kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream):
+        check(-1, "kmb_grad_clip")
 
 
 class DeviceArray:

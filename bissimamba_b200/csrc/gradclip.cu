@@ -14,14 +14,15 @@
 // whose squares are subnormal) it is taken again in 64 bits.  One partial sum per
 // block, added in block order by every block of the second pass: no atomics.
 //
-// The second pass walks the chunks from the last to the first: what the first
-// pass read last is still in L2 when the second begins.  It does nothing for a
+// A block takes a run of chunks, the second pass from the last to the first:
+// what the first pass read last is still in L2 when the second begins.  It does nothing for a
 // tensor that is scaled in place by 1.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cmath>
 #include <cstdint>
 #include "../../include/kmamba_clip.h"
+#include "kmb_launch.cuh"
 
 namespace kmb {
 int set_error(const char* msg);
@@ -53,6 +54,8 @@ __device__ __forceinline__ int head_of(const void* p, int esz, long long n) {
     const int h = (int)(((16 - ((uintptr_t)p & 15)) & 15) / esz);
     return (long long)h < n ? h : (int)n;
 }
+// chunks of this block: a run, so that the tensor of the next chunk is this one's or the one after
+__device__ __forceinline__ int run_start(int chunks, int b) { return (int)((long long)chunks * b / gridDim.x); }
 template <int CAP>
 __device__ __forceinline__ int find_tensor(const GcList<CAP>& l, int chunk) {
     int a = 0, b = l.count;   // last tensor whose first chunk is <= chunk and that has chunks
@@ -98,14 +101,18 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
 // squares of `cnt` 16-byte pieces: fp32 within the call, 64 bits across calls
 __device__ __forceinline__ double squares(const uint4* r, int cnt, bool bf) {
     float s = 0.0f;
-    bool any = false;
-    for (int k = 0; k < cnt; k++) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (k >= cnt) break;
         float v[8];
         unpack(r[k], bf, v);
+        any |= r[k].x | r[k].y | r[k].z | r[k].w;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            s = fmaf(v[i], v[i], s);
-            any |= v[i] != 0.0f;
+        for (int i = 0; i < 4; i++) s = fmaf(v[i], v[i], s);
+        if (bf) {
+#pragma unroll
+            for (int i = 4; i < 8; i++) s = fmaf(v[i], v[i], s);
         }
     }
     // between 2^-60 and 2^120 no square that matters was rounded to a subnormal and none overflowed (an
@@ -125,9 +132,12 @@ __global__ void __launch_bounds__(GC_THREADS)
 gc_norm_kernel(const __grid_constant__ GcList<CAP> l, double* __restrict__ part) {
     __shared__ double sh[GC_THREADS / 32];
     double acc = 0.0;
+    pdl_release();
     const int chunks = l.first[l.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = find_tensor(l, c);
+    const int c0 = run_start(chunks, blockIdx.x), c1 = run_start(chunks, blockIdx.x + 1);
+    int t = find_tensor(l, c0);
+    for (int c = c0; c < c1; c++) {
+        while (l.first[t + 1] <= c) t++;
         const GcTensor& x = l.t[t];
         const bool bf = l.bf16[t] != 0;
         const int esz = bf ? 2 : 4, vec = 16 / esz;
@@ -166,9 +176,9 @@ gc_norm_kernel(const __grid_constant__ GcList<CAP> l, double* __restrict__ part)
 
 template <int CAP>
 __global__ void __launch_bounds__(GC_THREADS)
-gc_scale_kernel(const __grid_constant__ GcList<CAP> l, const double* __restrict__ part, int nparts, float max_norm,
-                float* __restrict__ result) {
+gc_scale_kernel(const __grid_constant__ GcList<CAP> l, const double* part, int nparts, float max_norm, float* result) {
     __shared__ double sh[GC_THREADS / 32];
+    pdl_wait();
     double s = 0.0;
     for (int i = threadIdx.x; i < nparts; i += GC_THREADS) s += part[i];
     const double norm = sqrt(block_sum(s, sh));
@@ -179,9 +189,10 @@ gc_scale_kernel(const __grid_constant__ GcList<CAP> l, const double* __restrict_
         result[1] = coef;
     }
     const int chunks = l.first[l.count];
-    for (int cc = blockIdx.x; cc < chunks; cc += gridDim.x) {
-        const int c = chunks - 1 - cc;
-        const int t = find_tensor(l, c);
+    const int c0 = run_start(chunks, blockIdx.x), c1 = run_start(chunks, blockIdx.x + 1);
+    int t = c1 > c0 ? find_tensor(l, c1 - 1) : 0;
+    for (int c = c1 - 1; c >= c0; c--) {
+        while (l.first[t] > c) t--;
         const GcTensor& x = l.t[t];
         if (!x.out || (coef == 1.0f && x.out == x.in)) continue;
         const bool bf = l.bf16[t] != 0;
@@ -282,7 +293,8 @@ template <int CAP>
 cudaError_t clip_all(const KMBGradTensor* ts, long n, float max_norm, float* result, double* part, long max_parts,
                      cudaStream_t st, bool* too_long) {
     GcList<CAP> l;
-    int nparts = 0;
+    int nparts = 0, single = 0;
+    cudaError_t e = cudaSuccess;
     for (long i = 0; i < n;) {
         const long took = fill(l, ts, i, n);
         if (took == 0) { *too_long = true; return cudaSuccess; }
@@ -290,6 +302,7 @@ cudaError_t clip_all(const KMBGradTensor* ts, long n, float max_norm, float* res
             const int g = grid_of(l.first[l.count]);
             if (nparts + g > max_parts) return cudaErrorInvalidValue;
             gc_norm_kernel<CAP><<<g, GC_THREADS, 0, st>>>(l, part + nparts);
+            single++;
             nparts += g;
         }
         i += took;
@@ -297,13 +310,14 @@ cudaError_t clip_all(const KMBGradTensor* ts, long n, float max_norm, float* res
     bool first = true;
     for (long i = 0; i < n || first;) {   // an empty list still reports its norm
         const long took = fill(l, ts, i, n);
-        if (l.count || first)
-            gc_scale_kernel<CAP><<<grid_of(l.first[l.count]), GC_THREADS, 0, st>>>(l, part, nparts, max_norm,
-                                                                                   first ? result : nullptr);
+        // only the launch right behind the one sum may be set up while that runs
+        if ((l.count || first) && e == cudaSuccess)
+            e = launch(gc_scale_kernel<CAP>, dim3((unsigned)grid_of(l.first[l.count])), dim3(GC_THREADS), 0, st,
+                       first && single == 1, l, (const double*)part, nparts, max_norm, first ? result : (float*)nullptr);
         first = false;
         i += took;
     }
-    return cudaGetLastError();
+    return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 constexpr int GC_SMALL = 64;

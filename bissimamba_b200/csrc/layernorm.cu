@@ -5,19 +5,20 @@
 // backward s, dy, dtotal and dx, once each.  A row is read once into registers
 // and everything about it is computed there: the mean, then the centred square
 // sum (two passes over registers, so there is no cancellation), then the output.
-// Rows up to 1024 entries belong to one warp (no block barrier, the 8 warps of a
-// block run on independent rows); longer rows belong to a block.
+// Rows up to 512 entries belong to one warp (no block barrier, the 8 warps of a
+// block run on independent rows), longer rows to a block of 8 or 16 entries per
+// thread, so that enough warps fit an SM to keep its loads in flight.
 //
-// The weight's gradient is a sum over all rows: each warp keeps its lanes'
-// columns in registers over all of its rows (a block with long rows keeps them
-// in shared memory, every column owned by one thread), the block adds its warps
-// in order, and a second launch adds the blocks' partial sums in order.  No
-// atomics: the result does not depend on scheduling.
+// The weight's gradient is a sum over all rows: each thread keeps its columns in
+// registers over all of its rows, a block adds its warps in order, and a second
+// launch adds the blocks' partial sums in order.  No atomics: the result does
+// not depend on scheduling.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cmath>
 #include <cstdint>
 #include "../../include/kmamba_norm.h"
+#include "kmb_launch.cuh"
 
 namespace kmb {
 int set_error(const char* msg);
@@ -26,7 +27,11 @@ void clear_error();
 
 namespace {
 
-constexpr int LN_WARP_D = 1024;   // longest row of the warp kernels
+constexpr int LN_WARP_D = 512;    // longest row of the warp kernels
+constexpr int LN_BLOCK8_D = 8192; // longest row of blocks with 8 entries per thread
+#ifndef LN_BWD_BLOCKS
+#define LN_BWD_BLOCKS 2
+#endif
 constexpr int LN_WARPS = 8;       // rows in flight per block there
 
 struct LnDesc {
@@ -41,16 +46,41 @@ struct LnDesc {
     float* part;        // [blocks][2][D] partial dw, db
 };
 
-// VEC elements of T as they are in memory
-template <typename T, int VEC> struct Raw { T e[VEC]; };
-template <> struct __align__(16) Raw<float, 4> { float e[4]; };
-template <> struct __align__(16) Raw<__nv_bfloat16, 8> { __nv_bfloat16 e[8]; };
-template <> struct __align__(4) Raw<__nv_bfloat16, 2> { __nv_bfloat16 e[2]; };
-
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_f(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+
+// VEC elements of T as they are in memory (bf16 pairs stay packed: one register)
+template <typename T, int VEC> struct Raw {
+    T e[VEC];
+    __device__ __forceinline__ float get(int j) const { return to_f(e[j]); }
+    __device__ __forceinline__ void set(const float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) from_f(v[j], e[j]);
+    }
+};
+template <> struct __align__(16) Raw<float, 4> {
+    float e[4];
+    __device__ __forceinline__ float get(int j) const { return e[j]; }
+    __device__ __forceinline__ void set(const float (&v)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) e[j] = v[j];
+    }
+};
+template <> struct __align__(16) Raw<__nv_bfloat16, 8> {
+    uint32_t w[4];
+    __device__ __forceinline__ float get(int j) const {
+        return __uint_as_float((j & 1) ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> ld_raw(const T* p) {
@@ -68,6 +98,43 @@ __device__ __forceinline__ void ld_f(const float* p, float (&v)[VEC]) {
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[i] = p[i];
     }
+}
+
+// VEC columns from `col`, whose address is aligned; columns outside [0, D) read as 0 and are not written
+template <typename T, int VEC, bool ODD>
+__device__ __forceinline__ Raw<T, VEC> ld_cols(const T* row, int col, int D) {
+    if (!ODD || (col >= 0 && col + VEC <= D)) return ld_raw<T, VEC>(row + col);
+    Raw<T, VEC> r;
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = col + j >= 0 && col + j < D ? to_f(row[col + j]) : 0.0f;
+    r.set(v);
+    return r;
+}
+template <typename T, int VEC, bool ODD>
+__device__ __forceinline__ void st_cols(T* row, int col, int D, const Raw<T, VEC>& r) {
+    if (!ODD || (col >= 0 && col + VEC <= D)) {
+        *reinterpret_cast<Raw<T, VEC>*>(row + col) = r;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; j++)
+        if (col + j >= 0 && col + j < D) from_f(r.get(j), row[col + j]);
+}
+template <int VEC, bool ODD>
+__device__ __forceinline__ void ld_w(const float* p, int col, int D, float (&v)[VEC]) {
+    if constexpr (!ODD) {
+        ld_f<VEC>(p + col, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = col + j >= 0 && col + j < D ? p[col + j] : 0.0f;
+    }
+}
+// Entries between a 16-byte boundary and the start of a row: its chunks start that many columns early.  The rows of a
+// thread are a multiple of 8 apart, so it is the same for all of them.
+template <typename T, bool ODD>
+__device__ __forceinline__ int early(const T* row) {
+    return ODD ? (int)(((uintptr_t)row & 15) / sizeof(T)) : 0;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -91,7 +158,7 @@ __device__ __forceinline__ float row_sum(float v, float* sh) {
 }
 
 // NCH chunks of VEC consecutive columns per thread, chunks TPR * VEC columns apart.
-template <typename T, int VEC, int NCH, bool BLOCK>
+template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 32 * LN_WARPS)
 ln_fwd_kernel(const LnDesc d) {
     __shared__ float sh[32];
@@ -102,33 +169,33 @@ ln_fwd_kernel(const LnDesc d) {
     if (row >= d.rows) return;   // warps of their own, or the whole block
     const T* x = (const T*)d.x + row * d.ld_x;
     const T* r = (const T*)d.res + row * d.ld_res;
+    const int sft = early<T, ODD>(x);
     const bool has_res = d.res != nullptr;
+    const auto at = [&](int i) { return (i * tpr + lane) * VEC - sft; };
+    const auto in = [&](int c) { return ODD ? c >= 0 && c < d.D : true; };   // of a chunk that starts before D
     float v[NCH][VEC];
     {
         Raw<T, VEC> a[NCH], c[NCH];
 #pragma unroll
-        for (int i = 0; i < NCH; i++) {
-            const int col = (i * tpr + lane) * VEC;
-            if (col < d.D) a[i] = ld_raw<T, VEC>(x + col);
-        }
+        for (int i = 0; i < NCH; i++)
+            if (at(i) < d.D) a[i] = ld_cols<T, VEC, ODD>(x, at(i), d.D);
         if (has_res) {
 #pragma unroll
-            for (int i = 0; i < NCH; i++) {
-                const int col = (i * tpr + lane) * VEC;
-                if (col < d.D) c[i] = ld_raw<T, VEC>(r + col);
-            }
+            for (int i = 0; i < NCH; i++)
+                if (at(i) < d.D) c[i] = ld_cols<T, VEC, ODD>(r, at(i), d.D);
         }
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
-            const int col = (i * tpr + lane) * VEC;
-            if (col < d.D) {
+            if (at(i) < d.D) {
                 if (has_res) {
+                    float t[VEC];
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) from_f(to_f(a[i].e[j]) + to_f(c[i].e[j]), a[i].e[j]);
-                    if (d.tot) *reinterpret_cast<Raw<T, VEC>*>((T*)d.tot + row * d.ld_tot + col) = a[i];
+                    for (int j = 0; j < VEC; j++) t[j] = a[i].get(j) + c[i].get(j);
+                    a[i].set(t);
+                    if (d.tot) st_cols<T, VEC, ODD>((T*)d.tot + row * d.ld_tot, at(i), d.D, a[i]);
                 }
 #pragma unroll
-                for (int j = 0; j < VEC; j++) v[i][j] = to_f(a[i].e[j]);
+                for (int j = 0; j < VEC; j++) v[i][j] = a[i].get(j);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; j++) v[i][j] = 0.0f;
@@ -144,10 +211,10 @@ ln_fwd_kernel(const LnDesc d) {
     float q = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCH; i++)
-        if ((i * tpr + lane) * VEC < d.D) {
+        if (at(i) < d.D) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                v[i][j] -= mean;
+                v[i][j] = in(at(i) + j) ? v[i][j] - mean : 0.0f;
                 q = fmaf(v[i][j], v[i][j], q);
             }
         }
@@ -159,104 +226,87 @@ ln_fwd_kernel(const LnDesc d) {
     T* y = (T*)d.y + row * d.ld_y;
 #pragma unroll
     for (int i = 0; i < NCH; i++) {
-        const int col = (i * tpr + lane) * VEC;
-        if (col < d.D) {
+        if (at(i) < d.D) {
             float w[VEC], b[VEC];
+            float y8[VEC];
             Raw<T, VEC> o;
-            if (d.w) ld_f<VEC>(d.w + col, w);
-            if (d.b) ld_f<VEC>(d.b + col, b);
+            if (d.w) ld_w<VEC, ODD>(d.w, at(i), d.D, w);
+            if (d.b) ld_w<VEC, ODD>(d.b, at(i), d.D, b);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 const float h = v[i][j] * rstd;
-                from_f(fmaf(h, d.w ? w[j] : 1.0f, d.b ? b[j] : 0.0f), o.e[j]);
+                y8[j] = fmaf(h, d.w ? w[j] : 1.0f, d.b ? b[j] : 0.0f);
             }
-            *reinterpret_cast<Raw<T, VEC>*>(y + col) = o;
+            o.set(y8);
+            st_cols<T, VEC, ODD>(y, at(i), d.D, o);
         }
     }
 }
 
 // Backward.  Blocks walk rows with the grid's stride.  A row stays in registers as it is in memory (bf16: half
 // the registers), the normalised entries are computed twice; where registers allow it (PRE) the next row's loads
-// are issued before this row's sums.
+// are in flight while this row is worked on (two row buffers in turn).
 template <typename T, int VEC, int NCH, bool BLOCK>
 struct LnBwd {
     static constexpr int E = NCH * VEC;
-    static constexpr bool PRE = !BLOCK && E * (int)sizeof(T) <= 32;
-    static constexpr int MIN_BLOCKS = BLOCK ? 1 : E <= 16 ? 2 : 1;
+    static constexpr bool PRE = !BLOCK && LN_BWD_BLOCKS == 2 && E * (int)sizeof(T) <= 32;
+    static constexpr int MIN_BLOCKS = BLOCK ? 1 : LN_BWD_BLOCKS;
 };
-template <typename T, int VEC, int NCH, bool BLOCK>
+template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 32 * LN_WARPS, (LnBwd<T, VEC, NCH, BLOCK>::MIN_BLOCKS))
 ln_bwd_kernel(const LnDesc d) {
     constexpr bool PRE = LnBwd<T, VEC, NCH, BLOCK>::PRE;
-    extern __shared__ float dynsh[];   // BLOCK: dw, db sums [2][D]; else [2][D] to add the warps in
+    extern __shared__ float dynsh[];   // warp rows: [2][D] to add the warps in
     __shared__ float sh[32];
     const int lane = BLOCK ? threadIdx.x : (threadIdx.x & 31);
     const int warp = threadIdx.x >> 5;
     const int tpr = BLOCK ? blockDim.x : 32;
     const long long first = BLOCK ? (long long)blockIdx.x : (long long)blockIdx.x * LN_WARPS + warp;
     const long long step = BLOCK ? (long long)gridDim.x : (long long)gridDim.x * LN_WARPS;
-    constexpr int NA = BLOCK ? 1 : NCH;
-    float aw[NA][VEC], ab[NA][VEC];
-    if constexpr (BLOCK) {
-        for (int i = threadIdx.x; i < 2 * d.D; i += blockDim.x) dynsh[i] = 0.0f;
-        __syncthreads();
-    } else {
+    // (a thread of a row that does not exist reads nothing)
+    const int sft = early<T, ODD>((const T*)d.x + first * d.ld_x);
+    const auto at = [&](int i) { return (i * tpr + lane) * VEC - sft; };
+    const auto in = [&](int c) { return ODD ? c >= 0 && c < d.D : true; };
+    float aw[NCH][VEC], ab[NCH][VEC];
+    pdl_release();
 #pragma unroll
-        for (int i = 0; i < NA; i++)
+    for (int i = 0; i < NCH; i++)
 #pragma unroll
-            for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f;
-    }
+        for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f;
     struct Row {
         Raw<T, VEC> s[NCH], dy[NCH], t[NCH];
         float mean, rstd;
     };
+    const bool has_t = d.dtot != nullptr;
     auto load = [&](long long row, Row& r) {
         const T* s = (const T*)d.x + row * d.ld_x;
         const T* dy = (const T*)d.dy + row * d.ld_dy;
+        const T* t = (const T*)d.dtot + row * d.ld_dtot;
 #pragma unroll
-        for (int i = 0; i < NCH; i++) {
-            const int col = (i * tpr + lane) * VEC;
-            if (col < d.D) {
-                r.s[i] = ld_raw<T, VEC>(s + col);
-                r.dy[i] = ld_raw<T, VEC>(dy + col);
+        for (int i = 0; i < NCH; i++)
+            if (at(i) < d.D) {
+                r.s[i] = ld_cols<T, VEC, ODD>(s, at(i), d.D);
+                r.dy[i] = ld_cols<T, VEC, ODD>(dy, at(i), d.D);
+                if (has_t) r.t[i] = ld_cols<T, VEC, ODD>(t, at(i), d.D);
             }
-        }
-        if (d.dtot) {
-            const T* t = (const T*)d.dtot + row * d.ld_dtot;
-#pragma unroll
-            for (int i = 0; i < NCH; i++) {
-                const int col = (i * tpr + lane) * VEC;
-                if (col < d.D) r.t[i] = ld_raw<T, VEC>(t + col);
-            }
-        }
         r.mean = d.mean[row];
         r.rstd = d.rstd[row];
     };
-    Row cur, nxt;
-    if (PRE && first < d.rows) load(first, cur);
-    for (long long row = first; row < d.rows; row += step) {
-        if (!PRE) load(row, cur);
-        // dx may be dy or dtotal: the next row belongs to these threads alone, nobody writes it before they read it
-        if (PRE && row + step < d.rows) load(row + step, nxt);
+    auto work = [&](long long row, const Row& cur) {
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
-            const int col = (i * tpr + lane) * VEC;
+            const int col = at(i);
             if (col < d.D) {
                 float w[VEC];
-                if (d.w) ld_f<VEC>(d.w + col, w);
+                if (d.w) ld_w<VEC, ODD>(d.w, col, d.D, w);
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float xh = (to_f(cur.s[i].e[j]) - cur.mean) * cur.rstd;
-                    const float dy = to_f(cur.dy[i].e[j]);
-                    if constexpr (BLOCK) {
-                        dynsh[col + j] += dy * xh;
-                        dynsh[d.D + col + j] += dy;
-                    } else {
-                        aw[i][j] = fmaf(dy, xh, aw[i][j]);
-                        ab[i][j] += dy;
-                    }
-                    const float g = d.w ? dy * w[j] : dy;
+                    const float xh = (cur.s[i].get(j) - cur.mean) * cur.rstd;
+                    const float dy = cur.dy[i].get(j);   // 0 outside the row
+                    aw[i][j] = fmaf(dy, xh, aw[i][j]);
+                    ab[i][j] += dy;
+                    const float g = d.w ? __fmul_rn(dy, w[j]) : dy;
                     s1 += g;
                     s2 = fmaf(g, xh, s2);
                 }
@@ -264,44 +314,73 @@ ln_bwd_kernel(const LnDesc d) {
         }
         s1 = row_sum<BLOCK>(s1, sh) / (float)d.D;
         s2 = row_sum<BLOCK>(s2, sh) / (float)d.D;
+        if (!d.dx) return;
         T* dx = (T*)d.dx + row * d.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
-            const int col = (i * tpr + lane) * VEC;
-            if (col < d.D && d.dx) {
+            const int col = at(i);
+            if (col < d.D) {
                 float w[VEC];
-                if (d.w) ld_f<VEC>(d.w + col, w);
+                if (d.w) ld_w<VEC, ODD>(d.w, col, d.D, w);
+                float o8[VEC];
                 Raw<T, VEC> o;
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float xh = (to_f(cur.s[i].e[j]) - cur.mean) * cur.rstd;
-                    const float dy = to_f(cur.dy[i].e[j]);
-                    float v = cur.rstd * ((d.w ? dy * w[j] : dy) - s1 - xh * s2);
-                    if (d.dtot) v += to_f(cur.t[i].e[j]);
-                    from_f(v, o.e[j]);
+                    const float xh = (cur.s[i].get(j) - cur.mean) * cur.rstd;
+                    const float dy = cur.dy[i].get(j);
+                    // the product is rounded as in the sums: two columns (or one) cancel to what eps leaves
+                    o8[j] = cur.rstd * ((d.w ? __fmul_rn(dy, w[j]) : dy) - s1 - xh * s2);
+                    if (has_t) o8[j] += cur.t[i].get(j);
                 }
-                *reinterpret_cast<Raw<T, VEC>*>(dx + col) = o;
+                o.set(o8);
+                st_cols<T, VEC, ODD>(dx, col, d.D, o);
             }
         }
-        if (PRE) cur = nxt;
+    };
+    if constexpr (PRE) {
+        // dx may be dy or dtotal: the next row belongs to these threads alone, nobody writes it before they read it
+        Row a, b;
+        if (first < d.rows) load(first, a);
+        for (long long row = first; row < d.rows; row += 2 * step) {
+            if (row + step < d.rows) load(row + step, b);
+            work(row, a);
+            if (row + step >= d.rows) break;
+            if (row + 2 * step < d.rows) load(row + 2 * step, a);
+            work(row + step, b);
+        }
+    } else {
+        Row a;
+        for (long long row = first; row < d.rows; row += step) {
+            load(row, a);
+            work(row, a);
+        }
     }
     if (!d.part) return;
     float* part = d.part + (size_t)blockIdx.x * 2 * d.D;
     if constexpr (BLOCK) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * d.D; i += blockDim.x) part[i] = dynsh[i];
+#pragma unroll
+        for (int i = 0; i < NCH; i++)
+            if (at(i) < d.D) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if (in(at(i) + j)) {
+                        part[at(i) + j] = aw[i][j];
+                        part[d.D + at(i) + j] = ab[i][j];
+                    }
+            }
     } else {
         for (int k = 0; k < LN_WARPS; k++) {   // the warps add in order
             if (warp == k) {
 #pragma unroll
-                for (int i = 0; i < NA; i++) {
-                    const int col = (i * tpr + lane) * VEC;
+                for (int i = 0; i < NCH; i++) {
+                    const int col = at(i);
                     if (col < d.D) {
 #pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            dynsh[col + j] = k ? dynsh[col + j] + aw[i][j] : aw[i][j];
-                            dynsh[d.D + col + j] = k ? dynsh[d.D + col + j] + ab[i][j] : ab[i][j];
-                        }
+                        for (int j = 0; j < VEC; j++)
+                            if (in(col + j)) {
+                                dynsh[col + j] = k ? dynsh[col + j] + aw[i][j] : aw[i][j];
+                                dynsh[d.D + col + j] = k ? dynsh[d.D + col + j] + ab[i][j] : ab[i][j];
+                            }
                     }
                 }
             }
@@ -311,21 +390,29 @@ ln_bwd_kernel(const LnDesc d) {
     }
 }
 
-// dw[c], db[c] (+)= sum over the blocks' partial sums, in order: 32 columns per
-// block, 8 interleaved runs of blocks each, the runs added in order.
-__global__ void ln_reduce_kernel(const float* __restrict__ part, int nb, int D, float* __restrict__ dw,
-                                 float* __restrict__ db, int accumulate) {
-    __shared__ float sh[8][33];
+// dw[c], db[c] (+)= sum over the blocks' partial sums, in a fixed order: 32 columns per block, 32 interleaved runs of
+// the partial sums, four loads of each in flight, the runs added in order.
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int nb, int D, float* dw, float* db,
+                                                         int accumulate) {
+    __shared__ float sh[32][33];
+    pdl_wait();
     const int c = blockIdx.x * 32 + threadIdx.x, g = threadIdx.y;
     float v = 0.0f;
-    if (c < 2 * D)
-        for (int b = g; b < nb; b += 8) v += part[(size_t)b * 2 * D + c];
+    if (c < 2 * D) {
+        int b = g;
+        for (; b + 96 < nb; b += 128) {
+            const float* p = part + (size_t)b * 2 * D + c;
+            const size_t s = (size_t)64 * D;
+            v += (p[0] + p[s]) + (p[2 * s] + p[3 * s]);
+        }
+        for (; b < nb; b += 32) v += part[(size_t)b * 2 * D + c];
+    }
     sh[g][threadIdx.x] = v;
     __syncthreads();
     if (g == 0 && c < 2 * D) {
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) s += sh[k][threadIdx.x];
+        for (int k = 0; k < 32; k++) s += sh[k][threadIdx.x];
         float* o = c < D ? dw : db;
         const int i = c < D ? c : c - D;
         if (o) o[i] = accumulate ? o[i] + s : s;
@@ -340,73 +427,96 @@ int sm_count() {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// vector form: every row of every tensor starts on 16 bytes
+// How rows are read: 0 = in 16-byte pieces, every row of every tensor starts on 16 bytes; 1 = in 16-byte pieces
+// that start before the row, all tensors' rows being off the boundary by the same amount; 2 = by single entries.
 template <typename T>
-bool vec_ok(const LnDesc& d, bool bwd) {
+int row_form(const LnDesc& d, bool bwd) {
     const int V = 16 / (int)sizeof(T);
-    if (d.D % V || !aligned16(d.x) || d.ld_x % V || !aligned16(d.w)) return false;
-    if (bwd) return aligned16(d.dy) && d.ld_dy % V == 0 && aligned16(d.dtot) && (!d.dtot || d.ld_dtot % V == 0) &&
-                    aligned16(d.dx) && (!d.dx || d.ld_dx % V == 0);
-    return aligned16(d.b) && aligned16(d.res) && (!d.res || d.ld_res % V == 0) && aligned16(d.tot) &&
-           (!d.tot || d.ld_tot % V == 0) && aligned16(d.y) && d.ld_y % V == 0;
+    const void* p[5] = {d.x, bwd ? d.dy : d.res, bwd ? d.dtot : d.tot, bwd ? d.dx : d.y, nullptr};
+    const long long ld[5] = {d.ld_x, bwd ? d.ld_dy : d.ld_res, bwd ? d.ld_dtot : d.ld_tot, bwd ? d.ld_dx : d.ld_y, 0};
+    bool even = d.D % V == 0 && aligned16(d.w) && (bwd || aligned16(d.b)), alike = true;
+    for (int i = 0; i < 4; i++) {
+        if (!p[i]) continue;
+        even = even && aligned16(p[i]) && ld[i] % V == 0;
+        alike = alike && (((uintptr_t)p[i] ^ (uintptr_t)d.x) & 15) == 0 && (ld[i] - d.ld_x) % V == 0 &&
+                ((uintptr_t)p[i] % sizeof(T)) == 0;
+    }
+    return even ? 0 : alike ? 1 : 2;
 }
 
-// Blocks of the backward: enough to fill the device once (two warp blocks per SM, one long-row block), no
-// more than there are rows: the partial sums of dw and db grow with them.
-int bwd_blocks(long long rows, int D) {
-    const long long cap = D <= LN_WARP_D ? 2LL * sm_count() : (long long)sm_count();
-    const long long want = D <= LN_WARP_D ? (rows + LN_WARPS - 1) / LN_WARPS : rows;
+int block_entries(int D) { return D <= LN_BLOCK8_D ? 8 : 16; }
+int block_threads(int D) {
+    const int t = ((D + block_entries(D) - 1) / block_entries(D) + 31) & ~31;
+    return t < 64 ? 64 : t > 1024 ? 1024 : t;
+}
+// Blocks of the backward: enough to fill the device once (the partial sums of dw and db grow with them), a multiple
+// of 8 where they walk several rows.  span: columns that a row's chunks cover.
+int bwd_blocks(long long rows, int span) {
+    long long per_sm = LN_BWD_BLOCKS, want = (rows + LN_WARPS - 1) / LN_WARPS;
+    if (span > LN_WARP_D) {
+        per_sm = 1024 / block_threads(span);
+        per_sm = per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm;
+        want = rows;
+    }
+    const long long cap = (per_sm * sm_count() + 7) & ~7LL;
     return (int)(want < cap ? (want > 0 ? want : 1) : cap);
 }
-int block_threads(int D) {   // 16 entries per thread
-    int t = ((D + 15) / 16 + 31) & ~31;
-    return t < 64 ? 64 : t;
+template <typename T>
+int span_of(const LnDesc& d, int form) { return d.D + (form == 1 ? 16 / (int)sizeof(T) - 1 : 0); }
+template <typename T, bool BWD>
+int form_of(const LnDesc& d) {
+    const int form = row_form<T>(d, BWD);
+    // the longest rows would need more threads than a block has
+    return form == 1 && span_of<T>(d, 1) > KMB_NORM_MAX_D ? 2 : form;
 }
 
-template <typename T, int VEC, int NCH, bool BLOCK>
+template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 cudaError_t fwd_go(const LnDesc& d, cudaStream_t st) {
     const long long blocks = BLOCK ? d.rows : (d.rows + LN_WARPS - 1) / LN_WARPS;
-    ln_fwd_kernel<T, VEC, NCH, BLOCK><<<(unsigned)blocks, BLOCK ? block_threads(d.D) : 32 * LN_WARPS, 0, st>>>(d);
+    const int threads = BLOCK ? block_threads(d.D + (ODD ? VEC - 1 : 0)) : 32 * LN_WARPS;
+    ln_fwd_kernel<T, VEC, NCH, BLOCK, ODD><<<(unsigned)blocks, threads, 0, st>>>(d);
     return cudaGetLastError();
 }
-template <typename T, int VEC, int NCH, bool BLOCK>
+template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 cudaError_t bwd_go(const LnDesc& d, cudaStream_t st) {
-    const size_t sm = (size_t)2 * d.D * sizeof(float);
-    if (sm > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(ln_bwd_kernel<T, VEC, NCH, BLOCK>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
-        if (e != cudaSuccess) return e;
-    }
-    ln_bwd_kernel<T, VEC, NCH, BLOCK><<<bwd_blocks(d.rows, d.D), BLOCK ? block_threads(d.D) : 32 * LN_WARPS, sm,
-                                        st>>>(d);
+    const size_t sm = BLOCK ? 0 : (size_t)2 * d.D * sizeof(float);
+    const int threads = BLOCK ? block_threads(d.D + (ODD ? VEC - 1 : 0)) : 32 * LN_WARPS;
+    ln_bwd_kernel<T, VEC, NCH, BLOCK, ODD><<<bwd_blocks(d.rows, d.D + (ODD ? VEC - 1 : 0)), threads, sm, st>>>(d);
     return cudaGetLastError();
 }
 
-template <typename T, int VEC, bool BWD>
+template <typename T, int VEC, bool BWD, bool ODD>
 cudaError_t pick(const LnDesc& d, cudaStream_t st) {
-    if (d.D > LN_WARP_D) {
-        if constexpr (BWD) return bwd_go<T, VEC, 16 / VEC, true>(d, st);
-        else return fwd_go<T, VEC, 16 / VEC, true>(d, st);
+    const int D = d.D + (ODD ? VEC - 1 : 0);   // columns that the chunks may have to span
+    if (D > LN_WARP_D) {
+        if (block_entries(D) == 16) {
+            if constexpr (BWD) return bwd_go<T, VEC, 16 / VEC, true, ODD>(d, st);
+            else return fwd_go<T, VEC, 16 / VEC, true, ODD>(d, st);
+        }
+        if constexpr (BWD) return bwd_go<T, VEC, 8 / VEC, true, ODD>(d, st);
+        else return fwd_go<T, VEC, 8 / VEC, true, ODD>(d, st);
     }
-    // entries per lane: 8, 16 or 32
-#define KMB_LN_GO(E)                                                  \
-    {                                                                 \
-        if constexpr (BWD) return bwd_go<T, VEC, E / VEC, false>(d, st); \
-        else return fwd_go<T, VEC, E / VEC, false>(d, st);            \
+    // entries per lane: 8 or 16
+#define KMB_LN_GO(E)                                                       \
+    {                                                                      \
+        if constexpr (BWD) return bwd_go<T, VEC, E / VEC, false, ODD>(d, st); \
+        else return fwd_go<T, VEC, E / VEC, false, ODD>(d, st);            \
     }
-    if (d.D <= 256) KMB_LN_GO(8)
-    if (d.D <= 512) KMB_LN_GO(16)
-    KMB_LN_GO(32)
+    if (D <= 256) KMB_LN_GO(8)
+    KMB_LN_GO(16)
 #undef KMB_LN_GO
+}
+template <typename T, bool BWD>
+cudaError_t dispatch_t(const LnDesc& d, cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int form = form_of<T, BWD>(d);
+    if (form == 0) return pick<T, V, BWD, false>(d, st);
+    if (form == 1) return pick<T, V, BWD, true>(d, st);
+    return pick<T, 1, BWD, false>(d, st);
 }
 template <bool BWD>
 cudaError_t dispatch(const LnDesc& d, int dtype, cudaStream_t st) {
-    if (dtype == KMB_DTYPE_BF16) {
-        if (vec_ok<__nv_bfloat16>(d, BWD)) return pick<__nv_bfloat16, 8, BWD>(d, st);
-        return pick<__nv_bfloat16, 1, BWD>(d, st);
-    }
-    if (vec_ok<float>(d, BWD)) return pick<float, 4, BWD>(d, st);
-    return pick<float, 1, BWD>(d, st);
+    return dtype == KMB_DTYPE_BF16 ? dispatch_t<__nv_bfloat16, BWD>(d, st) : dispatch_t<float, BWD>(d, st);
 }
 
 const char* check(const KMBNormParams* p) {
@@ -448,7 +558,9 @@ int kmb_layernorm_forward(const KMBNormParams* p, void* stream) {
 
 size_t kmb_layernorm_workspace_floats(const KMBNormParams* p) {
     if (check(p)) return 0;
-    return (size_t)bwd_blocks(p->rows, (int)p->D) * 2 * p->D;
+    // the larger of what rows on and off 16-byte boundaries take
+    const int a = bwd_blocks(p->rows, (int)p->D), b = bwd_blocks(p->rows, (int)p->D + 7);
+    return (size_t)(a > b ? a : b) * 2 * p->D;
 }
 
 int kmb_layernorm_backward(const KMBNormParams* p, const KMBNormGrads* g, float* ws, void* stream) {
@@ -481,9 +593,10 @@ int kmb_layernorm_backward(const KMBNormParams* p, const KMBNormGrads* g, float*
     d.part = wgrad ? ws : nullptr;
     cudaError_t e = dispatch<true>(d, p->dtype, st);
     if (e == cudaSuccess && wgrad) {
-        ln_reduce_kernel<<<(unsigned)((2 * p->D + 31) / 32), dim3(32, 8), 0, st>>>(
-            ws, bwd_blocks(p->rows, (int)p->D), (int)p->D, g->dw, g->db, g->accumulate);
-        e = cudaGetLastError();
+        const int span = p->dtype == KMB_DTYPE_BF16 ? span_of<__nv_bfloat16>(d, form_of<__nv_bfloat16, true>(d))
+                                                    : span_of<float>(d, form_of<float, true>(d));
+        e = launch(ln_reduce_kernel, dim3((unsigned)((2 * p->D + 31) / 32)), dim3(32, 32), 0, st, true, ws,
+                   bwd_blocks(p->rows, span), (int)p->D, g->dw, g->db, g->accumulate);
     }
     return e == cudaSuccess ? 0 : set_cuda_error("kmb_layernorm_backward", e);
 }
