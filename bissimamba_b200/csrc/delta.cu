@@ -14,11 +14,13 @@ int* device_status();
 namespace {
 
 // ------------------------------------------------------------------ packed sequences
+constexpr int kSortSeqs = 512;   // beyond that many sequences no single one matters
 // One block: offsets clamped to [0, total] and made non-decreasing (cu), and the first chunk of each sequence
 // (cstart).  Whatever the caller's offsets hold, the kernels stay inside the tensors.
 __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ in, int nseq, int total, int C,
-                                                       int* __restrict__ cu, int* __restrict__ cstart) {
-    __shared__ int sh[256];
+                                                       int* __restrict__ cu, int* __restrict__ cstart,
+                                                       int* __restrict__ order) {
+    __shared__ int sh[256], len[kSortSeqs];
     const int t = threadIdx.x;
     const int per = (nseq + 1 + 255) / 256;
     const int a = min(t * per, nseq + 1), b = min(a + per, nseq + 1);
@@ -55,6 +57,15 @@ __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ i
         cstart[i] = n;
         if (i < nseq) n += (cu[i + 1] - cu[i] + C - 1) / C;
     }
+    // the longest sequences first, so that none of them starts last (ranks by counting; ties keep their order)
+    if (nseq > kSortSeqs) return;
+    for (int i = t; i < nseq; i += 256) len[i] = cu[i + 1] - cu[i];
+    __syncthreads();
+    for (int i = t; i < nseq; i += 256) {
+        int rank = 0;
+        for (int j = 0; j < nseq; j++) rank += len[j] > len[i] || (len[j] == len[i] && j < i);
+        order[rank] = i;
+    }
 }
 
 // ------------------------------------------------------------------ per-chunk matrices
@@ -90,6 +101,19 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
     long long tok0;
     int cnt;
     if (!chunk_range<C>(d, chunk, tok0, cnt)) return;
+
+    // gates of the first head: in flight under the tiles' loads
+    float g2[2], b2[2];
+    const auto load_gates = [&](int hv) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = h * 32 + lane;
+            const long long at = (tok0 + i) * d.Hv + hv;
+            g2[h] = (d.g && i < cnt) ? d.g[at] : 0.0f;
+            b2[h] = i < cnt ? (d.beta ? d.beta[at] : 1.0f) : 0.0f;
+        }
+    };
+    if (warp < 2) load_gates(hk * d.grp);
 
     char* gK = (char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
     char* gQ = (char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
@@ -189,15 +213,22 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
         float* tk = d.tok + head * TOK_ROWS * C;
         __syncthreads();   // the last head's matrices are read
         if (warp == 0) {
-            running_sums(d, tok0, cnt, hv, lane, gam);
-        } else if (warp < 3) {
-            const int i = threadIdx.x - 32;
-            const float b = i < cnt ? (d.beta ? d.beta[(tok0 + i) * d.Hv + hv] : 1.0f) : 0.0f;
-            bet[i] = b;
-            tk[TOK_BETA * C + i] = b;
-            tk[TOK_FK * C + i] = fK[i];
-            tk[TOK_FQ * C + i] = fQ[i];
+            running_sums(g2[0], g2[1], lane, gam);
+            if (train) {
+                d.gam[head * C + lane] = gam[lane];
+                d.gam[head * C + lane + 32] = gam[lane + 32];
+            }
+        } else if (warp == 1) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int i = h * 32 + lane;
+                bet[i] = b2[h];
+                tk[TOK_BETA * C + i] = b2[h];
+                tk[TOK_FK * C + i] = fK[i];
+                tk[TOK_FQ * C + i] = fQ[i];
+            }
         }
+        if (warp < 2 && hh + 1 < d.grp) load_gates(hv + 1);
         __syncthreads();
         decay_tables(dec, threadIdx.x);
         if (threadIdx.x < C) {
@@ -565,6 +596,7 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     if (p->cu_seqlens) {
         d.cu = (const int*)take((size_t)(d.nseq + 1) * 4);
         d.cstart = (const int*)take((size_t)(d.nseq + 1) * 4);
+        if (d.nseq <= kSortSeqs) d.order = (const int*)take((size_t)d.nseq * 4);
     }
     const size_t ck = (size_t)d.nch * d.Hk, cv = (size_t)d.nch * d.Hv;
     d.Kt = (__half*)take(ck * NPK * C * DKP * 2);
@@ -575,6 +607,7 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     if (train) {
         const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
         d.Tt = (__half*)take(cv * 2 * C * C * 2);
+        d.gam = (double*)take(cv * C * 8);
         d.Sh = (__half*)take(u * 2 * DKP);
         d.Wh = (__half*)take(u * 2 * C);
         d.Of = (float*)take(u * 2 * C);
@@ -630,7 +663,7 @@ int kmb_delta_forward(const KMBDeltaParams* p, float* ws, int keep, void* stream
     d.status = device_status();
     cudaError_t e = cudaSuccess;
     if (d.cu) {
-        delta_cu_kernel<<<1, 256, 0, st>>>(d.cu_in, d.nseq, (int)d.total, kDeltaC, (int*)d.cu, (int*)d.cstart);
+        delta_cu_kernel<<<1, 256, 0, st>>>(d.cu_in, d.nseq, (int)d.total, kDeltaC, (int*)d.cu, (int*)d.cstart, (int*)d.order);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess && d.nch > 0) e = delta_prep(d, DKP, bf16, keep != 0, st);

@@ -43,7 +43,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     unsigned char *exG = exS + FS::BYTES, *exX = exG + FG::BYTES, *exE = exX + FX::BYTES, *exF = exE + FX::BYTES;
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
-    const int hv = (int)(blockIdx.x / ub) % d.Hv, n = (int)(blockIdx.x / ub) / d.Hv;
+    const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
+    const int n = d.order ? d.order[nr] : nr;
     const bool on = u < d.units;
     const int r = lane >> 2, c2 = (lane & 3) * 2;
     const int col[2] = {u * 16 + r, u * 16 + r + 8};
@@ -342,6 +343,45 @@ struct GradSmem {
     static constexpr int BYTES = oCol + 3 * 48 * 4;
 };
 
+// One warp: gradients of the gates of a chunk's tokens (lane and lane + 32) from the recurrence's sums over dv
+__device__ __forceinline__ void gate_grads(const DeltaDesc& d, size_t head, long long tok0, int cnt, int hv, int lane) {
+    constexpr int C = kDeltaC;
+    double anchor = lane < d.units * 4 ? (double)d.anchor[head * d.units * 4 + lane] : 0.0;
+    double t[2] = {0.0, 0.0};
+    float b[2] = {0.0f, 0.0f};
+#pragma unroll 4
+    for (int x = 0; x < d.units; x++) {
+        const float* p = d.part + (head * d.units + x) * 2 * C + lane;
+        const float v0 = p[0], v1 = p[32], v2 = p[C], v3 = p[C + 32];
+        t[0] += v0;
+        t[1] += v1;
+        b[0] += v2;
+        b[1] += v3;
+    }
+    double s[2] = {t[0], t[1]};
+#pragma unroll
+    for (int o = 16; o; o >>= 1) anchor += __shfl_xor_sync(0xffffffffu, anchor, o);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, s[0], o), y = __shfl_up_sync(0xffffffffu, s[1], o);
+        if (lane >= o) {
+            s[0] += x;
+            s[1] += y;
+        }
+    }
+    s[1] += __shfl_sync(0xffffffffu, s[0], 31);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int i = h * 32 + lane;
+        if (i >= cnt) continue;
+        const long long at = (tok0 + i) * d.Hv + hv;
+        // a decay below e^-104 is 0 in fp32: nothing depends on it
+        const bool reset = d.g && d.g[at] < -104.0f;
+        if (d.dg) d.dg[at] = reset ? 0.0f : (float)(anchor - (s[h] - t[h]));
+        if (d.dbeta) d.dbeta[at] = b[h];
+    }
+}
+
 template <int DKP, typename IO>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1)
 delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
@@ -403,40 +443,11 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             cp_commit();
         };
         __syncthreads();
+        for (int i = tid; i < TOK_ROWS * C / 4; i += 256) cp16(sb + SM::oTok + i * 16, d.tok + head * TOK_ROWS * C + i * 4);
+        for (int i = tid; i < d.units * MX_ROWS; i += 256) cp16(sb + SM::oMx + i * 16, d.mx + head * d.units * 4 * MX_ROWS + i * 4);
+        for (int i = tid; i < C / 2; i += 256) cp16(sb + SM::oGam + i * 16, d.gam + head * C + i * 2);
         slice(0);
-        for (int i = tid; i < TOK_ROWS * C; i += 256) tk[i] = d.tok[head * TOK_ROWS * C + i];
-        for (int i = tid; i < d.units * 4 * MX_ROWS; i += 256) mx[i] = d.mx[head * d.units * 4 * MX_ROWS + i];
-        if (warp == 0) {
-            running_sums(d, tok0, cnt, hv, lane, dec.gam);
-        } else if (warp == 1 && (d.dg || d.dbeta)) {
-            // gates: tokens lane and lane + 32
-            double before = 0.0, anchor = 0.0;
-            for (int x = 0; x < d.units * 4; x++) anchor += d.anchor[head * d.units * 4 + x];
-#pragma unroll
-            for (int h = 0; h < C / 32; h++) {
-                const int i = h * 32 + lane;
-                double t = 0.0;
-                float b = 0.0f;
-                for (int x = 0; x < d.units; x++) {
-                    t += d.part[((head * d.units + x) * 2) * C + i];
-                    b += d.part[((head * d.units + x) * 2 + 1) * C + i];
-                }
-                double s = t;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xffffffffu, s, o);
-                    if (lane >= o) s += y;
-                }
-                if (i < cnt) {
-                    const long long at = (tok0 + i) * d.Hv + hv;
-                    // a decay below e^-104 is 0 in fp32: nothing depends on it
-                    const bool reset = d.g && d.g[at] < -104.0f;
-                    if (d.dg) d.dg[at] = reset ? 0.0f : (float)(anchor - (before + s - t));
-                    if (d.dbeta) d.dbeta[at] = b;
-                }
-                before += __shfl_sync(0xffffffffu, s, 31);
-            }
-        }
+        cp_wait<0>();
         __syncthreads();
         decay_tables(dec, tid);
 
@@ -456,9 +467,9 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             if (u0) {
                 __syncthreads();
                 slice(u0);
+                cp_wait<0>();
+                __syncthreads();
             }
-            cp_wait<0>();
-            __syncthreads();
             const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
             for (int kk = 0; kk < nx; kk++) {
                 const float* m4 = mx + (u0 + kk) * 4 * MX_ROWS;
@@ -577,6 +588,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             }
         }
         __syncthreads();
+        if (warp == 1 && (d.dg || d.dbeta)) gate_grads(d, head, tok0, cnt, hv, lane);
         // the four products over tokens
 #pragma unroll
         for (int k = 0; k < 4; k++) {

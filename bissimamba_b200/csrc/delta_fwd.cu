@@ -30,7 +30,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     unsigned char *exX = exS + FS::BYTES, *exU = exX + FX::BYTES, *exO = exU + FX::BYTES;
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
-    const int hv = (int)(blockIdx.x / ub) % d.Hv, n = (int)(blockIdx.x / ub) / d.Hv;
+    const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
+    const int n = d.order ? d.order[nr] : nr;
     const bool on = u < d.units;                 // a unit past dv computes on zeros and stores nothing
     const int r = lane >> 2, c2 = (lane & 3) * 2;
     const int col[2] = {u * 16 + r, u * 16 + r + 8};

@@ -61,6 +61,8 @@ struct DeltaDesc {
     __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
     __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], on and below the diagonal blocks; Tt for training only
     float* tok;                  // [nch][Hv][TOK_ROWS][C], see TOK_*
+    double* gam;                 // [nch][Hv][C]: running sums of g (training)
+    const int* order;            // packed: sequences, the longest first (NULL: as they are)
     // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
     // scaled by a power of two (mx)
     __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [2][16 * C]
@@ -242,24 +244,18 @@ __device__ __forceinline__ bool chunk_range(const DeltaDesc& d, int chunk, long 
 // ------------------------------------------------------------------ decays inside a chunk
 // Running sums of g in 64 bits (lane holds tokens lane and lane + 32), -104 for anything below it: exp is 0 in fp32
 // there, and differences of the sums stay what G needs after a reset (g = -inf) too.
-__device__ __forceinline__ void running_sums(const DeltaDesc& d, long long tok0, int cnt, int hv, int lane,
-                                             double* gam) {
-    double carry = 0.0;
+__device__ __forceinline__ void running_sums(float g0, float g1, int lane, double* gam) {
+    double s[2] = {g0 < -104.0f ? -104.0f : g0, g1 < -104.0f ? -104.0f : g1};
 #pragma unroll
-    for (int h = 0; h < kDeltaC / 32; h++) {
-        const int i = h * 32 + lane;
-        float g = (d.g && i < cnt) ? d.g[(tok0 + i) * d.Hv + hv] : 0.0f;
-        if (g < -104.0f) g = -104.0f;
-        double s = g;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double t = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += t;
+    for (int o = 1; o < 32; o <<= 1) {
+        const double a = __shfl_up_sync(0xffffffffu, s[0], o), b = __shfl_up_sync(0xffffffffu, s[1], o);
+        if (lane >= o) {
+            s[0] += a;
+            s[1] += b;
         }
-        s += carry;
-        gam[i] = s;
-        carry = __shfl_sync(0xffffffffu, s, 31);
     }
+    gam[lane] = s[0];
+    gam[lane + 32] = s[1] + __shfl_sync(0xffffffffu, s[0], 31);
 }
 // G_ij = exp(gamma_i - gamma_j), j <= i.  Between blocks of 16 tokens it is the product of two decays that meet at
 // the end of the block before i's (both at most e^0 where g <= 0, so nothing overflows on the way).
