@@ -210,7 +210,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
     for (int hh = 0; hh < d.grp; hh++) {
         const int hv = hk * d.grp + hh;
         const size_t head = (size_t)chunk * d.Hv + hv;
-        float* tk = d.tok + head * TOK_ROWS * C;
+        float* tk = d.tok + head * TOK_SIZE;
         __syncthreads();   // the last head's matrices are read
         if (warp == 0) {
             running_sums(g2[0], g2[1], lane, gam);
@@ -603,7 +603,7 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     d.Qt = (__half*)take(ck * NPK * C * DKP * 2);
     d.Mt = (__half*)take(cv * 2 * C * C * 2);
     d.Pt = (__half*)take(cv * 2 * C * C * 2);
-    d.tok = (float*)take(cv * TOK_ROWS * C * 4);
+    d.tok = (float*)take(cv * TOK_SIZE * 4);
     if (train) {
         const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
         d.Tt = (__half*)take(cv * 2 * C * C * 2);

@@ -4,8 +4,9 @@
 // to the first,
 //   dU = scale P^T dO + diag(G_C.) K dS_C;   dR = T^T dU;   dV = beta dR
 //   dS_0 = e^gamma_C dS_C + scale (e^gamma Q)^T dO - (beta e^gamma K)^T dR
-// the forward's three products again, run the other way by the same scheme (four
-// warps on 16 columns of dv, dS^T in registers).  All else has no
+// the forward's three products again, run the other way by the same scheme
+// (kmb_delta.cuh).  P^T dO and (e^gamma Q)^T dO carry nothing from chunk to chunk:
+// the side warps compute them ahead.  All else has no
 // recurrence and is a second kernel, one block per chunk and key head:
 //   dP = scale dO U^T (j <= i);   dA = -dR U^T (j < i)
 //   dQ = scale e^gamma dO S_0^T + (dP*G) K
@@ -22,25 +23,42 @@
 namespace kmb {
 namespace {
 
-template <int DKP, typename IO, int NU>
-__global__ void __launch_bounds__(128 * NU, 2 / NU)
-delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
-    constexpr int C = kDeltaC;
-    constexpr bool F32 = sizeof(IO) == 4;
-    constexpr int NPK = F32 ? 2 : 1;
+template <int DKP, typename IO>
+struct BwdSmem {
+    static constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1, KT = DKP / 8;
     using ST = DeltaStage<C, DKP, NPK, 2>;
-    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;
-    constexpr int PK = C * DKP * 2;
     using FS = FragBuf<DKP / 16, 2>;
     using FX = FragBuf<C / 16, 2>;
     using FG = FragBuf<C / 16, NPK>;
-    constexpr int EX = FS::BYTES + 3 * FX::BYTES + FG::BYTES;
+    // of a unit: fragments of dS, dU, of dO and dR with the factors of the state's products; accumulators of the
+    // state's product with dO.  dO's fragments share dU's place (the side warps use it after a chunk's dU is read),
+    // P^T dO, from the side warps for the next chunk, shares that of dR, to them.
+    static constexpr int oX = FS::BYTES, oE = oX + FX::BYTES, oF = oE + FX::BYTES, oR = oF + FX::BYTES, oZ = oR + 4096,
+                         EX = oZ + KT * 512;
+    // tiles are loaded two chunks ahead where three stages fit
+    static constexpr int stages(int nu) { return 3 * ST::BYTES + nu * EX + 128 <= 227 * 1024 ? 3 : 2; }
+    static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * EX; }
+};
+
+template <int DKP, typename IO, int NU>
+__global__ void __launch_bounds__(256 * NU, 1)
+delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
+    using SM = BwdSmem<DKP, IO>;
+    constexpr int C = kDeltaC, NPK = SM::NPK;
+    using ST = typename SM::ST;
+    using FS = typename SM::FS;
+    using FX = typename SM::FX;
+    using FG = typename SM::FG;
+    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;
+    constexpr int PK = C * DKP * 2;
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ __align__(8) uint64_t full[2];
+    constexpr int NS = SM::stages(NU);
+    __shared__ __align__(8) uint64_t full[NS];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 2, w = warp & 3;
-    unsigned char* exS = sm + 2 * ST::BYTES + grp * EX;
-    unsigned char *exG = exS + FS::BYTES, *exX = exG + FG::BYTES, *exE = exX + FX::BYTES, *exF = exE + FX::BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
+    const bool chain = (warp & 4) == 0;
+    unsigned char* exS = sm + NS * ST::BYTES + grp * SM::EX;
+    unsigned char *exX = exS + SM::oX, *exE = exS + SM::oE, *exF = exS + SM::oF, *exR = exS + SM::oR, *exZ = exS + SM::oZ;
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
@@ -49,22 +67,144 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     const int r = lane >> 2, c2 = (lane & 3) * 2;
     const int col[2] = {u * 16 + r, u * 16 + r + 8};
     const bool cok[2] = {col[0] < d.dv, col[1] < d.dv};
-    const int ldv = (int)d.ld_v, ldg = (int)d.ld_do, lddv = (int)d.ld_dv;
     long long start, len;
     seq_range(d, n, start, len);
     const int chunk0 = d.cu ? d.cstart[n] : n * d.nc;
     const int nch = (int)((len + C - 1) / C);
-
-    float S[KTW][4];   // dS^T, the warp's quarter of dk
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
-#pragma unroll
-    for (int t = 0; t < KTW; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int i = (w * KTW + t) * 8 + c2 + (e & 1);
-            S[t][e] = (d.dhT && i < d.dk && cok[e >> 1]) ? d.dhT[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
+
+    const auto stage = [&](int i) { return i % NS; };
+    const auto fetch = [&](int i) {   // the tiles of the recurrence's step i
+        ST::load(d, d.Tt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + nch - 1 - i, hv);
+    };
+    const auto arrived = [&](int i) { return mbar_wait(smem_u32(&full[stage(i)]), (i / NS) & 1); };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < NS - 1 && i < nch; i++) fetch(i);
+    }
+    // The chunk's tiles are there, the state's fragments too, and the last chunk's stage is read; false: a wait ran out.
+    const auto begin = [&](int i) {
+        const bool got = arrived(i);
+        if (!__syncthreads_and(got)) {
+            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            return false;
         }
+        if (threadIdx.x == 0 && i + NS - 1 < nch) fetch(i + NS - 1);
+        return true;
+    };
+
+    if (chain) {
+        float S[KTW][4], up, dn;   // dS^T, the warp's quarter of dk
+#pragma unroll
+        for (int t = 0; t < KTW; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = (w * KTW + t) * 8 + c2 + (e & 1);
+                S[t][e] = (d.dhT && i < d.dk && cok[e >> 1]) ? d.dhT[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
+            }
+        const auto put_state = [&]() {
+            frag_scale(S, up, dn);
+#pragma unroll
+            for (int b = 0; b < KBW; b++) {
+                uint32_t a[2][4];
+                frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
+                FS::put(exS, w * KBW + b, lane, a, dn);
+            }
+        };
+        put_state();
+        __syncthreads();
+        for (int it = 0; it < nch; it++) {
+            if (!begin(it)) return;
+            const uint32_t st = sb + stage(it) * ST::BYTES;
+            const float* tk = (const float*)(sm + stage(it) * ST::BYTES + ST::oTok);
+            const float* tw = tk + w * 16 + c2;
+            // dU = diag(G_C.) K dS_C + scale P^T dO (the latter from the side warps)
+            float X[2][4], Y[2][4], part[2][4];
+            zero(X);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                zero(part);
+#pragma unroll
+                for (int b = 0; b < KBW; b++) {
+                    const int kk = s * KBW + b;
+                    uint32_t a[2][4];
+                    FS::template get<2>(exS, kk, lane, a);
+                    const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                    mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
+                }
+                add_scaled(X, part, FS::scale(exS, s * KBW));
+            }
+            get_acc(exR, w * 2, lane, Y);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + (e & 1);
+                    X[t][e] = fmaf(X[t][e], tw[TOK_GC * C + i] * tw[TOK_FK * C + i], Y[t][e]);
+                    Y[t][e] = 0.0f;
+                }
+            frag_scale(X, up, dn);
+            FX::put(exX, w, lane, X, up, dn);
+            chain_bar(grp);
+            // dR^T = dU^T T: column j of T has rows i >= j only
+#pragma unroll
+            for (int kk = 0; kk < C / 16; kk++) {
+                if (kk < w) continue;
+                uint32_t a[2][4];
+                FX::template get<2>(exX, kk, lane, a);
+                const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
+                zero(part);
+                mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oT + p * ST::TT + o); });
+                add_scaled(Y, part, FX::scale(exX, kk) * tk[TOK_MISC * C + 8 + kk]);
+            }
+            put_acc(exR, w * 2, lane, Y);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + (e & 1);
+                    X[t][e] = Y[t][e] * -(tw[TOK_BETA * C + i] * tw[TOK_EG * C + i] * tw[TOK_FK * C + i]);
+                }
+            frag_scale(X, up, dn);
+            FX::put(exF, w, lane, X, up, dn);
+            unit_bar(grp);
+            // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q (from the side warps) - (beta e^gamma dR)^T K
+            const float last = tk[TOK_EG * C + C - 1];
+            float ps[KTW][4];
+            get_acc(exZ, w * KTW, lane, ps);
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) S[t][e] = fmaf(S[t][e], last, ps[t][e]);
+#pragma unroll
+            for (int kk = 0; kk < C / 16; kk++) {
+                uint32_t a[2][4];
+                FX::template get<2>(exF, kk, lane, a);
+                zero(ps);
+                mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                    ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+                });
+                add_scaled(S, ps, FX::scale(exF, kk));
+            }
+            put_state();
+        }
+        __syncthreads();   // the side warps read the last fragments
+        if (d.dh0) {
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = (w * KTW + t) * 8 + c2 + (e & 1);
+                    if (i < d.dk && cok[e >> 1]) d.dh0[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
+                }
+        }
+        return;
+    }
+
+    // side warps
     using RT = typename RawOf<IO>::type;
+    const int ldv = (int)d.ld_v, ldg = (int)d.ld_do, lddv = (int)d.ld_dv;
     const auto load_t = [&](const void* base, long long ld, int ldi, int c, RT (&V)[2][4]) {
         const long long t0 = (long long)c * C + w * 16;
         const RT* p = (const RT*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
@@ -76,193 +216,145 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                 V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldi + (e >> 1) * 8] : RT(0);
             }
     };
-    float up, dn;
-    // fragments of dS_C and of dO for chunk c, kept too
-    const auto put_state = [&](int c) {
-        frag_scale(S, up, dn);
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        const bool keep = on && c >= 0;
-        if (keep && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_DS] = dn;
-#pragma unroll
-        for (int b = 0; b < KBW; b++) {
-            uint32_t a[2][4];
-            frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
-            FS::put(exS, w * KBW + b, lane, a, dn);
-            if (keep) put_frag<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
-        }
-    };
-    float G[2][4];   // dO^T of the warp's tokens
-    RT Gn[2][4];     // the next chunk's
-    const auto put_go = [&](int c) {
+    const auto unit_at = [&](int c) { return ((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u; };
+    float G[2][4], part[2][4], up, dn;   // dO^T of the warp's tokens
+    RT Gn[2][4];
+    // ahead of chunk c (tile stage `s`): dO's fragments, plain and with the factors of the state's product; P^T dO
+    const auto ahead = [&](int c, int s) {
+        const uint32_t st = sb + s * ST::BYTES;
+        const float* tk = (const float*)(sm + s * ST::BYTES + ST::oTok);
+        const float* tw = tk + w * 16 + c2;
+        uint32_t a[NPK][4];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) G[t][e] = from_raw(Gn[t][e]);
         frag_scale(G, up, dn);
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        uint32_t a[NPK][4];
         frag_pieces<NPK>(G[0], G[1], up, a);
-        FG::put(exG, w, lane, a, dn);
+        FG::put(exX, w, lane, a, dn);
         if (on) {
+            const size_t fb = unit_at(c);
             put_frag<NPK, 64>(d.Gh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
             if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_DO] = dn;
         }
+        float Y[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + (e & 1);
+                Y[t][e] = G[t][e] * (d.scale * tw[TOK_EG * C + i] * tw[TOK_FQ * C + i]);
+            }
+        frag_scale(Y, up, dn);
+        FX::put(exE, w, lane, Y, up, dn);
+        side_bar(grp);
+        zero(Y);
+#pragma unroll
+        for (int kk = 0; kk < C / 16; kk++) {   // column j of P has rows i >= j only
+            if (kk < w) continue;
+            uint32_t a1[NPK][4];
+            FG::template get<NPK>(exX, kk, lane, a1);
+            const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
+            zero(part);
+            mma_row<NPK, 2>(part, a1, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
+            add_scaled(Y, part, FG::scale(exX, kk) * (tk[TOK_MISC * C + 4 + kk] * d.scale));
+        }
+        put_acc(exR, w * 2, lane, Y);
     };
-    if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&full[0]), 1);
-        mbar_init(smem_u32(&full[1]), 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (nch > 0) ST::load(d, d.Tt, sb, smem_u32(&full[0]), chunk0 + nch - 1, hv);
-    }
-    put_state(nch - 1);
-    if (nch > 0) {
-        load_t(d.go, d.ld_do, ldg, nch - 1, Gn);
-        put_go(nch - 1);
-    }
+    uint32_t sr[KBW][2][2][2];   // the warp's part of the state at the start of the last chunk done
+    float fs = 0.0f;
+    // <S_0, dS_0> at the start of chunk c, from the fragments that the chain left
+    const auto anchor = [&](int c) {
+        float an = 0.0f;
+#pragma unroll
+        for (int b = 0; b < KBW; b++) {
+            uint32_t a[2][4];
+            FS::template get<2>(exS, w * KBW + b, lane, a);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {   // fragment word i: row half i & 1, tile i >> 1
+                const float2 x = join(a[0][i], a[1][i]), y = join(sr[b][i >> 1][i & 1][0], sr[b][i >> 1][i & 1][1]);
+                an = fmaf(x.x, y.x, an);
+                an = fmaf(x.y, y.y, an);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
+        // magnitudes are up to 2^30 and more per product: the scales are applied one after the other
+        if (on && lane == 0) d.anchor[unit_at(c) * 4 + w] = an * fs * FS::scale(exS, w * KBW);
+    };
+    if (nch > 0) load_t(d.go, d.ld_do, ldg, nch - 1, Gn);
     __syncthreads();
+    if (nch > 0) {
+        if (!arrived(0)) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+        ahead(nch - 1, 0);
+    }
     for (int it = 0; it < nch; it++) {
         const int c = nch - 1 - it;
-        const bool got = mbar_wait(smem_u32(&full[it & 1]), (it >> 1) & 1);
-        if (!__syncthreads_and(got)) {
-            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
-            return;
-        }
-        if (threadIdx.x == 0 && c > 0)
-            ST::load(d, d.Tt, sb + ((it + 1) & 1) * ST::BYTES, smem_u32(&full[(it + 1) & 1]), chunk0 + c - 1, hv);
-        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);
-        const uint32_t st = sb + (it & 1) * ST::BYTES;
-        const float* tk = (const float*)(sm + (it & 1) * ST::BYTES + ST::oTok);
+        if (!begin(it)) return;
+        const uint32_t st = sb + stage(it) * ST::BYTES;
+        const float* tk = (const float*)(sm + stage(it) * ST::BYTES + ST::oTok);
         const float* tw = tk + w * 16 + c2;
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        // what the end of the chunk reads: in flight under the products
+        const size_t fb = unit_at(c);
+        float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
+        // what the chunk's sums need, and the next chunk's dO: in flight under the products
         RT V[2][4];
         uint32_t wr[2][2][2];
         float4 o4[2];
+        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);
         load_t(d.v, d.ld_v, ldv, c, V);
+        float fw = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const size_t at = (fb * (C / 8) + w * 2 + t) * 32 + lane;
-            o4[t] = on ? ((const float4*)d.Of)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (on) get_tile<64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, wr[t]);
-            else wr[t][0][0] = wr[t][0][1] = wr[t][1][0] = wr[t][1][1] = 0;
+            o4[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            wr[t][0][0] = wr[t][0][1] = wr[t][1][0] = wr[t][1][1] = 0;
+            if (on) {
+                o4[t] = ((const float4*)d.Of)[(fb * (C / 8) + w * 2 + t) * 32 + lane];
+                get_tile<64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, wr[t]);
+            }
         }
-        float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
-        const float fw = on ? mx[MX_W] : 0.0f, fs = on ? mx[MX_S] : 0.0f;
-        uint32_t sr[KTW][2][2];   // S_0
-        if (on) {
+        if (on) fw = mx[MX_W];
+        // keep dS_C; its product with the state at the same place
+        if (it > 0) anchor(c + 1);
 #pragma unroll
-            for (int t = 0; t < KTW; t++)
-                get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KTW + t) * 8, sr[t]);
+        for (int b = 0; b < KBW; b++) {
+            uint32_t a[2][4];
+            FS::template get<2>(exS, w * KBW + b, lane, a);
+            if (on) {
+                put_frag<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
+                if (lane == 0) mx[MX_DS] = FS::scale(exS, w * KBW);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, ((w * KBW + b) * 2 + t) * 8, sr[b][t]);
+                fs = mx[MX_S];
+            }
         }
-        // K dS_C
-        float X[2][4], Y[2][4], part[2][4];
-        zero(X);
-        zero(Y);
+        // (scale e^gamma dO)^T Q
+        {
+            float Z[KTW][4], ps[KTW][4];
+            zero(Z);
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            zero(part);
-#pragma unroll
-            for (int b = 0; b < KBW; b++) {
-                const int kk = s * KBW + b;
+            for (int kk = 0; kk < C / 16; kk++) {
                 uint32_t a[2][4];
-                FS::template get<2>(exS, kk, lane, a);
-                const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-                mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
+                FX::template get<2>(exE, kk, lane, a);
+                zero(ps);
+                mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                    ldm4t(f, st + ST::oQ + p * PK +
+                                 wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+                });
+                add_scaled(Z, ps, FX::scale(exE, kk));
             }
-            dn = FS::scale(exS, s * KBW);
-            add_scaled(X, part, dn);
+            put_acc(exZ, w * KTW, lane, Z);
         }
-        // P^T dO: column j of P has rows i >= j only
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            if (kk < w) continue;
-            uint32_t a[NPK][4];
-            FG::template get<NPK>(exG, kk, lane, a);
-            dn = FG::scale(exG, kk) * tk[TOK_MISC * C + 4 + kk];
-            const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
-            zero(part);
-            mma_row<NPK, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
-            add_scaled(Y, part, dn);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + (e & 1);
-                X[t][e] = fmaf(Y[t][e], d.scale, X[t][e] * (tw[TOK_GC * C + i] * tw[TOK_FK * C + i]));
-                Y[t][e] = 0.0f;
-            }
-        frag_scale(X, up, dn);
-        FX::put(exX, w, lane, X, up, dn);
-        // dO with the factors of the state's product
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + (e & 1);
-                X[t][e] = G[t][e] * (d.scale * tw[TOK_EG * C + i] * tw[TOK_FQ * C + i]);
-            }
-        frag_scale(X, up, dn);
-        FX::put(exE, w, lane, X, up, dn);
         unit_bar(grp);
-        // dR^T = dU^T T
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            if (kk < w) continue;
-            uint32_t a[2][4];
-            FX::template get<2>(exX, kk, lane, a);
-            dn = FX::scale(exX, kk) * tk[TOK_MISC * C + 8 + kk];
-            const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
-            zero(part);
-            mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oT + p * ST::TT + o); });
-            add_scaled(Y, part, dn);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + (e & 1);
-                X[t][e] = Y[t][e] * -(tw[TOK_BETA * C + i] * tw[TOK_EG * C + i] * tw[TOK_FK * C + i]);
-            }
-        frag_scale(X, up, dn);
-        FX::put(exF, w, lane, X, up, dn);
-        unit_bar(grp);
-        // dS^T <- e^gamma_C dS^T + (scale e^gamma dO)^T Q - (beta e^gamma dR)^T K
-        const float last = tk[TOK_EG * C + C - 1];
-#pragma unroll
-        for (int t = 0; t < KTW; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[t][e] *= last;
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            uint32_t a[2][4];
-            float ps[KTW][4];
-            FX::template get<2>(exE, kk, lane, a);
-            dn = FX::scale(exE, kk);
-            zero(ps);
-            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
-                ldm4t(f, st + ST::oQ + p * PK +
-                             wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
-            });
-            add_scaled(S, ps, dn);
-            FX::template get<2>(exF, kk, lane, a);
-            dn = FX::scale(exF, kk);
-            zero(ps);
-            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
-                ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
-            });
-            add_scaled(S, ps, dn);
-        }
-        put_state(c - 1);
         // dV, and what the gates' gradients sum over dv
-        frag_scale(Y, up, dn);
+        float Y[2][4];
+        get_acc(exR, w * 2, lane, Y);
         if (on) {
             uint32_t a[NPK][4];
+            frag_scale(Y, up, dn);
             frag_pieces<NPK>(Y[0], Y[1], up, a);
             put_frag<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
             if (lane == 0) mx[MX_R] = dn;
-        }
-        {
             const long long t0 = (long long)c * C + w * 16;
             IO* pd = (IO*)d.dvv + (start + t0) * d.ld_dv + (long long)hv * d.dv + col[0];
             float ts[2][2], bs[2][2];
@@ -287,40 +379,20 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
                         ts[t][h] += __shfl_xor_sync(0xffffffffu, ts[t][h], o);
                         bs[t][h] += __shfl_xor_sync(0xffffffffu, bs[t][h], o);
                     }
-                if (on && r == t) {
+                if (r == t) {
                     float* pp = d.part + fb * 2 * C + w * 16 + t * 8 + c2;
                     *(float2*)pp = make_float2(ts[t][0], ts[t][1]);
                     *(float2*)(pp + C) = make_float2(bs[t][0] * fw, bs[t][1] * fw);
                 }
             }
         }
-        // <S_0, dS_0> over the warp's entries
-        if (on) {
-            float an = 0.0f;
-#pragma unroll
-            for (int t = 0; t < KTW; t++) {
-                const float2 x = join(sr[t][0][0], sr[t][0][1]), y = join(sr[t][1][0], sr[t][1][1]);
-                an = fmaf(S[t][0], x.x, an);
-                an = fmaf(S[t][1], x.y, an);
-                an = fmaf(S[t][2], y.x, an);
-                an = fmaf(S[t][3], y.y, an);
-            }
-            an *= fs;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
-            if (lane == 0) d.anchor[fb * 4 + w] = an;
+        if (c > 0) {
+            if (!arrived(it + 1)) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            ahead(c - 1, stage(it + 1));
         }
-        if (c > 0) put_go(c - 1);
     }
-    if (d.dh0) {
-#pragma unroll
-        for (int t = 0; t < KTW; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = (w * KTW + t) * 8 + c2 + (e & 1);
-                if (i < d.dk && cok[e >> 1]) d.dh0[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
-            }
-    }
+    __syncthreads();
+    if (nch > 0) anchor(0);
 }
 
 // ------------------------------------------------------------------ gradients without recurrence
@@ -337,7 +409,7 @@ struct GradSmem {
     // the four weighted matrices take the place of the slices
     static constexpr int oE = oG, TE = C * C * 2;
     static constexpr int oTok = (oE + 4 * NP * TE > oEnd ? oE + 4 * NP * TE : oEnd);
-    static constexpr int oMx = oTok + TOK_ROWS * C * 4;
+    static constexpr int oMx = oTok + TOK_SIZE * 4;
     static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
     static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
     static constexpr int BYTES = oCol + 3 * 48 * 4;
@@ -443,7 +515,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             cp_commit();
         };
         __syncthreads();
-        for (int i = tid; i < TOK_ROWS * C / 4; i += 256) cp16(sb + SM::oTok + i * 16, d.tok + head * TOK_ROWS * C + i * 4);
+        for (int i = tid; i < TOK_SIZE / 4; i += 256) cp16(sb + SM::oTok + i * 16, d.tok + head * TOK_SIZE + i * 4);
         for (int i = tid; i < d.units * MX_ROWS; i += 256) cp16(sb + SM::oMx + i * 16, d.mx + head * d.units * 4 * MX_ROWS + i * 4);
         for (int i = tid; i < C / 2; i += 256) cp16(sb + SM::oGam + i * 16, d.gam + head * C + i * 2);
         slice(0);
@@ -640,15 +712,13 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
 
 template <int DKP, typename IO, int NU>
 cudaError_t chain_go(const DeltaDesc& d, cudaStream_t st) {
-    constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
-    using ST = DeltaStage<C, DKP, NPK, 2>;
-    constexpr int EX = FragBuf<DKP / 16, 2>::BYTES + 3 * FragBuf<C / 16, 2>::BYTES + FragBuf<C / 16, NPK>::BYTES;
-    constexpr int SMEM = 2 * ST::BYTES + NU * EX;
+    constexpr int SMEM = BwdSmem<DKP, IO>::bytes(NU);
+    static_assert(BwdSmem<DKP, IO>::bytes(1) + 64 <= 227 * 1024, "shared memory of a block");
     auto kern = delta_chain_bwd_kernel<DKP, IO, NU>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
-    kern<<<(unsigned)blocks, 128 * NU, SMEM, st>>>(d);
+    kern<<<(unsigned)blocks, 256 * NU, SMEM, st>>>(d);
     return cudaGetLastError();
 }
 template <int DKP, typename IO>

@@ -8,26 +8,41 @@
 namespace kmb {
 namespace {
 
-template <int DKP, typename IO, bool KEEP, int NU>
-__global__ void __launch_bounds__(128 * NU, 2 / NU)
-delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
-    constexpr int C = kDeltaC;
-    constexpr bool F32 = sizeof(IO) == 4;
-    constexpr int NPK = F32 ? 2 : 1;
-    constexpr int NPO = (F32 || KEEP) ? 2 : 1;   // pieces behind o: it is rounded to bf16 unless it is kept in fp32
+template <int DKP, typename IO, bool KEEP>
+struct FwdSmem {
+    static constexpr int C = kDeltaC;
+    static constexpr int NPK = sizeof(IO) == 4 ? 2 : 1;
+    static constexpr int NPO = (sizeof(IO) == 4 || KEEP) ? 2 : 1;   // pieces behind o: it is rounded to bf16 unless it is kept in fp32
     using ST = DeltaStage<C, DKP, NPK, NPO>;
-    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;   // dk tiles, of a warp; its blocks of 16
-    constexpr int PK = C * DKP * 2;              // bytes of a K or Q piece
     using FS = FragBuf<DKP / 16, 2>;
     using FX = FragBuf<C / 16, 2>;
     using FO = FragBuf<C / 16, NPO>;
-    constexpr int EX = FS::BYTES + 2 * FX::BYTES + FO::BYTES;   // exchange buffers of a unit
+    // of a unit: fragments of S, X, G_C. U and U, W as accumulators
+    static constexpr int oX = FS::BYTES, oU = oX + FX::BYTES, oO = oU + FX::BYTES, oW = oO + FO::BYTES, EX = oW + 4096;
+    // tiles are loaded two chunks ahead where three stages fit
+    static constexpr int stages(int nu) { return 3 * ST::BYTES + nu * EX + 128 <= 227 * 1024 ? 3 : 2; }
+    static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * EX; }
+};
+
+template <int DKP, typename IO, bool KEEP, int NU>
+__global__ void __launch_bounds__(256 * NU, 1)
+delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
+    using SM = FwdSmem<DKP, IO, KEEP>;
+    constexpr int C = kDeltaC, NPK = SM::NPK, NPO = SM::NPO;
+    using ST = typename SM::ST;
+    using FS = typename SM::FS;
+    using FX = typename SM::FX;
+    using FO = typename SM::FO;
+    constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;   // dk tiles, of a warp; its blocks of 16
+    constexpr int PK = C * DKP * 2;              // bytes of a K or Q piece
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ __align__(8) uint64_t full[2];
+    constexpr int NS = SM::stages(NU);
+    __shared__ __align__(8) uint64_t full[NS];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 2, w = warp & 3;
-    unsigned char* exS = sm + 2 * ST::BYTES + grp * EX;
-    unsigned char *exX = exS + FS::BYTES, *exU = exX + FX::BYTES, *exO = exU + FX::BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
+    const bool chain = (warp & 4) == 0;
+    unsigned char* exS = sm + NS * ST::BYTES + grp * SM::EX;
+    unsigned char *exX = exS + SM::oX, *exU = exS + SM::oU, *exO = exS + SM::oO, *exW = exS + SM::oW;
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
@@ -41,216 +56,240 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     seq_range(d, n, start, len);
     const int chunk0 = d.cu ? d.cstart[n] : n * d.nc;
     const int nch = (int)((len + C - 1) / C);
-
-    float S[KTW][4];
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
-#pragma unroll
-    for (int t = 0; t < KTW; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int i = (w * KTW + t) * 8 + c2 + (e & 1);
-            S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
-        }
-    // v of the warp's tokens of chunk c as accumulator tiles [16 columns][16 tokens]
-    using RT = typename RawOf<IO>::type;
-    const auto load_v = [&](int c, RT (&V)[2][4]) {
-        const long long t0 = (long long)c * C + w * 16;
-        const RT* p = (const RT*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + c2 + (e & 1);
-                V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
-            }
+
+    const auto stage = [&](int i) { return i % NS; };
+    const auto fetch = [&](int i) {   // the tiles of the recurrence's step i
+        ST::load(d, d.Mt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + i, hv);
     };
-    // the state's fragments for chunk c, kept too
-    const auto put_state = [&](int c) {
-        float up, dn;
-        frag_scale(S, up, dn);
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        const bool keep = KEEP && on && c < nch;
-        if (keep && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = dn;
-#pragma unroll
-        for (int b = 0; b < KBW; b++) {
-            uint32_t a[2][4];
-            frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
-            FS::put(exS, w * KBW + b, lane, a, dn);
-            if (keep) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
-        }
-    };
+    const auto arrived = [&](int i) { return mbar_wait(smem_u32(&full[stage(i)]), (i / NS) & 1); };
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&full[0]), 1);
-        mbar_init(smem_u32(&full[1]), 1);
+        for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (nch > 0) ST::load(d, d.Mt, sb, smem_u32(&full[0]), chunk0, hv);
+        for (int i = 0; i < NS - 1 && i < nch; i++) fetch(i);
     }
-    put_state(0);
-    __syncthreads();
-    RT Vn[2][4];
-    if (nch > 0) load_v(0, Vn);
-    for (int c = 0; c < nch; c++) {
-        const bool got = mbar_wait(smem_u32(&full[c & 1]), (c >> 1) & 1);
-        // the state's fragments and this chunk's tiles are there; the other stage is read
+    // The chunk's tiles are there, the state's fragments too, and the last chunk's stage is read; false: a wait ran out.
+    const auto begin = [&](int i) {
+        const bool got = arrived(i);
         if (!__syncthreads_and(got)) {
             if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
-            return;
+            return false;
         }
-        if (threadIdx.x == 0 && c + 1 < nch)
-            ST::load(d, d.Mt, sb + ((c + 1) & 1) * ST::BYTES, smem_u32(&full[(c + 1) & 1]), chunk0 + c + 1, hv);
-        RT V[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) V[t][e] = Vn[t][e];
-        if (c + 1 < nch) load_v(c + 1, Vn);
-        const uint32_t st = sb + (c & 1) * ST::BYTES;
-        const float* tk = (const float*)(sm + (c & 1) * ST::BYTES + ST::oTok);
-        const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
-        const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-        float X[2][4], O[2][4], part[2][4], dn, up;
-        zero(X);
-        zero(O);
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            float po[2][4];
-            zero(part);
-            zero(po);
-#pragma unroll
-            for (int b = 0; b < KBW; b++) {
-                const int kk = s * KBW + b;
-                uint32_t a[2][4];
-                FS::template get<2>(exS, kk, lane, a);
-                const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-                mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
-                mma_row<NPO, NPK>(po, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
-                                  [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oQ + p * PK + o); });
-            }
-            dn = FS::scale(exS, s * KBW);
-            add_scaled(X, part, dn);
-            add_scaled(O, po, dn);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + (e & 1);
-                const float eg = tw[TOK_EG * C + i];
-                X[t][e] = from_raw(V[t][e]) - eg * tw[TOK_FK * C + i] * X[t][e];
-                O[t][e] *= eg * tw[TOK_FQ * C + i];
-            }
-        frag_scale(X, up, dn);
-        FX::put(exX, w, lane, X, up, dn);
-        unit_bar(grp);
-        // W^T = X M^T: row i of M reaches columns j <= i only
-        float W[2][4];
-        zero(W);
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            if (kk > w) continue;
-            uint32_t a[2][4];
-            FX::template get<2>(exX, kk, lane, a);
-            dn = FX::scale(exX, kk);
-            const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-            zero(part);
-            mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
-            add_scaled(W, part, dn);
-        }
-        const float fm = tk[TOK_MISC * C + w], fp = tk[TOK_MISC * C + 4 + w];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) W[t][e] *= fm;
-        if (KEEP && on) {
-            uint32_t a[2][4];
-            frag_scale(W, up, dn);
-            frag_pieces<2>(W[0], W[1], up, a);
-            put_frag<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
-            if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = dn;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
-        frag_scale(W, up, dn);
-        FO::put(exO, w, lane, W, up, dn);
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + (e & 1);
-                W[t][e] *= tw[TOK_GC * C + i] * tw[TOK_FK * C + i];
-            }
-        frag_scale(W, up, dn);
-        FX::put(exU, w, lane, W, up, dn);
-        unit_bar(grp);
-        // S^T <- e^gamma_C S^T + (G_C. U)^T K
-        const float last = tk[TOK_EG * C + C - 1];
-#pragma unroll
-        for (int t = 0; t < KTW; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[t][e] *= last;
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            uint32_t a[2][4];
-            float ps[KTW][4];
-            FX::template get<2>(exU, kk, lane, a);
-            dn = FX::scale(exU, kk);
-            zero(ps);
-            mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
-                ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
-            });
-            add_scaled(S, ps, dn);
-        }
-        put_state(c + 1);
-        // O^T += U^T P^T
-#pragma unroll
-        for (int kk = 0; kk < C / 16; kk++) {
-            if (kk > w) continue;
-            uint32_t a[NPO][4];
-            FO::template get<NPO>(exO, kk, lane, a);
-            dn = FO::scale(exO, kk) * fp;
-            const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-            zero(part);
-            mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });
-            add_scaled(O, part, dn);
-        }
-        const long long t0 = (long long)c * C + w * 16;
-        IO* po = (IO*)d.o + (start + t0) * d.ld_o + (long long)hv * d.dv + col[0];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + c2 + (e & 1);
-                O[t][e] *= d.scale;
-                if (t0 + i < len && cok[e >> 1]) stt(po + (long long)i * ldo, (e >> 1) * 8, O[t][e]);
-            }
-            if (KEEP && on)
-                *((float4*)d.Of + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(O[t][0], O[t][1], O[t][2], O[t][3]);
-        }
-    }
-    if (d.hT) {
+        if (threadIdx.x == 0 && i + NS - 1 < nch) fetch(i + NS - 1);
+        return true;
+    };
+
+    if (chain) {
+        float S[KTW][4];
 #pragma unroll
         for (int t = 0; t < KTW; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = (w * KTW + t) * 8 + c2 + (e & 1);
-                if (i < d.dk && cok[e >> 1]) d.hT[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
+                S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
             }
+        // v of the warp's tokens of chunk c, as accumulator tiles [16 columns][16 tokens]
+        using RT = typename RawOf<IO>::type;
+        const auto load_v = [&](int c, RT (&V)[2][4]) {
+            const long long t0 = (long long)c * C + w * 16;
+            const RT* p = (const RT*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + c2 + (e & 1);
+                    V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
+                }
+        };
+        const auto put_state = [&]() {
+            float up, dn;
+            frag_scale(S, up, dn);
+#pragma unroll
+            for (int b = 0; b < KBW; b++) {
+                uint32_t a[2][4];
+                frag_pieces<2>(S[2 * b], S[2 * b + 1], up, a);
+                FS::put(exS, w * KBW + b, lane, a, dn);
+            }
+        };
+        put_state();
+        __syncthreads();
+        RT V[2][4], Vn[2][4];
+        if (nch > 0) load_v(0, Vn);
+        for (int c = 0; c < nch; c++) {
+            if (!begin(c)) return;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) V[t][e] = Vn[t][e];
+            if (c + 1 < nch) load_v(c + 1, Vn);
+            const uint32_t st = sb + stage(c) * ST::BYTES;
+            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
+            const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
+            float X[2][4], part[2][4], dn, up;
+            zero(X);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                zero(part);
+#pragma unroll
+                for (int b = 0; b < KBW; b++) {
+                    const int kk = s * KBW + b;
+                    uint32_t a[2][4];
+                    FS::template get<2>(exS, kk, lane, a);
+                    const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                    mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
+                }
+                add_scaled(X, part, FS::scale(exS, s * KBW));
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + (e & 1);
+                    X[t][e] = from_raw(V[t][e]) - tw[TOK_EG * C + i] * tw[TOK_FK * C + i] * X[t][e];
+                }
+            frag_scale(X, up, dn);
+            FX::put(exX, w, lane, X, up, dn);
+            chain_bar(grp);
+            // W^T = X M^T: row i of M reaches columns j <= i only
+            float W[2][4];
+            zero(W);
+            const float fm = tk[TOK_MISC * C + w];
+#pragma unroll
+            for (int kk = 0; kk < C / 16; kk++) {
+                if (kk > w) continue;
+                uint32_t a[2][4];
+                FX::template get<2>(exX, kk, lane, a);
+                const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                zero(part);
+                mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
+                add_scaled(W, part, FX::scale(exX, kk) * fm);
+            }
+            put_acc(exW, w * 2, lane, W);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + (e & 1);
+                    W[t][e] *= tw[TOK_BETA * C + i] * (tw[TOK_GC * C + i] * tw[TOK_FK * C + i]);
+                }
+            frag_scale(W, up, dn);
+            FX::put(exU, w, lane, W, up, dn);
+            unit_bar(grp);
+            // S^T <- e^gamma_C S^T + (G_C. U)^T K
+            const float last = tk[TOK_EG * C + C - 1];
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) S[t][e] *= last;
+#pragma unroll
+            for (int kk = 0; kk < C / 16; kk++) {
+                uint32_t a[2][4];
+                float ps[KTW][4];
+                FX::template get<2>(exU, kk, lane, a);
+                zero(ps);
+                mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
+                    ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+                });
+                add_scaled(S, ps, FX::scale(exU, kk));
+            }
+            put_state();
+        }
+        if (d.hT) {
+#pragma unroll
+            for (int t = 0; t < KTW; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = (w * KTW + t) * 8 + c2 + (e & 1);
+                    if (i < d.dk && cok[e >> 1]) d.hT[sbase + (size_t)i * d.dv + col[e >> 1]] = S[t][e];
+                }
+        }
+    } else {
+        // side warps: O^T = e^gamma S^T Q^T + U^T P^T, and what the backward reads
+        __syncthreads();
+        for (int c = 0; c < nch; c++) {
+            if (!begin(c)) return;
+            const uint32_t st = sb + stage(c) * ST::BYTES;
+            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
+            const float* tw = tk + w * 16 + c2;
+            const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+            float O[2][4], W[2][4], part[2][4], dn, up;
+            zero(O);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float f = FS::scale(exS, s * KBW);
+                zero(part);
+#pragma unroll
+                for (int b = 0; b < KBW; b++) {
+                    const int kk = s * KBW + b;
+                    uint32_t a[2][4];
+                    FS::template get<2>(exS, kk, lane, a);
+                    if (KEEP && on && s == w) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, kk * 16, a);
+                    const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                    mma_row<NPO, NPK>(part, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
+                                      [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });
+                }
+                add_scaled(O, part, f);
+                if (KEEP && on && s == w && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = f;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + (e & 1);
+                    O[t][e] *= tw[TOK_EG * C + i] * tw[TOK_FQ * C + i];
+                }
+            unit_bar(grp);
+            get_acc(exW, w * 2, lane, W);
+            if (KEEP && on) {
+                uint32_t a[2][4];
+                frag_scale(W, up, dn);
+                frag_pieces<2>(W[0], W[1], up, a);
+                put_frag<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
+                if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = dn;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
+            frag_scale(W, up, dn);
+            FO::put(exO, w, lane, W, up, dn);
+            side_bar(grp);
+            const float fp = tk[TOK_MISC * C + 4 + w];
+#pragma unroll
+            for (int kk = 0; kk < C / 16; kk++) {
+                if (kk > w) continue;
+                uint32_t a[NPO][4];
+                FO::template get<NPO>(exO, kk, lane, a);
+                const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
+                zero(part);
+                mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });
+                add_scaled(O, part, FO::scale(exO, kk) * fp);
+            }
+            const long long t0 = (long long)c * C + w * 16;
+            IO* po = (IO*)d.o + (start + t0) * d.ld_o + (long long)hv * d.dv + col[0];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + c2 + (e & 1);
+                    O[t][e] *= d.scale;
+                    if (t0 + i < len && cok[e >> 1]) stt(po + (long long)i * ldo, (e >> 1) * 8, O[t][e]);
+                }
+                if (KEEP && on)
+                    *((float4*)d.Of + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(O[t][0], O[t][1], O[t][2], O[t][3]);
+            }
+        }
     }
 }
 
 template <int DKP, typename IO, bool KEEP, int NU>
 cudaError_t go(const DeltaDesc& d, cudaStream_t st) {
-    constexpr int C = kDeltaC, NPO = (sizeof(IO) == 4 || KEEP) ? 2 : 1;
-    using ST = DeltaStage<C, DKP, sizeof(IO) == 4 ? 2 : 1, NPO>;
-    constexpr int EX = FragBuf<DKP / 16, 2>::BYTES + 2 * FragBuf<C / 16, 2>::BYTES + FragBuf<C / 16, NPO>::BYTES;
-    constexpr int SMEM = 2 * ST::BYTES + NU * EX;
+    constexpr int SMEM = FwdSmem<DKP, IO, KEEP>::bytes(NU);
     auto kern = delta_chain_fwd_kernel<DKP, IO, KEEP, NU>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
-    kern<<<(unsigned)blocks, 128 * NU, SMEM, st>>>(d);
+    kern<<<(unsigned)blocks, 256 * NU, SMEM, st>>>(d);
     return cudaGetLastError();
 }
 template <int DKP, typename IO>

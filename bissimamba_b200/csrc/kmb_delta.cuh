@@ -38,7 +38,7 @@ enum {
     TOK_FK = 3,    // k_i = FK_i * row i of the K tile
     TOK_FQ = 4,
     TOK_MISC = 5,  // [b], [4 + b], [8 + b]: rows 16 b .. 16 b + 15 of M, P, T = that factor times their tiles
-    TOK_ROWS = 6
+    TOK_SIZE = 5 * 64 + 16   // floats
 };
 enum { MX_S = 0, MX_W = 1, MX_DO = 2, MX_R = 3, MX_DS = 4, MX_ROWS = 8 };
 constexpr int kDeltaC = 64;      // tokens per chunk
@@ -60,7 +60,7 @@ struct DeltaDesc {
     // workspace
     __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
     __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], on and below the diagonal blocks; Tt for training only
-    float* tok;                  // [nch][Hv][TOK_ROWS][C], see TOK_*
+    float* tok;                  // [nch][Hv][TOK_SIZE], see TOK_*
     double* gam;                 // [nch][Hv][C]: running sums of g (training)
     const int* order;            // packed: sequences, the longest first (NULL: as they are)
     // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
@@ -286,18 +286,20 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // ------------------------------------------------------------------ chunk recurrences
-// A unit is 16 columns of dv of one head; four warps work on it, one per SM sub-partition.  Transposed, the state
-// S^T [16][dk] is an m16 product's accumulator: warp w keeps the quarter w of dk in registers, and owns the tokens
+// A unit is 16 columns of dv of one head.  Transposed, the state S^T [16][dk] is an m16 product's accumulator: of the
+// four warps that carry the recurrence, warp w keeps quarter w of dk in registers, and owns the tokens
 // 16 w .. 16 w + 15 of a chunk.  What all four need (the state, then the chunk's right-hand side, then U) goes
 // through shared memory as fp16 A fragments, each warp's with a power of two of its own, so no warp waits for
-// another's largest entry: the products of a block of k are summed apart and added in fp32.
-// Three barriers a chunk.  A block holds NU units that share the staged tiles.
+// another's largest entry: the products of a block of k are summed apart and added in fp32.  Three barriers a
+// chunk.  The chain of a chunk is bound by latency and by the warps' instructions, so four more warps of the unit do
+// what does not carry it: the outputs, what is kept, what can be computed ahead.  A block holds NU units that
+// share the staged tiles.
 template <int C, int DKP, int NPK, int NPP>
 struct DeltaStage {
     static constexpr int KQ = NPK * C * DKP * 2;   // bytes of K (and of Q)
     static constexpr int TT = C * C * 2;           // one piece of M, T or P
     static constexpr int oQ = KQ, oT = 2 * KQ, oP = oT + 2 * TT, oTok = oP + NPP * TT;
-    static constexpr int TOK = TOK_ROWS * C * 4;
+    static constexpr int TOK = TOK_SIZE * 4;
     static constexpr int BYTES = oTok + TOK;
 
     // one thread: bulk copies of one chunk into the stage at `dst`, M or T from `tiles`
@@ -310,7 +312,7 @@ struct DeltaStage {
         bulk(dst + oQ, d.Qt + kh, KQ, bar);
         bulk(dst + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
         bulk(dst + oP, d.Pt + vh * 2 * C * C, NPP * TT, bar);
-        bulk(dst + oTok, d.tok + vh * TOK_ROWS * C, TOK, bar);
+        bulk(dst + oTok, d.tok + vh * TOK_SIZE, TOK, bar);
     }
     static __device__ __forceinline__ void bulk(uint32_t dst, const void* src, unsigned bytes, uint32_t bar) {
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -391,7 +393,25 @@ __device__ __forceinline__ void add_scaled(float (&acc)[N][4], const float (&par
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[i][e] = fmaf(part[i][e], f, acc[i][e]);
 }
-__device__ __forceinline__ void unit_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
+// barriers of unit g: its chain warps, its side warps, all of them
+__device__ __forceinline__ void chain_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 1) : "memory"); }
+__device__ __forceinline__ void side_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 2) : "memory"); }
+__device__ __forceinline__ void unit_bar(int g) { asm volatile("bar.sync %0, 256;" ::"r"(3 * g + 3) : "memory"); }
+// accumulator tiles through shared memory, [tile][lane] 16 bytes
+template <int N>
+__device__ __forceinline__ void put_acc(unsigned char* base, int tile, int lane, const float (&t)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        *(float4*)(base + (tile + i) * 512 + lane * 16) = make_float4(t[i][0], t[i][1], t[i][2], t[i][3]);
+}
+template <int N>
+__device__ __forceinline__ void get_acc(const unsigned char* base, int tile, int lane, float (&t)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float4 v = *(const float4*)(base + (tile + i) * 512 + lane * 16);
+        t[i][0] = v.x; t[i][1] = v.y; t[i][2] = v.z; t[i][3] = v.w;
+    }
+}
 
 int delta_sms();
 // Units per block: one where every SM gets a unit at most (the chain of a chunk is bound by latency), two where
