@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstring>
 #include "kmb_delta.cuh"
+#include "kmb_launch.cuh"
 #include "../../include/kmamba_delta.h"
 
 namespace kmb {
@@ -14,12 +15,16 @@ int* device_status();
 namespace {
 
 // ------------------------------------------------------------------ packed sequences
+#ifndef KMB_PREP_BLOCKS
+#define KMB_PREP_BLOCKS 4
+#endif
 constexpr int kSortSeqs = 512;   // beyond that many sequences no single one matters
 // One block: offsets clamped to [0, total] and made non-decreasing (cu), and the first chunk of each sequence
 // (cstart).  Whatever the caller's offsets hold, the kernels stay inside the tensors.
 __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ in, int nseq, int total, int C,
                                                        int* __restrict__ cu, int* __restrict__ cstart,
                                                        int* __restrict__ order) {
+    pdl_release();
     __shared__ int sh[256], len[kSortSeqs];
     const int t = threadIdx.x;
     const int per = (nseq + 1 + 255) / 256;
@@ -69,9 +74,9 @@ __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ i
 }
 
 // ------------------------------------------------------------------ per-chunk matrices
-// Block = (chunk, key head), four warps of 16 rows: the chunk's K and Q as swizzled fp16 tiles (zero behind the
-// last token and behind dk), K K^T and Q K^T once per key head; then for each of its value heads the token
-// factors, P, and the chunk's triangular system.  With a_ij = G_ij k_i.k_j (j < i) and
+// First K and Q as swizzled fp16 tiles (zero behind the last token and behind dk), each row with a power of two, per
+// chunk and key head.  Then, per chunk and value head, four warps of 16 rows: K K^T and Q K^T, the token factors, P,
+// and the chunk's triangular system.  With a_ij = G_ij k_i.k_j (j < i) and
 //   C = (I + a diag(beta))^-1 a:   M = I - C diag(beta),   T = I - diag(beta) C
 // (no division: both are exact where beta is 0).  By blocks of 16, diagonal blocks by forward substitution, one
 // column per lane, then row block after row block
@@ -80,40 +85,20 @@ __global__ void __launch_bounds__(256) delta_cu_kernel(const int* __restrict__ i
 // from shared memory.
 
 template <int DKP, typename IO>
-__global__ void __launch_bounds__(128, 3)
-delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
+__global__ void __launch_bounds__(128)
+delta_tiles_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     constexpr int C = kDeltaC;
     constexpr bool F32 = sizeof(IO) == 4;
     constexpr int NPK = F32 ? 2 : 1;
     constexpr int TILE = C * DKP * 2;                     // bytes of one piece
     constexpr int G8 = DKP / 8;                           // threads per row of the tiles
-    constexpr int TT = C * C * 2;
-    extern __shared__ __align__(128) unsigned char sm[];
-    const uint32_t sK = (uint32_t)__cvta_generic_to_shared(sm), sQ = sK + NPK * TILE;
-    unsigned char* Csm = sm + 2 * NPK * TILE;             // C, two pieces
-    __shared__ double gam[C];
-    __shared__ float rowE[C], colE[3 * 48], bet[C], fK[C], fQ[C], fC[4];
-    __shared__ float dg[4][16][17];                       // diagonal blocks, per warp
-    __shared__ __align__(128) unsigned char Ysm[2 * 16 * 128];   // the row block in work, two pieces
-    const DecaySmem dec{gam, rowE, colE};
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunk = blockIdx.x, hk = blockIdx.y;
     long long tok0;
     int cnt;
+    pdl_release();
+    pdl_wait();   // the packed offsets
     if (!chunk_range<C>(d, chunk, tok0, cnt)) return;
-
-    // gates of the first head: in flight under the tiles' loads
-    float g2[2], b2[2];
-    const auto load_gates = [&](int hv) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int i = h * 32 + lane;
-            const long long at = (tok0 + i) * d.Hv + hv;
-            g2[h] = (d.g && i < cnt) ? d.g[at] : 0.0f;
-            b2[h] = i < cnt ? (d.beta ? d.beta[at] : 1.0f) : 0.0f;
-        }
-    };
-    if (warp < 2) load_gates(hk * d.grp);
+    float* kf = d.kf + ((size_t)chunk * d.Hk + hk) * 2 * C;
 
     char* gK = (char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
     char* gQ = (char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
@@ -171,7 +156,7 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
 #pragma unroll
             for (int o = 1; o < G8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             row_scale(m, up, down);
-            if (c8 == 0) (isq ? fQ : fK)[row] = down;
+            if (c8 == 0) kf[(isq ? C : 0) + row] = down;
             uint32_t w[4][NPK];
 #pragma unroll
             for (int e = 0; e < 4; e++) split_pair<NPK>(x[2 * e] * up, x[2 * e + 1] * up, w[e]);
@@ -179,19 +164,91 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
 #pragma unroll
             for (int k = 0; k < NPK; k++) {
                 const uint4 p = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
-                *(uint4*)(sm + (isq ? NPK * TILE : 0) + k * TILE + o) = p;
                 *(uint4*)((isq ? gQ : gK) + k * TILE + o) = p;
             }
         }
     }
+}
+
+template <int DKP, int NPK>
+__global__ void __launch_bounds__(128, DKP * NPK <= 128 ? KMB_PREP_BLOCKS : 3)
+delta_prep_kernel(const __grid_constant__ DeltaDesc d, int train) {
+    constexpr int C = kDeltaC;
+    constexpr int TILE = C * DKP * 2;                     // bytes of one piece
+    constexpr int TT = C * C * 2;
+    extern __shared__ __align__(128) unsigned char sm[];
+    const uint32_t sK = (uint32_t)__cvta_generic_to_shared(sm), sQ = sK + NPK * TILE;
+    unsigned char* Csm = sm;                              // C, two pieces, in the place of K and Q
+    __shared__ double gam[C];
+    __shared__ float rowE[C], colE[3 * 48], bet[C], fK[C], fQ[C], fC[4];
+    __shared__ float dg[4][16][17];                       // diagonal blocks, per warp
+    __shared__ __align__(128) unsigned char Ysm[2 * 16 * 128];   // the row block in work, two pieces
+    const DecaySmem dec{gam, rowE, colE};
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunk = blockIdx.x, hv = blockIdx.y, hk = hv / d.grp;
+    long long tok0;
+    int cnt;
+    pdl_release();
+    if (d.cu) pdl_wait();   // the packed offsets
+    if (!chunk_range<C>(d, chunk, tok0, cnt)) return;
+    float g2[2], b2[2];     // gates: tokens lane and lane + 32
+    if (warp < 2) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = h * 32 + lane;
+            const long long at = (tok0 + i) * d.Hv + hv;
+            g2[h] = (warp == 0 && d.g && i < cnt) ? d.g[at] : 0.0f;
+            b2[h] = (warp == 1 && i < cnt) ? (d.beta ? d.beta[at] : 1.0f) : 0.0f;
+        }
+    }
+    if (!d.cu) pdl_wait();
+    {
+        const char* gK = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+        const char* gQ = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NPK * C * DKP);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < NPK * TILE / 16; i += 128) {
+            cp16(sK + i * 16, gK + i * 16);
+            cp16(sQ + i * 16, gQ + i * 16);
+        }
+        cp_commit();
+    }
+    const size_t head = (size_t)chunk * d.Hv + hv;
+    float* tk = d.tok + head * TOK_SIZE;
+    if (warp == 0) {
+        running_sums(g2[0], g2[1], lane, gam);
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = h * 32 + lane;
+            if (train) d.gam[head * C + i] = gam[i];
+            tk[TOK_EG * C + i] = expf((float)gam[i]);
+            tk[TOK_GC * C + i] = expf((float)(gam[C - 1] - gam[i]));
+        }
+    } else if (warp == 1) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = h * 32 + lane;
+            bet[i] = b2[h];
+            tk[TOK_BETA * C + i] = b2[h];
+        }
+    } else {
+        const float* kf = d.kf + ((size_t)chunk * d.Hk + hk) * 2 * C;
+        const int i = threadIdx.x - 64;
+        const float k = kf[i], q = kf[C + i];
+        fK[i] = k;
+        fQ[i] = q;
+        tk[TOK_FK * C + i] = k;
+        tk[TOK_FQ * C + i] = q;
+    }
+    cp_wait<0>();
     __syncthreads();
+    decay_tables(dec, threadIdx.x);
     const int rg = warp;
     const int r = lane >> 2, c2 = (lane & 3) * 2;
-    float kk[C / 8][4], qk[C / 8][4];
+    float A[C / 8][4], B[C / 8][4];   // K K^T and Q K^T, columns up to the diagonal block; then a and P
+    zero(A);
+    zero(B);
 #pragma unroll
-    for (int t = 0; t < C / 8; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) kk[t][e] = qk[t][e] = 0.0f;
     for (int s = 0; s < DKP / 16; s++) {
         uint32_t ak[NPK][4], aq[NPK][4];
         const uint32_t oa = wide_off<C>(rg * 16 + la_row(lane), s * 16 + la_col(lane));
@@ -200,57 +257,39 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
             ldm4(ak[p], sK + p * TILE + oa);
             ldm4(aq[p], sQ + p * TILE + oa);
         }
-        auto ldb = [&](int p, int t2, uint32_t (&b)[4]) {
-            ldm4(b, sK + p * TILE + wide_off<C>(t2 * 16 + lb_row(lane), s * 16 + lb_col(lane)));
-        };
-        mma_row<NPK, NPK>(kk, ak, 0, C / 16, ldb);
-        mma_row<NPK, NPK>(qk, aq, 0, C / 16, ldb);
-    }
-    const uint32_t sC = (uint32_t)__cvta_generic_to_shared(Csm), sY = (uint32_t)__cvta_generic_to_shared(Ysm);
-    for (int hh = 0; hh < d.grp; hh++) {
-        const int hv = hk * d.grp + hh;
-        const size_t head = (size_t)chunk * d.Hv + hv;
-        float* tk = d.tok + head * TOK_SIZE;
-        __syncthreads();   // the last head's matrices are read
-        if (warp == 0) {
-            running_sums(g2[0], g2[1], lane, gam);
-            if (train) {
-                d.gam[head * C + lane] = gam[lane];
-                d.gam[head * C + lane + 32] = gam[lane + 32];
-            }
-        } else if (warp == 1) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int i = h * 32 + lane;
-                bet[i] = b2[h];
-                tk[TOK_BETA * C + i] = b2[h];
-                tk[TOK_FK * C + i] = fK[i];
-                tk[TOK_FQ * C + i] = fQ[i];
-            }
+        for (int t2 = 0; t2 < C / 16; t2++) {
+            if (t2 > rg) continue;
+            uint32_t b[NPK][4];
+#pragma unroll
+            for (int p = 0; p < NPK; p++)
+                ldm4(b[p], sK + p * TILE + wide_off<C>(t2 * 16 + lb_row(lane), s * 16 + lb_col(lane)));
+#pragma unroll
+            for (int pb = 0; pb < NPK; pb++)
+#pragma unroll
+                for (int pa = 0; pa + pb < NPK; pa++) {
+                    mma(A[2 * t2], ak[pa], b[pb][0], b[pb][1]);
+                    mma(A[2 * t2 + 1], ak[pa], b[pb][2], b[pb][3]);
+                    mma(B[2 * t2], aq[pa], b[pb][0], b[pb][1]);
+                    mma(B[2 * t2 + 1], aq[pa], b[pb][2], b[pb][3]);
+                }
         }
-        if (warp < 2 && hh + 1 < d.grp) load_gates(hv + 1);
-        __syncthreads();
-        decay_tables(dec, threadIdx.x);
-        if (threadIdx.x < C) {
-            const int i = threadIdx.x;
-            tk[TOK_EG * C + i] = expf((float)gam[i]);
-            tk[TOK_GC * C + i] = expf((float)(gam[C - 1] - gam[i]));
-        }
-        __syncthreads();
+    }
+    __syncthreads();   // the tables are there, K and Q are read
+    {
+        const uint32_t sC = sK, sY = (uint32_t)__cvta_generic_to_shared(Ysm);
         // rows of a and P on and below the warp's diagonal block
-        float A[C / 8][4], B[C / 8][4], pm = 0.0f;
+        float pm = 0.0f;
 #pragma unroll
         for (int t = 0; t < C / 8; t++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) A[t][e] = B[t][e] = 0.0f;
             if ((t >> 1) > rg) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = rg * 16 + r + (e >> 1) * 8, j = t * 8 + c2 + (e & 1);
                 const float G = dec.at(i, j, (t >> 1) == rg, rg) * fK[j];
-                B[t][e] = G * fQ[i] * qk[t][e];
+                B[t][e] *= G * fQ[i];
                 pm = fmaxf(pm, fabsf(B[t][e]));
-                A[t][e] = j < i ? G * fK[i] * kk[t][e] : 0.0f;
+                A[t][e] = j < i ? A[t][e] * (G * fK[i]) : 0.0f;
             }
         }
         float up, down;
@@ -403,15 +442,17 @@ delta_prep_kernel(const __grid_constant__ DeltaDesc d, int vec, int train) {
 template <int DKP, typename IO>
 cudaError_t prep_go(const DeltaDesc& d, int train, cudaStream_t st) {
     constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1;
-    const int sm = 2 * NPK * C * DKP * 2 + 2 * C * C * 2;
-    auto kern = delta_prep_kernel<DKP, IO>;
+    constexpr int kq = 2 * NPK * C * DKP * 2, cc = 2 * C * C * 2, sm = kq > cc ? kq : cc;
+    auto kern = delta_prep_kernel<DKP, NPK>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm);
     if (e != cudaSuccess) return e;
     const int V = 16 / (int)sizeof(IO);
     const int vec = d.dk % V == 0 && d.ld_q % V == 0 && d.ld_k % V == 0 && ((uintptr_t)d.q & 15) == 0 &&
                     ((uintptr_t)d.k & 15) == 0;
-    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 128, sm, st>>>(d, vec, train);
-    return cudaGetLastError();
+    e = launch(delta_tiles_kernel<DKP, IO>, dim3((unsigned)d.nch, (unsigned)d.Hk), dim3(128), 0, st, d.cu != nullptr, d,
+               vec);
+    if (e != cudaSuccess) return e;
+    return launch(kern, dim3((unsigned)d.nch, (unsigned)d.Hv), dim3(128), sm, st, true, d, train);
 }
 
 // ------------------------------------------------------------------ recurrent form
@@ -603,6 +644,7 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
     d.Qt = (__half*)take(ck * NPK * C * DKP * 2);
     d.Mt = (__half*)take(cv * 2 * C * C * 2);
     d.Pt = (__half*)take(cv * 2 * C * C * 2);
+    d.kf = (float*)take(ck * 2 * C * 4);
     d.tok = (float*)take(cv * TOK_SIZE * 4);
     if (train) {
         const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
@@ -612,9 +654,8 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
         d.Wh = (__half*)take(u * 2 * C);
         d.Of = (float*)take(u * 2 * C);
         d.Gh = (__half*)take(u * NPK * C);
-        d.Rh = (__half*)take(u * NPK * C);
+        d.Rh = (__half*)take(u * 2 * C);
         d.dSh = (__half*)take(u * NPK * DKP);
-        d.part = (float*)take(cv * d.units * 2 * C * 4);
         d.anchor = (float*)take(cv * d.units * 4 * 4);
         d.mx = (float*)take(cv * d.units * 4 * MX_ROWS * 4);
     }

@@ -17,8 +17,9 @@
 //   dgamma_t = do_t.o_t - v_t.dv_t;   dg_t = <S_0, dS_0> - sum_{s < t in chunk} dgamma_s
 // (the state's inner product at the chunk's start anchors the sum, so errors do
 // not add up along the sequence), and dbeta_t = dR_t.w_t.  Both are sums
-// over dv of what the recurrence holds in fp32.
+// over dv of what the recurrences leave in two pieces.
 #include "kmb_delta.cuh"
+#include "kmb_launch.cuh"
 
 namespace kmb {
 namespace {
@@ -62,6 +63,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
+    pdl_release();
     const int n = d.order ? d.order[nr] : nr;
     const bool on = u < d.units;
     const int r = lane >> 2, c2 = (lane & 3) * 2;
@@ -204,7 +206,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
 
     // side warps
     using RT = typename RawOf<IO>::type;
-    const int ldv = (int)d.ld_v, ldg = (int)d.ld_do, lddv = (int)d.ld_dv;
+    const int ldg = (int)d.ld_do;
     const auto load_t = [&](const void* base, long long ld, int ldi, int c, RT (&V)[2][4]) {
         const long long t0 = (long long)c * C + w * 16;
         const RT* p = (const RT*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
@@ -292,27 +294,9 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         const int c = nch - 1 - it;
         if (!begin(it)) return;
         const uint32_t st = sb + stage(it) * ST::BYTES;
-        const float* tk = (const float*)(sm + stage(it) * ST::BYTES + ST::oTok);
-        const float* tw = tk + w * 16 + c2;
         const size_t fb = unit_at(c);
         float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
-        // what the chunk's sums need, and the next chunk's dO: in flight under the products
-        RT V[2][4];
-        uint32_t wr[2][2][2];
-        float4 o4[2];
-        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);
-        load_t(d.v, d.ld_v, ldv, c, V);
-        float fw = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            o4[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            wr[t][0][0] = wr[t][0][1] = wr[t][1][0] = wr[t][1][1] = 0;
-            if (on) {
-                o4[t] = ((const float4*)d.Of)[(fb * (C / 8) + w * 2 + t) * 32 + lane];
-                get_tile<64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, (w * 2 + t) * 8, wr[t]);
-            }
-        }
-        if (on) fw = mx[MX_W];
+        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);   // in flight under the products
         // keep dS_C; its product with the state at the same place
         if (it > 0) anchor(c + 1);
 #pragma unroll
@@ -346,45 +330,14 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             put_acc(exZ, w * KTW, lane, Z);
         }
         unit_bar(grp);
-        // dV, and what the gates' gradients sum over dv
-        float Y[2][4];
+        float Y[2][4];   // dR, kept
         get_acc(exR, w * 2, lane, Y);
         if (on) {
-            uint32_t a[NPK][4];
+            uint32_t a[2][4];
             frag_scale(Y, up, dn);
-            frag_pieces<NPK>(Y[0], Y[1], up, a);
-            put_frag<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+            frag_pieces<2>(Y[0], Y[1], up, a);
+            put_frag<2, 64>(d.Rh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
             if (lane == 0) mx[MX_R] = dn;
-            const long long t0 = (long long)c * C + w * 16;
-            IO* pd = (IO*)d.dvv + (start + t0) * d.ld_dv + (long long)hv * d.dv + col[0];
-            float ts[2][2], bs[2][2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const float2 wa = join(wr[t][0][0], wr[t][0][1]), wb = join(wr[t][1][0], wr[t][1][1]);
-                const float ww[4] = {wa.x, wa.y, wb.x, wb.y}, oo[4] = {o4[t].x, o4[t].y, o4[t].z, o4[t].w};
-                ts[t][0] = ts[t][1] = bs[t][0] = bs[t][1] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    const float dv = tw[TOK_BETA * C + t * 8 + (e & 1)] * Y[t][e];
-                    bs[t][e & 1] = fmaf(Y[t][e], ww[e], bs[t][e & 1]);
-                    ts[t][e & 1] = fmaf(G[t][e], oo[e], ts[t][e & 1]);
-                    ts[t][e & 1] = fmaf(-from_raw(V[t][e]), dv, ts[t][e & 1]);
-                    if (t0 + i < len && cok[e >> 1]) stt(pd + (long long)i * lddv, (e >> 1) * 8, dv);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        ts[t][h] += __shfl_xor_sync(0xffffffffu, ts[t][h], o);
-                        bs[t][h] += __shfl_xor_sync(0xffffffffu, bs[t][h], o);
-                    }
-                if (r == t) {
-                    float* pp = d.part + fb * 2 * C + w * 16 + t * 8 + c2;
-                    *(float2*)pp = make_float2(ts[t][0], ts[t][1]);
-                    *(float2*)(pp + C) = make_float2(bs[t][0] * fw, bs[t][1] * fw);
-                }
-            }
         }
         if (c > 0) {
             if (!arrived(it + 1)) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
@@ -412,23 +365,23 @@ struct GradSmem {
     static constexpr int oMx = oTok + TOK_SIZE * 4;
     static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
     static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
-    static constexpr int BYTES = oCol + 3 * 48 * 4;
+    static constexpr int oPart = oCol + 3 * 48 * 4;   // [8 units][2][C]
+    static constexpr int BYTES = oPart + 8 * 2 * C * 4;
 };
 
-// One warp: gradients of the gates of a chunk's tokens (lane and lane + 32) from the recurrence's sums over dv
-__device__ __forceinline__ void gate_grads(const DeltaDesc& d, size_t head, long long tok0, int cnt, int hv, int lane) {
+// One warp: gradients of the gates of a chunk's tokens (lane and lane + 32) from the sums over dv, part [units][2][C]
+__device__ __forceinline__ void gate_grads(const DeltaDesc& d, const float* part, size_t head, long long tok0, int cnt,
+                                           int hv, int lane) {
     constexpr int C = kDeltaC;
     double anchor = lane < d.units * 4 ? (double)d.anchor[head * d.units * 4 + lane] : 0.0;
     double t[2] = {0.0, 0.0};
     float b[2] = {0.0f, 0.0f};
-#pragma unroll 4
     for (int x = 0; x < d.units; x++) {
-        const float* p = d.part + (head * d.units + x) * 2 * C + lane;
-        const float v0 = p[0], v1 = p[32], v2 = p[C], v3 = p[C + 32];
-        t[0] += v0;
-        t[1] += v1;
-        b[0] += v2;
-        b[1] += v3;
+        const float* p = part + x * 2 * C + lane;
+        t[0] += p[0];
+        t[1] += p[32];
+        b[0] += p[C];
+        b[1] += p[C + 32];
     }
     double s[2] = {t[0], t[1]};
 #pragma unroll
@@ -467,7 +420,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     __shared__ float red[4][8];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     float* tk = (float*)(sm + SM::oTok);
-    float* mx = (float*)(sm + SM::oMx);
+    float *mx = (float*)(sm + SM::oMx), *part = (float*)(sm + SM::oPart);
     DecaySmem dec{(double*)(sm + SM::oGam), (float*)(sm + SM::oRow), (float*)(sm + SM::oCol)};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rg = warp & 3, ch = warp >> 2;
@@ -475,7 +428,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     const int chunk = blockIdx.x, hk = blockIdx.y;
     long long tok0;
     int cnt;
-    if (!chunk_range<C>(d, chunk, tok0, cnt)) return;
+    if (!chunk_range<C>(d, chunk, tok0, cnt)) return;   // the offsets are the forward's
     {
         const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NP * C * DKP);
         const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NP * C * DKP);
@@ -485,6 +438,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
         }
         cp_commit();
     }
+    pdl_wait();
     float dQ[HT][4], dK[HT][4];
     zero(dQ);
     zero(dK);
@@ -498,10 +452,10 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             for (int i = tid; i < nx * NP * 128; i += 256) {
                 const int x = i / (NP * 128), p = i / 128 % NP, o = (i & 127) * 16;
                 const size_t g = ((head * d.units + u0 + x) * NP + p) * 2048 + o;
-                const size_t gw = ((head * d.units + u0 + x) * 2 + p) * 2048 + o;   // W keeps both pieces
+                const size_t gw = ((head * d.units + u0 + x) * 2 + p) * 2048 + o;   // dR and W keep both pieces
                 const uint32_t s = sb + p * SM::T64 + x * 2048 + o;
                 cp16(s + SM::oG, (const char*)d.Gh + g);
-                cp16(s + SM::oR, (const char*)d.Rh + g);
+                cp16(s + SM::oR, (const char*)d.Rh + gw);
                 cp16(s + SM::oW, (const char*)d.Wh + gw);
             }
             for (int i = tid; i < nx * NP * SM::NH * 128; i += 256) {
@@ -513,6 +467,74 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 cp16(s + SM::oS, (const char*)d.Sh + gs);
             }
             cp_commit();
+        };
+        // dV of a unit's 16 columns and 16 tokens, and what the gates' gradients sum over dv: do.o - v.dv and dR.w
+        const auto sums_over_dv = [&](size_t head, int hv, int u0, int x, int wb) {
+            const size_t fb = head * d.units + u0 + x;
+            const float* m4 = mx + ((u0 + x) * 4 + wb) * MX_ROWS;
+            const float sG = m4[MX_DO], sR = m4[MX_R], sW = m4[MX_W];
+            const int c0 = (u0 + x) * 16 + r;
+            const bool ok[2] = {c0 < d.dv, c0 + 8 < d.dv};
+            const IO* pv = (const IO*)d.v + (tok0 + wb * 16) * d.ld_v + (long long)hv * d.dv + c0;
+            IO* pd = (IO*)d.dvv + (tok0 + wb * 16) * d.ld_dv + (long long)hv * d.dv + c0;
+            const int ldv = (int)d.ld_v, lddv = (int)d.ld_dv;
+            float4 o4[2];
+            uint32_t rl[2][2], wl[2][2];
+            typename RawOf<IO>::type V[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                o4[t] = ((const float4*)d.Of)[(fb * (C / 8) + wb * 2 + t) * 32 + lane];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t o = tile_off<64>(r + 8 * h, wb * 16 + t * 8 + c2);
+                    if (NP == 1) {   // the second pieces are not in shared memory
+                        rl[t][h] = *(const uint32_t*)((const char*)(d.Rh + (fb * 2 + 1) * 16 * C) + o);
+                        wl[t][h] = *(const uint32_t*)((const char*)(d.Wh + (fb * 2 + 1) * 16 * C) + o);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = t * 8 + c2 + (e & 1);
+                    V[t][e] = (wb * 16 + i < cnt && ok[e >> 1])
+                                  ? ((const typename RawOf<IO>::type*)pv)[(long long)i * ldv + (e >> 1) * 8] : 0;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                float ts[2] = {0.0f, 0.0f}, bs[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t o = x * 2048 + tile_off<64>(r + 8 * h, wb * 16 + t * 8 + c2);
+                    const auto at = [&](int base, int p) { return *(const uint32_t*)(sm + base + p * SM::T64 + o); };
+                    const float2 R2 = join(at(SM::oR, 0), NP == 1 ? rl[t][h] : at(SM::oR, NP - 1));
+                    const float2 W2 = join(at(SM::oW, 0), NP == 1 ? wl[t][h] : at(SM::oW, NP - 1));
+                    const float2 G2 = NP == 1 ? __half22float2(*reinterpret_cast<const __half2*>(sm + SM::oG + o))
+                                              : join(at(SM::oG, 0), at(SM::oG, NP - 1));
+                    const float Rr[2] = {R2.x * sR, R2.y * sR}, Ww[2] = {W2.x * sW, W2.y * sW}, Gg[2] = {G2.x * sG, G2.y * sG};
+                    const float oo[2] = {h ? o4[t].z : o4[t].x, h ? o4[t].w : o4[t].y};
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int i = t * 8 + c2 + e;
+                        const float dv = tk[TOK_BETA * C + wb * 16 + i] * Rr[e];
+                        bs[e] = fmaf(Rr[e], Ww[e], bs[e]);
+                        ts[e] = fmaf(Gg[e], oo[e], ts[e]);
+                        ts[e] = fmaf(-from_raw(V[t][h * 2 + e]), dv, ts[e]);
+                        if (wb * 16 + i < cnt && ok[h]) stt(pd + (long long)i * lddv, h * 8, dv);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        ts[e] += __shfl_xor_sync(0xffffffffu, ts[e], o);
+                        bs[e] += __shfl_xor_sync(0xffffffffu, bs[e], o);
+                    }
+                if (r == t) {
+                    float* pp = part + (u0 + x) * 2 * C + wb * 16 + t * 8 + c2;
+                    *(float2*)pp = make_float2(ts[0], ts[1]);
+                    *(float2*)(pp + C) = make_float2(bs[0], bs[1]);
+                }
+            }
         };
         __syncthreads();
         for (int i = tid; i < TOK_SIZE / 4; i += 256) cp16(sb + SM::oTok + i * 16, d.tok + head * TOK_SIZE + i * 4);
@@ -543,6 +565,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 __syncthreads();
             }
             const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
+            for (int pr = warp; pr < nx * 4; pr += 8) sums_over_dv(head, hv, u0, pr >> 2, pr & 3);
             for (int kk = 0; kk < nx; kk++) {
                 const float* m4 = mx + (u0 + kk) * 4 * MX_ROWS;
                 const float sG = m4[rg * MX_ROWS + MX_DO], sR = m4[rg * MX_ROWS + MX_R], sW = m4[rg * MX_ROWS + MX_W];
@@ -660,7 +683,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             }
         }
         __syncthreads();
-        if (warp == 1 && (d.dg || d.dbeta)) gate_grads(d, head, tok0, cnt, hv, lane);
+        if (warp == 1 && (d.dg || d.dbeta)) gate_grads(d, part, head, tok0, cnt, hv, lane);
         // the four products over tokens
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -734,8 +757,7 @@ cudaError_t grads_go(const DeltaDesc& d, cudaStream_t st) {
     auto kern = delta_grads_kernel<DKP, IO>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES);
     if (e != cudaSuccess) return e;
-    kern<<<dim3((unsigned)d.nch, (unsigned)d.Hk), 256, SM::BYTES, st>>>(d);
-    return cudaGetLastError();
+    return launch(kern, dim3((unsigned)d.nch, (unsigned)d.Hk), dim3(256), SM::BYTES, st, true, d);
 }
 }  // namespace
 

@@ -4,6 +4,7 @@
 // all transposed.  The chain of a chunk is latency: three products that each wait
 // for the last, with fp16 pieces made and passed on between them.
 #include "kmb_delta.cuh"
+#include "kmb_launch.cuh"
 
 namespace kmb {
 namespace {
@@ -46,6 +47,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
+    pdl_release();
+    pdl_wait();
     const int n = d.order ? d.order[nr] : nr;
     const bool on = u < d.units;                 // a unit past dv computes on zeros and stores nothing
     const int r = lane >> 2, c2 = (lane & 3) * 2;
@@ -289,8 +292,7 @@ cudaError_t go(const DeltaDesc& d, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
-    kern<<<(unsigned)blocks, 256 * NU, SMEM, st>>>(d);
-    return cudaGetLastError();
+    return launch(kern, dim3((unsigned)blocks), dim3(256 * NU), SMEM, st, d.nch > 0, d);
 }
 template <int DKP, typename IO>
 cudaError_t pick(const DeltaDesc& d, bool keep, cudaStream_t st) {

@@ -60,6 +60,7 @@ struct DeltaDesc {
     // workspace
     __half *Kt, *Qt;             // [nch][Hk][pieces][C * DKP] swizzled tiles, rows scaled
     __half *Mt, *Pt, *Tt;        // [nch][Hv][2][C * C], on and below the diagonal blocks; Tt for training only
+    float* kf;                   // [nch][Hk][2][C]: what the rows of the K and of the Q tile are times
     float* tok;                  // [nch][Hv][TOK_SIZE], see TOK_*
     double* gam;                 // [nch][Hv][C]: running sums of g (training)
     const int* order;            // packed: sequences, the longest first (NULL: as they are)
@@ -67,8 +68,8 @@ struct DeltaDesc {
     // scaled by a power of two (mx)
     __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [2][16 * C]
     float* Of;                   // O, in accumulator order [C / 8 tiles][32 lanes][4]
-    __half *Gh, *Rh, *dSh;       // backward: dO, dR = T^T dU [pieces][16 * C], adjoint of the state at the chunk's end
-    float *part, *anchor;        // [nch][Hv][units][2][C], [nch][Hv][units][4 warps]
+    __half *Gh, *Rh, *dSh;       // backward: dO [pieces][16 * C], dR = T^T dU [2][16 * C], adjoint of the state at the end
+    float* anchor;               // [nch][Hv][units][4 warps]: <S_0, dS_0> of their parts
     float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: what the tiles of S, W, dO, dR, dS are times
     // gradients
     const void* go;
@@ -414,10 +415,13 @@ __device__ __forceinline__ void get_acc(const unsigned char* base, int tile, int
 }
 
 int delta_sms();
-// Units per block: one where every SM gets a unit at most (the chain of a chunk is bound by latency), two where
-// there are more units than SMs (they share the copies of the tiles).
+// Units per block.  One gives the shorter chain (a chunk of dk = dv = 64: forward 2.2 us against 3.1, backward 4.0
+// against 5.2 with two), two more units per SM.  So one where every SM gets a unit at most; with sequences of one
+// length two above that.  Packed sequences are of unknown lengths, and the longest's chain is what counts
+// until there are several times as many units as SMs.
 inline int delta_units(const DeltaDesc& d) {
-    return d.units > 1 && (long long)d.nseq * d.Hv * d.units > delta_sms() ? 2 : 1;
+    const long long all = (long long)d.nseq * d.Hv * d.units;
+    return d.units > 1 && all > (d.cu ? 8 : 1) * delta_sms() ? 2 : 1;
 }
 
 cudaError_t delta_chain_fwd(const DeltaDesc& d, int DKP, bool bf16, bool keep, cudaStream_t st);
