@@ -17,7 +17,7 @@
 //   dgamma_t = do_t.o_t - v_t.dv_t;   dg_t = <S_0, dS_0> - sum_{s < t in chunk} dgamma_s
 // (the state's inner product at the chunk's start anchors the sum, so errors do
 // not add up along the sequence), and dbeta_t = dR_t.w_t.  Both are sums
-// over dv of what the recurrences leave in two pieces.
+// over dv of what the recurrences leave in fp32.
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 
@@ -333,11 +333,12 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         float Y[2][4];   // dR, kept
         get_acc(exR, w * 2, lane, Y);
         if (on) {
-            uint32_t a[2][4];
+            uint32_t a[NPK][4];
             frag_scale(Y, up, dn);
-            frag_pieces<2>(Y[0], Y[1], up, a);
-            put_frag<2, 64>(d.Rh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
+            frag_pieces<NPK>(Y[0], Y[1], up, a);
+            put_frag<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
             if (lane == 0) mx[MX_R] = dn;
+            put_acc((unsigned char*)(d.Rf + fb * 16 * C), w * 2, lane, Y);
         }
         if (c > 0) {
             if (!arrived(it + 1)) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
@@ -348,41 +349,91 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     if (nch > 0) anchor(0);
 }
 
-// ------------------------------------------------------------------ gradients without recurrence
-// Eight warps: 16 token rows x half of dk (and half of the 64 columns of dP, dA) each.  dv is walked in slices of
-// four units, whose fp16 tiles come as the recurrences left them: one piece for bf16 results (11 bits are enough
-// before the rounding), two for fp32.  A unit is one step of 16 in the products over dv, so its powers of two are
-// applied when the step's products are added to the fp32 sums.
-template <int DKP, int NP>
-struct GradSmem {
-    static constexpr int C = kDeltaC, NH = DKP / 64;
-    static constexpr int KQ = NP * C * DKP * 2, T64 = 64 * C * 2, SD = NH * 64 * 128;
-    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oW = oG + NP * T64, oR = oW + NP * T64, oS = oR + NP * T64,
-                         oD = oS + NP * SD, oEnd = oD + NP * SD;
-    // the four weighted matrices take the place of the slices
-    static constexpr int oE = oG, TE = C * C * 2;
-    static constexpr int oTok = (oE + 4 * NP * TE > oEnd ? oE + 4 * NP * TE : oEnd);
-    static constexpr int oMx = oTok + TOK_SIZE * 4;
-    static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
-    static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
-    static constexpr int oPart = oCol + 3 * 48 * 4;   // [8 units][2][C]
-    static constexpr int BYTES = oPart + 8 * 2 * C * 4;
-};
-
-// One warp: gradients of the gates of a chunk's tokens (lane and lane + 32) from the sums over dv, part [units][2][C]
-__device__ __forceinline__ void gate_grads(const DeltaDesc& d, const float* part, size_t head, long long tok0, int cnt,
-                                           int hv, int lane) {
-    constexpr int C = kDeltaC;
-    double anchor = lane < d.units * 4 ? (double)d.anchor[head * d.units * 4 + lane] : 0.0;
-    double t[2] = {0.0, 0.0};
-    float b[2] = {0.0f, 0.0f};
-    for (int x = 0; x < d.units; x++) {
-        const float* p = part + x * 2 * C + lane;
-        t[0] += p[0];
-        t[1] += p[32];
-        b[0] += p[C];
-        b[1] += p[C + 32];
+// ------------------------------------------------------------------ dV and the gates
+// Block = (chunk, value head), warp = 16 of its tokens over all of dv: dV = beta dR, and per token the sums over dv
+// that the gates' gradients are made of.  Bound by what it reads and writes.
+template <typename IO>
+__global__ void __launch_bounds__(128)
+delta_gates_kernel(const __grid_constant__ DeltaDesc d) {
+    constexpr int C = kDeltaC, NP = sizeof(IO) == 4 ? 2 : 1;
+    using RT = typename RawOf<IO>::type;
+    __shared__ float sums[2][C];
+    const int lane = threadIdx.x & 31, wb = threadIdx.x >> 5;
+    const int r = lane >> 2, c2 = (lane & 3) * 2;
+    const int chunk = blockIdx.x, hv = blockIdx.y;
+    long long tok0;
+    int cnt;
+    pdl_release();
+    if (!chunk_range<C>(d, chunk, tok0, cnt)) return;   // the offsets are the forward's
+    pdl_wait();
+    const size_t head = (size_t)chunk * d.Hv + hv;
+    const int ldv = (int)d.ld_v, lddv = (int)d.ld_dv;
+    const float* tk = d.tok + head * TOK_SIZE + TOK_BETA * C + wb * 16 + c2;
+    const float2 be[2] = {*(const float2*)tk, *(const float2*)(tk + 8)};
+    float ts[2][2] = {}, bs[2][2] = {};
+#pragma unroll 2
+    for (int u = 0; u < d.units; u++) {
+        const size_t fb = head * d.units + u;
+        const float* mx = d.mx + (fb * 4 + wb) * MX_ROWS;
+        const int c0 = u * 16 + r;
+        const bool ok[2] = {c0 < d.dv, c0 + 8 < d.dv};
+        const RT* pv = (const RT*)d.v + (tok0 + wb * 16) * d.ld_v + (long long)hv * d.dv + c0;
+        IO* pd = (IO*)d.dvv + (tok0 + wb * 16) * d.ld_dv + (long long)hv * d.dv + c0;
+        float O[2][4], R[2][4], W[2][4];
+        uint32_t G[2][2][2];
+        RT V[2][4];
+        get_acc((const unsigned char*)(d.Of + fb * 16 * C), wb * 2, lane, O);
+        get_acc((const unsigned char*)(d.Rf + fb * 16 * C), wb * 2, lane, R);
+        get_acc((const unsigned char*)(d.Wf + fb * 16 * C), wb * 2, lane, W);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            get_tile<64, NP>(d.Gh + fb * NP * 16 * C, 16 * C, lane, wb * 16 + t * 8, G[t]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = t * 8 + c2 + (e & 1);
+                V[t][e] = (wb * 16 + i < cnt && ok[e >> 1]) ? pv[(long long)i * ldv + (e >> 1) * 8] : RT(0);
+            }
+        }
+        const float sG = mx[MX_DO];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float2 g2 = NP == 2 ? join(G[t][h][0], G[t][h][1])
+                                          : __half22float2(*reinterpret_cast<const __half2*>(&G[t][h][0]));
+                const float gg[2] = {g2.x * sG, g2.y * sG};
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = t * 8 + c2 + e;
+                    const float dv = (e ? be[t].y : be[t].x) * R[t][h * 2 + e];
+                    bs[t][e] = fmaf(R[t][h * 2 + e], W[t][h * 2 + e], bs[t][e]);
+                    ts[t][e] = fmaf(gg[e], O[t][h * 2 + e], ts[t][e]);
+                    ts[t][e] = fmaf(-from_raw(V[t][h * 2 + e]), dv, ts[t][e]);
+                    if (wb * 16 + i < cnt && ok[h]) stt(pd + (long long)i * lddv, h * 8, dv);
+                }
+            }
     }
+    if (!d.dg && !d.dbeta) return;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                ts[t][e] += __shfl_xor_sync(0xffffffffu, ts[t][e], o);
+                bs[t][e] += __shfl_xor_sync(0xffffffffu, bs[t][e], o);
+            }
+    if (r < 2) {   // row r of the lanes writes tile r
+        sums[0][wb * 16 + r * 8 + c2] = r ? ts[1][0] : ts[0][0];
+        sums[0][wb * 16 + r * 8 + c2 + 1] = r ? ts[1][1] : ts[0][1];
+        sums[1][wb * 16 + r * 8 + c2] = r ? bs[1][0] : bs[0][0];
+        sums[1][wb * 16 + r * 8 + c2 + 1] = r ? bs[1][1] : bs[0][1];
+    }
+    __syncthreads();
+    if (wb) return;
+    // one warp: running sums over the chunk's tokens (lane and lane + 32) from <S_0, dS_0>
+    double anchor = lane < d.units * 4 ? (double)d.anchor[head * d.units * 4 + lane] : 0.0;
+    const double t[2] = {sums[0][lane], sums[0][lane + 32]};
     double s[2] = {t[0], t[1]};
 #pragma unroll
     for (int o = 16; o; o >>= 1) anchor += __shfl_xor_sync(0xffffffffu, anchor, o);
@@ -403,9 +454,29 @@ __device__ __forceinline__ void gate_grads(const DeltaDesc& d, const float* part
         // a decay below e^-104 is 0 in fp32: nothing depends on it
         const bool reset = d.g && d.g[at] < -104.0f;
         if (d.dg) d.dg[at] = reset ? 0.0f : (float)(anchor - (s[h] - t[h]));
-        if (d.dbeta) d.dbeta[at] = b[h];
+        if (d.dbeta) d.dbeta[at] = sums[1][i];
     }
 }
+
+// ------------------------------------------------------------------ gradients without recurrence
+// Eight warps: 16 token rows x half of dk (and half of the 64 columns of dP, dA) each.  dv is walked in slices of
+// four units, whose fp16 tiles come as the recurrences left them: one piece for bf16 results (11 bits are enough
+// before the rounding), two for fp32.  A unit is one step of 16 in the products over dv, so its powers of two are
+// applied when the step's products are added to the fp32 sums.
+template <int DKP, int NP>
+struct GradSmem {
+    static constexpr int C = kDeltaC, NH = DKP / 64;
+    static constexpr int KQ = NP * C * DKP * 2, T64 = 64 * C * 2, SD = NH * 64 * 128;
+    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oW = oG + NP * T64, oR = oW + NP * T64, oS = oR + NP * T64,
+                         oD = oS + NP * SD, oEnd = oD + NP * SD;
+    // the four weighted matrices take the place of the slices
+    static constexpr int oE = oG, TE = C * C * 2;
+    static constexpr int oTok = (oE + 4 * NP * TE > oEnd ? oE + 4 * NP * TE : oEnd);
+    static constexpr int oMx = oTok + TOK_SIZE * 4;
+    static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
+    static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
+    static constexpr int BYTES = oCol + 3 * 48 * 4;
+};
 
 template <int DKP, typename IO>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1)
@@ -420,7 +491,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     __shared__ float red[4][8];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     float* tk = (float*)(sm + SM::oTok);
-    float *mx = (float*)(sm + SM::oMx), *part = (float*)(sm + SM::oPart);
+    float* mx = (float*)(sm + SM::oMx);
     DecaySmem dec{(double*)(sm + SM::oGam), (float*)(sm + SM::oRow), (float*)(sm + SM::oCol)};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rg = warp & 3, ch = warp >> 2;
@@ -452,11 +523,10 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             for (int i = tid; i < nx * NP * 128; i += 256) {
                 const int x = i / (NP * 128), p = i / 128 % NP, o = (i & 127) * 16;
                 const size_t g = ((head * d.units + u0 + x) * NP + p) * 2048 + o;
-                const size_t gw = ((head * d.units + u0 + x) * 2 + p) * 2048 + o;   // dR and W keep both pieces
                 const uint32_t s = sb + p * SM::T64 + x * 2048 + o;
                 cp16(s + SM::oG, (const char*)d.Gh + g);
-                cp16(s + SM::oR, (const char*)d.Rh + gw);
-                cp16(s + SM::oW, (const char*)d.Wh + gw);
+                cp16(s + SM::oR, (const char*)d.Rh + g);
+                cp16(s + SM::oW, (const char*)d.Wh + g);
             }
             for (int i = tid; i < nx * NP * SM::NH * 128; i += 256) {
                 const int x = i / (NP * SM::NH * 128), p = i / (SM::NH * 128) % NP, h = i / 128 % SM::NH, o = (i & 127) * 16;
@@ -467,74 +537,6 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 cp16(s + SM::oS, (const char*)d.Sh + gs);
             }
             cp_commit();
-        };
-        // dV of a unit's 16 columns and 16 tokens, and what the gates' gradients sum over dv: do.o - v.dv and dR.w
-        const auto sums_over_dv = [&](size_t head, int hv, int u0, int x, int wb) {
-            const size_t fb = head * d.units + u0 + x;
-            const float* m4 = mx + ((u0 + x) * 4 + wb) * MX_ROWS;
-            const float sG = m4[MX_DO], sR = m4[MX_R], sW = m4[MX_W];
-            const int c0 = (u0 + x) * 16 + r;
-            const bool ok[2] = {c0 < d.dv, c0 + 8 < d.dv};
-            const IO* pv = (const IO*)d.v + (tok0 + wb * 16) * d.ld_v + (long long)hv * d.dv + c0;
-            IO* pd = (IO*)d.dvv + (tok0 + wb * 16) * d.ld_dv + (long long)hv * d.dv + c0;
-            const int ldv = (int)d.ld_v, lddv = (int)d.ld_dv;
-            float4 o4[2];
-            uint32_t rl[2][2], wl[2][2];
-            typename RawOf<IO>::type V[2][4];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                o4[t] = ((const float4*)d.Of)[(fb * (C / 8) + wb * 2 + t) * 32 + lane];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t o = tile_off<64>(r + 8 * h, wb * 16 + t * 8 + c2);
-                    if (NP == 1) {   // the second pieces are not in shared memory
-                        rl[t][h] = *(const uint32_t*)((const char*)(d.Rh + (fb * 2 + 1) * 16 * C) + o);
-                        wl[t][h] = *(const uint32_t*)((const char*)(d.Wh + (fb * 2 + 1) * 16 * C) + o);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    V[t][e] = (wb * 16 + i < cnt && ok[e >> 1])
-                                  ? ((const typename RawOf<IO>::type*)pv)[(long long)i * ldv + (e >> 1) * 8] : 0;
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                float ts[2] = {0.0f, 0.0f}, bs[2] = {0.0f, 0.0f};
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t o = x * 2048 + tile_off<64>(r + 8 * h, wb * 16 + t * 8 + c2);
-                    const auto at = [&](int base, int p) { return *(const uint32_t*)(sm + base + p * SM::T64 + o); };
-                    const float2 R2 = join(at(SM::oR, 0), NP == 1 ? rl[t][h] : at(SM::oR, NP - 1));
-                    const float2 W2 = join(at(SM::oW, 0), NP == 1 ? wl[t][h] : at(SM::oW, NP - 1));
-                    const float2 G2 = NP == 1 ? __half22float2(*reinterpret_cast<const __half2*>(sm + SM::oG + o))
-                                              : join(at(SM::oG, 0), at(SM::oG, NP - 1));
-                    const float Rr[2] = {R2.x * sR, R2.y * sR}, Ww[2] = {W2.x * sW, W2.y * sW}, Gg[2] = {G2.x * sG, G2.y * sG};
-                    const float oo[2] = {h ? o4[t].z : o4[t].x, h ? o4[t].w : o4[t].y};
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int i = t * 8 + c2 + e;
-                        const float dv = tk[TOK_BETA * C + wb * 16 + i] * Rr[e];
-                        bs[e] = fmaf(Rr[e], Ww[e], bs[e]);
-                        ts[e] = fmaf(Gg[e], oo[e], ts[e]);
-                        ts[e] = fmaf(-from_raw(V[t][h * 2 + e]), dv, ts[e]);
-                        if (wb * 16 + i < cnt && ok[h]) stt(pd + (long long)i * lddv, h * 8, dv);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        ts[e] += __shfl_xor_sync(0xffffffffu, ts[e], o);
-                        bs[e] += __shfl_xor_sync(0xffffffffu, bs[e], o);
-                    }
-                if (r == t) {
-                    float* pp = part + (u0 + x) * 2 * C + wb * 16 + t * 8 + c2;
-                    *(float2*)pp = make_float2(ts[0], ts[1]);
-                    *(float2*)(pp + C) = make_float2(bs[0], bs[1]);
-                }
-            }
         };
         __syncthreads();
         for (int i = tid; i < TOK_SIZE / 4; i += 256) cp16(sb + SM::oTok + i * 16, d.tok + head * TOK_SIZE + i * 4);
@@ -565,7 +567,6 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 __syncthreads();
             }
             const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
-            for (int pr = warp; pr < nx * 4; pr += 8) sums_over_dv(head, hv, u0, pr >> 2, pr & 3);
             for (int kk = 0; kk < nx; kk++) {
                 const float* m4 = mx + (u0 + kk) * 4 * MX_ROWS;
                 const float sG = m4[rg * MX_ROWS + MX_DO], sR = m4[rg * MX_ROWS + MX_R], sW = m4[rg * MX_ROWS + MX_W];
@@ -683,7 +684,6 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             }
         }
         __syncthreads();
-        if (warp == 1 && (d.dg || d.dbeta)) gate_grads(d, part, head, tok0, cnt, hv, lane);
         // the four products over tokens
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -756,6 +756,8 @@ cudaError_t grads_go(const DeltaDesc& d, cudaStream_t st) {
     using SM = GradSmem<DKP, sizeof(IO) == 4 ? 2 : 1>;
     auto kern = delta_grads_kernel<DKP, IO>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES);
+    if (e != cudaSuccess) return e;
+    e = launch(delta_gates_kernel<IO>, dim3((unsigned)d.nch, (unsigned)d.Hv), dim3(128), 0, st, true, d);
     if (e != cudaSuccess) return e;
     return launch(kern, dim3((unsigned)d.nch, (unsigned)d.Hk), dim3(256), SM::BYTES, st, true, d);
 }

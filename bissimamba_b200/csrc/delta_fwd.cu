@@ -244,10 +244,11 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             unit_bar(grp);
             get_acc(exW, w * 2, lane, W);
             if (KEEP && on) {
-                uint32_t a[2][4];
+                uint32_t a[NPK][4];
                 frag_scale(W, up, dn);
-                frag_pieces<2>(W[0], W[1], up, a);
-                put_frag<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
+                frag_pieces<NPK>(W[0], W[1], up, a);
+                put_frag<NPK, 64>(d.Wh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+                put_acc((unsigned char*)(d.Wf + fb * 16 * C), w * 2, lane, W);
                 if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = dn;
             }
 #pragma unroll
@@ -278,9 +279,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                     O[t][e] *= d.scale;
                     if (t0 + i < len && cok[e >> 1]) stt(po + (long long)i * ldo, (e >> 1) * 8, O[t][e]);
                 }
-                if (KEEP && on)
-                    *((float4*)d.Of + (fb * (C / 8) + w * 2 + t) * 32 + lane) = make_float4(O[t][0], O[t][1], O[t][2], O[t][3]);
             }
+            if (KEEP && on) put_acc((unsigned char*)(d.Of + fb * 16 * C), w * 2, lane, O);
         }
     }
 }

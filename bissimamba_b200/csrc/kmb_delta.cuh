@@ -66,9 +66,9 @@ struct DeltaDesc {
     const int* order;            // packed: sequences, the longest first (NULL: as they are)
     // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
     // scaled by a power of two (mx)
-    __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [2][16 * C]
-    float* Of;                   // O, in accumulator order [C / 8 tiles][32 lanes][4]
-    __half *Gh, *Rh, *dSh;       // backward: dO [pieces][16 * C], dR = T^T dU [2][16 * C], adjoint of the state at the end
+    __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [pieces][16 * C]
+    __half *Gh, *Rh, *dSh;       // backward: dO, dR = T^T dU [pieces][16 * C], adjoint of the state at the end
+    float *Of, *Wf, *Rf;         // O, W and dR in accumulator order [C / 8 tiles][32 lanes][4]
     float* anchor;               // [nch][Hv][units][4 warps]: <S_0, dS_0> of their parts
     float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: what the tiles of S, W, dO, dR, dS are times
     // gradients
@@ -362,15 +362,15 @@ __device__ __forceinline__ void put_frag(__half* base, size_t piece, int lane, i
         for (int k = 0; k < NP; k++) *(uint32_t*)((char*)(base + k * piece) + o) = a[k][i];
     }
 }
-// entries (r, c) (r, c + 1) and (r + 8, ...) of an accumulator tile, both pieces as they are
-template <int W>
+// entries (r, c) (r, c + 1) and (r + 8, ...) of an accumulator tile, N pieces as they are
+template <int W, int N = 2>
 __device__ __forceinline__ void get_tile(const __half* base, size_t piece, int lane, int col, uint32_t (&v)[2][2]) {
     const int c = col + (lane & 3) * 2;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const uint32_t o = W == 64 ? tile_off<64>((lane >> 2) + 8 * h, c) : wide_off<16>((lane >> 2) + 8 * h, c);
 #pragma unroll
-        for (int k = 0; k < 2; k++) v[h][k] = *(const uint32_t*)((const char*)(base + k * piece) + o);
+        for (int k = 0; k < N; k++) v[h][k] = *(const uint32_t*)((const char*)(base + k * piece) + o);
     }
 }
 // x, y of a pair of pieces
