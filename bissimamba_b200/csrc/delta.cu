@@ -473,9 +473,39 @@ struct StepDesc {
     const int* slots;
 };
 
+// The lane's NR entries of a token's key or query
+template <typename IO, int NR>
+struct StepRow {
+    static constexpr int N4 = NR * (int)sizeof(IO) / 16;
+    uint4 w[N4];
+    __device__ __forceinline__ void load(const IO* p, int r0, int dk, bool vec) {
+        if (vec) {   // dk is a multiple of 16 bytes: whole pieces are inside or outside
+#pragma unroll
+            for (int i = 0; i < N4; i++)
+                w[i] = r0 + i * (16 / (int)sizeof(IO)) < dk ? *(const uint4*)(p + r0 + i * (16 / (int)sizeof(IO)))
+                                                            : make_uint4(0, 0, 0, 0);
+        } else {
+            IO e[NR];
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                if (r0 + i < dk) e[i] = p[r0 + i];
+                else stt(e, i, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < N4; i++) w[i] = ((const uint4*)e)[i];
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t* u = (const uint32_t*)w;
+        if constexpr (sizeof(IO) == 4) return __uint_as_float(u[i]);
+        else return __uint_as_float((i & 1) ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
+    }
+};
+
+// four blocks of four warps per SM: 128 registers, of which the state takes 64
 template <typename IO, int NR, bool VEC>
-__global__ void __launch_bounds__(128)
-delta_step_kernel(const __grid_constant__ StepDesc d) {
+__global__ void __launch_bounds__(128, NR == 16 ? 4 : 6)
+delta_step_kernel(const __grid_constant__ StepDesc d, int vec) {
     const int lane = threadIdx.x & 31;
     const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (id >= d.batch * d.Hv * d.units) return;
@@ -509,13 +539,10 @@ delta_step_kernel(const __grid_constant__ StepDesc d) {
         const long long tok = b * d.T + t;
         const float al = d.g ? expf(d.g[tok * d.Hv + hv]) : 1.0f;
         const float be = d.beta ? d.beta[tok * d.Hv + hv] : 1.0f;
-        float kr[NR], qr[NR], vc[4];
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const bool ok = r0 + i < d.dk;
-            kr[i] = ok ? ldt(k, tok * d.ld_k + (long long)hk * d.dk + r0 + i) : 0.0f;
-            qr[i] = ok ? ldt(q, tok * d.ld_q + (long long)hk * d.dk + r0 + i) : 0.0f;
-        }
+        StepRow<IO, NR> kr, qr;
+        float vc[4];
+        kr.load(k + tok * d.ld_k + (long long)hk * d.dk, r0, d.dk, vec);
+        qr.load(q + tok * d.ld_q + (long long)hk * d.dk, r0, d.dk, vec);
 #pragma unroll
         for (int e = 0; e < 4; e++)
             vc[e] = c0 + e < d.dv ? ldt(v, tok * d.ld_v + (long long)hv * d.dv + c0 + e) : 0.0f;
@@ -525,7 +552,7 @@ delta_step_kernel(const __grid_constant__ StepDesc d) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 S[i][e] *= al;
-                p[e] = fmaf(S[i][e], kr[i], p[e]);
+                p[e] = fmaf(S[i][e], kr.get(i), p[e]);
             }
 #pragma unroll
         for (int s = 4; s < 32; s <<= 1)
@@ -538,8 +565,8 @@ delta_step_kernel(const __grid_constant__ StepDesc d) {
         for (int i = 0; i < NR; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                S[i][e] = fmaf(kr[i], p[e], S[i][e]);
-                y[e] = fmaf(S[i][e], qr[i], y[e]);
+                S[i][e] = fmaf(kr.get(i), p[e], S[i][e]);
+                y[e] = fmaf(S[i][e], qr.get(i), y[e]);
             }
 #pragma unroll
         for (int s = 4; s < 32; s <<= 1)
@@ -568,12 +595,15 @@ cudaError_t step_go(const StepDesc& d, cudaStream_t st) {
     const long long warps = d.batch * d.Hv * d.units;
     const unsigned blocks = (unsigned)((warps + 3) / 4);
     const bool vec = d.dv % 4 == 0 && ((uintptr_t)d.pool & 15) == 0;
+    const int V = 16 / (int)sizeof(IO);
+    const int vkq = d.dk % V == 0 && d.ld_q % V == 0 && d.ld_k % V == 0 && ((uintptr_t)d.q & 15) == 0 &&
+                    ((uintptr_t)d.k & 15) == 0;
     if (d.dk <= 64) {
-        if (vec) delta_step_kernel<IO, 8, true><<<blocks, 128, 0, st>>>(d);
-        else delta_step_kernel<IO, 8, false><<<blocks, 128, 0, st>>>(d);
+        if (vec) delta_step_kernel<IO, 8, true><<<blocks, 128, 0, st>>>(d, vkq);
+        else delta_step_kernel<IO, 8, false><<<blocks, 128, 0, st>>>(d, vkq);
     } else {
-        if (vec) delta_step_kernel<IO, 16, true><<<blocks, 128, 0, st>>>(d);
-        else delta_step_kernel<IO, 16, false><<<blocks, 128, 0, st>>>(d);
+        if (vec) delta_step_kernel<IO, 16, true><<<blocks, 128, 0, st>>>(d, vkq);
+        else delta_step_kernel<IO, 16, false><<<blocks, 128, 0, st>>>(d, vkq);
     }
     return cudaGetLastError();
 }
