@@ -29,9 +29,7 @@ namespace {
 
 constexpr int LN_WARP_D = 512;    // longest row of the warp kernels
 constexpr int LN_BLOCK8_D = 8192; // longest row of blocks with 8 entries per thread
-#ifndef LN_BWD_BLOCKS
-#define LN_BWD_BLOCKS 2
-#endif
+constexpr int LN_BWD_BLOCKS = 2;   // blocks of the warp kernels per SM in the backward
 constexpr int LN_WARPS = 8;       // rows in flight per block there
 
 struct LnDesc {
@@ -243,20 +241,24 @@ ln_fwd_kernel(const LnDesc d) {
     }
 }
 
-// Backward.  Blocks walk rows with the grid's stride.  A row stays in registers as it is in memory (bf16: half
-// the registers), the normalised entries are computed twice; where registers allow it (PRE) the next row's loads
-// are in flight while this row is worked on (two row buffers in turn).
+// Backward.  Blocks walk rows with the grid's stride; the normalised entries are computed twice.  Where a warp's rows
+// are aligned (PRE) they come through a ring of shared memory filled by cp.async, two rows ahead (each lane reads
+// what it copied itself, so the warp never waits for another): keeping two rows in registers instead held 128
+// of them and took 135 us at 131072 x 512 bf16, against 115; three blocks per SM spill: 160.  Elsewhere a row stays in registers as it is in memory.
 template <typename T, int VEC, int NCH, bool BLOCK>
 struct LnBwd {
     static constexpr int E = NCH * VEC;
-    static constexpr bool PRE = !BLOCK && LN_BWD_BLOCKS == 2 && E * (int)sizeof(T) <= 32;
     static constexpr int MIN_BLOCKS = BLOCK ? 1 : LN_BWD_BLOCKS;
+    static constexpr int SLOT = NCH * 512;                        // bytes of one tensor's row (32 lanes x 16 x NCH)
+    static constexpr int DEPTH = SLOT <= 1024 ? 3 : 2;
+    static constexpr int RING = LN_WARPS * DEPTH * 3 * SLOT;
 };
 template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 32 * LN_WARPS, (LnBwd<T, VEC, NCH, BLOCK>::MIN_BLOCKS))
 ln_bwd_kernel(const LnDesc d) {
-    constexpr bool PRE = LnBwd<T, VEC, NCH, BLOCK>::PRE;
-    extern __shared__ float dynsh[];   // warp rows: [2][D] to add the warps in
+    using B = LnBwd<T, VEC, NCH, BLOCK>;
+    constexpr bool PRE = !BLOCK && !ODD && VEC > 1;
+    extern __shared__ __align__(16) float dynsh[];   // warp rows: [2][D] to add the warps in, over the ring
     __shared__ float sh[32];
     const int lane = BLOCK ? threadIdx.x : (threadIdx.x & 31);
     const int warp = threadIdx.x >> 5;
@@ -278,6 +280,7 @@ ln_bwd_kernel(const LnDesc d) {
         float mean, rstd;
     };
     const bool has_t = d.dtot != nullptr;
+    const float inv_d = 1.0f / (float)d.D;
     auto load = [&](long long row, Row& r) {
         const T* s = (const T*)d.x + row * d.ld_x;
         const T* dy = (const T*)d.dy + row * d.ld_dy;
@@ -292,7 +295,8 @@ ln_bwd_kernel(const LnDesc d) {
         r.mean = d.mean[row];
         r.rstd = d.rstd[row];
     };
-    auto work = [&](long long row, const Row& cur) {
+    // get(k, i): 16-byte pieces of s, dy, dtotal (k = 0, 1, 2)
+    auto work = [&](long long row, float mean, float rstd, auto get) {
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
@@ -300,10 +304,11 @@ ln_bwd_kernel(const LnDesc d) {
             if (col < d.D) {
                 float w[VEC];
                 if (d.w) ld_w<VEC, ODD>(d.w, col, d.D, w);
+                const Raw<T, VEC> rs = get(0, i), ry = get(1, i);
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float xh = (cur.s[i].get(j) - cur.mean) * cur.rstd;
-                    const float dy = cur.dy[i].get(j);   // 0 outside the row
+                    const float xh = (rs.get(j) - mean) * rstd;
+                    const float dy = ry.get(j);   // 0 outside the row
                     aw[i][j] = fmaf(dy, xh, aw[i][j]);
                     ab[i][j] += dy;
                     const float g = d.w ? __fmul_rn(dy, w[j]) : dy;
@@ -312,25 +317,26 @@ ln_bwd_kernel(const LnDesc d) {
                 }
             }
         }
-        s1 = row_sum<BLOCK>(s1, sh) / (float)d.D;
-        s2 = row_sum<BLOCK>(s2, sh) / (float)d.D;
+        s1 = row_sum<BLOCK>(s1, sh) * inv_d;
+        s2 = row_sum<BLOCK>(s2, sh) * inv_d;
         if (!d.dx) return;
         T* dx = (T*)d.dx + row * d.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
             const int col = at(i);
             if (col < d.D) {
-                float w[VEC];
+                float w[VEC], o8[VEC];
                 if (d.w) ld_w<VEC, ODD>(d.w, col, d.D, w);
-                float o8[VEC];
-                Raw<T, VEC> o;
+                const Raw<T, VEC> rs = get(0, i), ry = get(1, i);
+                Raw<T, VEC> rt, o;
+                if (has_t) rt = get(2, i);
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float xh = (cur.s[i].get(j) - cur.mean) * cur.rstd;
-                    const float dy = cur.dy[i].get(j);
+                    const float xh = (rs.get(j) - mean) * rstd;
+                    const float dy = ry.get(j);
                     // the product is rounded as in the sums: two columns (or one) cancel to what eps leaves
-                    o8[j] = cur.rstd * ((d.w ? __fmul_rn(dy, w[j]) : dy) - s1 - xh * s2);
-                    if (has_t) o8[j] += cur.t[i].get(j);
+                    o8[j] = rstd * ((d.w ? __fmul_rn(dy, w[j]) : dy) - s1 - xh * s2);
+                    if (has_t) o8[j] += rt.get(j);
                 }
                 o.set(o8);
                 st_cols<T, VEC, ODD>(dx, col, d.D, o);
@@ -338,21 +344,49 @@ ln_bwd_kernel(const LnDesc d) {
         }
     };
     if constexpr (PRE) {
-        // dx may be dy or dtotal: the next row belongs to these threads alone, nobody writes it before they read it
-        Row a, b;
-        if (first < d.rows) load(first, a);
-        for (long long row = first; row < d.rows; row += 2 * step) {
-            if (row + step < d.rows) load(row + step, b);
-            work(row, a);
-            if (row + step >= d.rows) break;
-            if (row + 2 * step < d.rows) load(row + 2 * step, a);
-            work(row + step, b);
+        // dx may be dy or dtotal: the rows ahead belong to this warp alone, nobody writes them before they are copied
+        unsigned char* ring = (unsigned char*)dynsh + warp * (B::DEPTH * 3 * B::SLOT) + lane * 16;
+        const uint32_t ra = (uint32_t)__cvta_generic_to_shared(ring);
+        const auto copy = [&](long long k) {
+            const long long row = first + k * step;
+            if (row < d.rows) {
+                const T* src[3] = {(const T*)d.x + row * d.ld_x, (const T*)d.dy + row * d.ld_dy,
+                                   (const T*)d.dtot + row * d.ld_dtot};
+                const uint32_t dst = ra + (uint32_t)(k % B::DEPTH) * (3 * B::SLOT);
+#pragma unroll
+                for (int i = 0; i < NCH; i++)
+                    if (at(i) < d.D) {
+#pragma unroll
+                        for (int t = 0; t < 3; t++)
+                            if (t < 2 || has_t)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                             ::"r"(dst + t * B::SLOT + i * 512), "l"(src[t] + at(i)) : "memory");
+                    }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int k = 0; k < B::DEPTH - 1; k++) copy(k);
+        float mS = 0.0f, rS = 0.0f;   // statistics of 32 rows, one per lane
+        long long k = 0;
+        for (long long row = first; row < d.rows; row += step, k++) {
+            copy(k + B::DEPTH - 1);
+            if ((k & 31) == 0) {
+                const long long mine = row + lane * step;
+                mS = mine < d.rows ? d.mean[mine] : 0.0f;
+                rS = mine < d.rows ? d.rstd[mine] : 0.0f;
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(B::DEPTH - 1) : "memory");
+            const unsigned char* slot = ring + (k % B::DEPTH) * (3 * B::SLOT);
+            work(row, __shfl_sync(0xffffffffu, mS, k & 31), __shfl_sync(0xffffffffu, rS, k & 31),
+                 [&](int t, int i) { return *(const Raw<T, VEC>*)(slot + t * B::SLOT + i * 512); });
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-        Row a;
         for (long long row = first; row < d.rows; row += step) {
+            Row a;
             load(row, a);
-            work(row, a);
+            work(row, a.mean, a.rstd, [&](int t, int i) { return t == 0 ? a.s[i] : t == 1 ? a.dy[i] : a.t[i]; });
         }
     }
     if (!d.part) return;
@@ -369,6 +403,7 @@ ln_bwd_kernel(const LnDesc d) {
                     }
             }
     } else {
+        __syncthreads();                       // the ring is read
         for (int k = 0; k < LN_WARPS; k++) {   // the warps add in order
             if (warp == k) {
 #pragma unroll
@@ -455,7 +490,7 @@ int bwd_blocks(long long rows, int span) {
     long long per_sm = LN_BWD_BLOCKS, want = (rows + LN_WARPS - 1) / LN_WARPS;
     if (span > LN_WARP_D) {
         per_sm = 1024 / block_threads(span);
-        per_sm = per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm;
+        per_sm = per_sm < 1 ? 1 : per_sm;
         want = rows;
     }
     const long long cap = (per_sm * sm_count() + 7) & ~7LL;
@@ -479,7 +514,14 @@ cudaError_t fwd_go(const LnDesc& d, cudaStream_t st) {
 }
 template <typename T, int VEC, int NCH, bool BLOCK, bool ODD>
 cudaError_t bwd_go(const LnDesc& d, cudaStream_t st) {
-    const size_t sm = BLOCK ? 0 : (size_t)2 * d.D * sizeof(float);
+    using B = LnBwd<T, VEC, NCH, BLOCK>;
+    const size_t ring = !BLOCK && !ODD && VEC > 1 ? B::RING : 0, add = (size_t)2 * d.D * sizeof(float);
+    const size_t sm = BLOCK ? 0 : ring > add ? ring : add;
+    if (sm > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(ln_bwd_kernel<T, VEC, NCH, BLOCK, ODD>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+        if (e != cudaSuccess) return e;
+    }
     const int threads = BLOCK ? block_threads(d.D + (ODD ? VEC - 1 : 0)) : 32 * LN_WARPS;
     ln_bwd_kernel<T, VEC, NCH, BLOCK, ODD><<<bwd_blocks(d.rows, d.D + (ODD ? VEC - 1 : 0)), threads, sm, st>>>(d);
     return cudaGetLastError();
