@@ -19,10 +19,14 @@ struct FwdSmem {
     using FX = FragBuf<C / 16, 2>;
     using FO = FragBuf<C / 16, NPO>;
     // of a unit: fragments of S, X, G_C. U and U, W as accumulators
-    static constexpr int oX = FS::BYTES, oU = oX + FX::BYTES, oO = oU + FX::BYTES, oW = oO + FO::BYTES, EX = oW + 4096;
-    // tiles are loaded two chunks ahead where three stages fit
-    static constexpr int stages(int nu) { return 3 * ST::BYTES + nu * EX + 128 <= 227 * 1024 ? 3 : 2; }
-    static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * EX; }
+    static constexpr int SW = FS::BYTES + 4096, XUO = 2 * FX::BYTES + FO::BYTES;
+    // Where three stages of tiles and two buffers of S and W fit, the side warps finish a chunk's outputs during the
+    // next chunk (LAG), and only one barrier a chunk holds the chain to them.  Else two stages, and the chain waits
+    // for them between its own steps.
+    static constexpr bool lag(int nu) { return 3 * ST::BYTES + nu * (2 * SW + XUO) + 128 <= 227 * 1024; }
+    static constexpr int stages(int nu) { return lag(nu) ? 3 : 2; }
+    static constexpr int ex(int nu) { return (lag(nu) ? 2 : 1) * SW + XUO; }
+    static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * ex(nu); }
 };
 
 template <int DKP, typename IO, bool KEEP, int NU>
@@ -38,12 +42,16 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int PK = C * DKP * 2;              // bytes of a K or Q piece
     extern __shared__ __align__(128) unsigned char sm[];
     constexpr int NS = SM::stages(NU);
+    constexpr bool LAG = SM::lag(NU);
     __shared__ __align__(8) uint64_t full[NS];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
     const bool chain = (warp & 4) == 0;
-    unsigned char* exS = sm + NS * ST::BYTES + grp * SM::EX;
-    unsigned char *exX = exS + SM::oX, *exU = exS + SM::oU, *exO = exS + SM::oO, *exW = exS + SM::oW;
+    unsigned char* ex = sm + NS * ST::BYTES + grp * SM::ex(NU);
+    unsigned char *exX = ex, *exU = exX + FX::BYTES, *exO = exU + FX::BYTES;
+    // buffers of step i
+    const auto bufS = [&](int i) { return exO + FO::BYTES + (LAG ? (i & 1) * SM::SW : 0); };
+    const auto bufW = [&](int i) { return bufS(i) + FS::BYTES; };
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
     const int hv = (int)(blockIdx.x / ub) % d.Hv, nr = (int)(blockIdx.x / ub) / d.Hv;
@@ -69,16 +77,17 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int i = 0; i < NS - 1 && i < nch; i++) fetch(i);
+        if (nch > 0) fetch(0);
     }
-    // The chunk's tiles are there, the state's fragments too, and the last chunk's stage is read; false: a wait ran out.
+    // The chunk's tiles are there, the state's fragments too, and the stage before the last (LAG; else the last) is
+    // read; false: a wait ran out.
     const auto begin = [&](int i) {
         const bool got = arrived(i);
         if (!__syncthreads_and(got)) {
             if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
             return false;
         }
-        if (threadIdx.x == 0 && i + NS - 1 < nch) fetch(i + NS - 1);
+        if (threadIdx.x == 0 && i + 1 < nch) fetch(i + 1);
         return true;
     };
 
@@ -104,7 +113,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                     V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
                 }
         };
-        const auto put_state = [&]() {
+        const auto put_state = [&](int i) {   // for step i
+            unsigned char* exS = bufS(i);
             float up, dn;
             frag_scale(S, up, dn);
 #pragma unroll
@@ -114,7 +124,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 FS::put(exS, w * KBW + b, lane, a, dn);
             }
         };
-        put_state();
+        put_state(0);
         __syncthreads();
         RT V[2][4], Vn[2][4];
         if (nch > 0) load_v(0, Vn);
@@ -128,6 +138,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             const uint32_t st = sb + stage(c) * ST::BYTES;
             const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
             const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
+            const unsigned char* exS = bufS(c);
             float X[2][4], part[2][4], dn, up;
             zero(X);
 #pragma unroll
@@ -167,7 +178,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
                 add_scaled(W, part, FX::scale(exX, kk) * fm);
             }
-            put_acc(exW, w * 2, lane, W);
+            put_acc(bufW(c), w * 2, lane, W);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -177,7 +188,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 }
             frag_scale(W, up, dn);
             FX::put(exU, w, lane, W, up, dn);
-            unit_bar(grp);
+            if (LAG) chain_bar(grp);
+            else unit_bar(grp);
             // S^T <- e^gamma_C S^T + (G_C. U)^T K
             const float last = tk[TOK_EG * C + C - 1];
 #pragma unroll
@@ -195,8 +207,9 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 });
                 add_scaled(S, ps, FX::scale(exU, kk));
             }
-            put_state();
+            put_state(c + 1);
         }
+        if (LAG) __syncthreads();   // the side warps' last chunk
         if (d.hT) {
 #pragma unroll
             for (int t = 0; t < KTW; t++)
@@ -209,13 +222,13 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     } else {
         // side warps: O^T = e^gamma S^T Q^T + U^T P^T, and what the backward reads
         __syncthreads();
-        for (int c = 0; c < nch; c++) {
-            if (!begin(c)) return;
+        float O[2][4];
+        const auto from_state = [&](int c) {   // the first term
+            const unsigned char* exS = bufS(c);
             const uint32_t st = sb + stage(c) * ST::BYTES;
-            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
-            const float* tw = tk + w * 16 + c2;
+            const float* tw = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok) + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
-            float O[2][4], W[2][4], part[2][4], dn, up;
+            float part[2][4];
             zero(O);
 #pragma unroll
             for (int s = 0; s < 4; s++) {
@@ -241,8 +254,14 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                     const int i = t * 8 + (e & 1);
                     O[t][e] *= tw[TOK_EG * C + i] * tw[TOK_FQ * C + i];
                 }
-            unit_bar(grp);
-            get_acc(exW, w * 2, lane, W);
+        };
+        const auto from_chunk = [&](int c) {   // the second, and out
+            const uint32_t st = sb + stage(c) * ST::BYTES;
+            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
+            const float* tw = tk + w * 16 + c2;
+            const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
+            float W[2][4], part[2][4], dn, up;
+            get_acc(bufW(c), w * 2, lane, W);
             if (KEEP && on) {
                 uint32_t a[NPK][4];
                 frag_scale(W, up, dn);
@@ -281,6 +300,21 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 }
             }
             if (KEEP && on) put_acc((unsigned char*)(d.Of + fb * 16 * C), w * 2, lane, O);
+        };
+        for (int c = 0; c < nch; c++) {
+            if (!begin(c)) return;
+            if (LAG && c > 0) {
+                from_chunk(c - 1);
+            }
+            from_state(c);
+            if (!LAG) {
+                unit_bar(grp);
+                from_chunk(c);
+            }
+        }
+        if (LAG) {
+            __syncthreads();
+            if (nch > 0) from_chunk(nch - 1);
         }
     }
 }
