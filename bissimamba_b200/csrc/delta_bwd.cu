@@ -43,7 +43,7 @@ struct BwdSmem {
 
 template <int DKP, typename IO, int NU>
 __global__ void __launch_bounds__(256 * NU, 1)
-delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
+delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     using SM = BwdSmem<DKP, IO>;
     constexpr int C = kDeltaC, NPK = SM::NPK;
     using ST = typename SM::ST;
@@ -76,15 +76,19 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
 
     const auto stage = [&](int i) { return i % NS; };
-    const auto fetch = [&](int i) {   // the tiles of the recurrence's step i
-        ST::load(d, d.Tt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + nch - 1 - i, hv);
+    // the chain warps of the first unit copy the tiles of the recurrence's step i (the side warps have more to do)
+    const bool copies = warp < 4 && lane == 0;
+    const auto fetch = [&](int i) {
+        ST::load(d, d.Tt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + nch - 1 - i, hv, w);
     };
     const auto arrived = [&](int i) { return mbar_wait(smem_u32(&full[stage(i)]), (i / NS) & 1); };
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int i = 0; i < NS - 1 && i < nch; i++) fetch(i);
     }
+    __syncthreads();
+    if (copies)
+        for (int i = 0; i < NS - 1 && i < nch; i++) fetch(i);
     // The chunk's tiles are there, the state's fragments too, and the last chunk's stage is read; false: a wait ran out.
     const auto begin = [&](int i) {
         const bool got = arrived(i);
@@ -92,7 +96,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
             if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
             return false;
         }
-        if (threadIdx.x == 0 && i + NS - 1 < nch) fetch(i + NS - 1);
+        if (copies && i + NS - 1 < nch) fetch(i + NS - 1);
         return true;
     };
 
@@ -205,32 +209,21 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
     }
 
     // side warps
-    using RT = typename RawOf<IO>::type;
-    const int ldg = (int)d.ld_do;
-    const auto load_t = [&](const void* base, long long ld, int ldi, int c, RT (&V)[2][4]) {
+    TokenTile<IO> Gn;
+    const auto load_go = [&](int c) {
         const long long t0 = (long long)c * C + w * 16;
-        const RT* p = (const RT*)base + (start + t0) * ld + (long long)hv * d.dv + col[0];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = t * 8 + c2 + (e & 1);
-                V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldi + (e >> 1) * 8] : RT(0);
-            }
+        Gn.load(d.go, start + t0, d.ld_do, (long long)hv * d.dv + u * 16, on ? d.dv - u * 16 : 0,
+                (int)(len - t0 < 16 ? len - t0 : 16), lane, vec);
     };
     const auto unit_at = [&](int c) { return ((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u; };
     float G[2][4], part[2][4], up, dn;   // dO^T of the warp's tokens
-    RT Gn[2][4];
     // ahead of chunk c (tile stage `s`): dO's fragments, plain and with the factors of the state's product; P^T dO
     const auto ahead = [&](int c, int s) {
         const uint32_t st = sb + s * ST::BYTES;
         const float* tk = (const float*)(sm + s * ST::BYTES + ST::oTok);
         const float* tw = tk + w * 16 + c2;
         uint32_t a[NPK][4];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) G[t][e] = from_raw(Gn[t][e]);
+        Gn.tiles(G, exR + w * 1024, lane, vec);   // the place of the dR that this warp has read
         frag_scale(G, up, dn);
         frag_pieces<NPK>(G[0], G[1], up, a);
         FG::put(exX, w, lane, a, dn);
@@ -284,7 +277,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         // magnitudes are up to 2^30 and more per product: the scales are applied one after the other
         if (on && lane == 0) d.anchor[unit_at(c) * 4 + w] = an * fs * FS::scale(exS, w * KBW);
     };
-    if (nch > 0) load_t(d.go, d.ld_do, ldg, nch - 1, Gn);
+    if (nch > 0) load_go(nch - 1);
     __syncthreads();
     if (nch > 0) {
         if (!arrived(0)) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
@@ -296,7 +289,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d) {
         const uint32_t st = sb + stage(it) * ST::BYTES;
         const size_t fb = unit_at(c);
         float* mx = d.mx + (fb * 4 + w) * MX_ROWS;
-        if (c > 0) load_t(d.go, d.ld_do, ldg, c - 1, Gn);   // in flight under the products
+        if (c > 0) load_go(c - 1);   // in flight under the products
         // keep dS_C; its product with the state at the same place
         if (it > 0) anchor(c + 1);
 #pragma unroll
@@ -741,7 +734,8 @@ cudaError_t chain_go(const DeltaDesc& d, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
-    kern<<<(unsigned)blocks, 256 * NU, SMEM, st>>>(d);
+    const int vec = sizeof(IO) == 2 && d.dv % 8 == 0 && d.ld_do % 8 == 0 && ((uintptr_t)d.go & 15) == 0;
+    kern<<<(unsigned)blocks, 256 * NU, SMEM, st>>>(d, vec);
     return cudaGetLastError();
 }
 template <int DKP, typename IO>

@@ -23,7 +23,7 @@ struct FwdSmem {
     // Where three stages of tiles and two buffers of S and W fit, the side warps finish a chunk's outputs during the
     // next chunk (LAG), and only one barrier a chunk holds the chain to them.  Else two stages, and the chain waits
     // for them between its own steps.
-    static constexpr bool lag(int nu) { return 3 * ST::BYTES + nu * (2 * SW + XUO) + 128 <= 227 * 1024; }
+    static constexpr bool lag(int nu) { return 3 * ST::BYTES + nu * (2 * SW + XUO) + nu * 2048 + 128 <= 227 * 1024; }
     static constexpr int stages(int nu) { return lag(nu) ? 3 : 2; }
     static constexpr int ex(int nu) { return (lag(nu) ? 2 : 1) * SW + XUO; }
     static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * ex(nu); }
@@ -31,7 +31,7 @@ struct FwdSmem {
 
 template <int DKP, typename IO, bool KEEP, int NU>
 __global__ void __launch_bounds__(256 * NU, 1)
-delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
+delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     using SM = FwdSmem<DKP, IO, KEEP>;
     constexpr int C = kDeltaC, NPK = SM::NPK, NPO = SM::NPO;
     using ST = typename SM::ST;
@@ -44,6 +44,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int NS = SM::stages(NU);
     constexpr bool LAG = SM::lag(NU);
     __shared__ __align__(8) uint64_t full[NS];
+    __shared__ int dead;
+    __shared__ __align__(16) unsigned char vbuf[NU * 4][512];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
     const bool chain = (warp & 4) == 0;
@@ -69,25 +71,37 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
     const int nch = (int)((len + C - 1) / C);
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
 
-    const auto stage = [&](int i) { return i % NS; };
-    const auto fetch = [&](int i) {   // the tiles of the recurrence's step i
-        ST::load(d, d.Mt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + i, hv);
+    // the side warps of the first unit copy the tiles of the recurrence's step i into stage s
+    const bool copies = warp >= 4 && warp < 8 && lane == 0;
+    const auto fetch = [&](int i, int s) {
+        ST::load(d, d.Mt, sb + s * ST::BYTES, smem_u32(&full[s]), chunk0 + i, hv, w);
     };
-    const auto arrived = [&](int i) { return mbar_wait(smem_u32(&full[stage(i)]), (i / NS) & 1); };
     if (threadIdx.x == 0) {
+        dead = 0;
         for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (nch > 0) fetch(0);
     }
+    __syncthreads();
+    if (copies && nch > 0) fetch(0, 0);
     // The chunk's tiles are there, the state's fragments too, and the stage before the last (LAG; else the last) is
     // read; false: a wait ran out.
+    int slot = 0, phase = 0, last_slot = 0;   // of the step's tiles, of the last step's
     const auto begin = [&](int i) {
-        const bool got = arrived(i);
-        if (!__syncthreads_and(got)) {
-            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
-            return false;
+        if (i > 0) {
+            last_slot = slot;
+            if (++slot == NS) {
+                slot = 0;
+                phase ^= 1;
+            }
         }
-        if (threadIdx.x == 0 && i + 1 < nch) fetch(i + 1);
+        // (the side warps wait for the copies; the barrier passes on what they saw)
+        if (!chain && !mbar_wait(smem_u32(&full[slot]), phase)) {
+            set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            dead = 1;
+        }
+        __syncthreads();
+        if (dead) return false;
+        if (copies && i + 1 < nch) fetch(i + 1, slot + 1 == NS ? 0 : slot + 1);
         return true;
     };
 
@@ -100,18 +114,11 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                 const int i = (w * KTW + t) * 8 + c2 + (e & 1);
                 S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
             }
-        // v of the warp's tokens of chunk c, as accumulator tiles [16 columns][16 tokens]
-        using RT = typename RawOf<IO>::type;
-        const auto load_v = [&](int c, RT (&V)[2][4]) {
+        TokenTile<IO> Vn;   // v of the warp's tokens of the next chunk
+        const auto load_v = [&](int c) {
             const long long t0 = (long long)c * C + w * 16;
-            const RT* p = (const RT*)d.v + (start + t0) * d.ld_v + (long long)hv * d.dv + col[0];
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = t * 8 + c2 + (e & 1);
-                    V[t][e] = (t0 + i < len && cok[e >> 1]) ? p[(long long)i * ldv + (e >> 1) * 8] : RT(0);
-                }
+            Vn.load(d.v, start + t0, ldv, (long long)hv * d.dv + u * 16, on ? d.dv - u * 16 : 0,
+                    (int)(len - t0 < 16 ? len - t0 : 16), lane, vec);
         };
         const auto put_state = [&](int i) {   // for step i
             unsigned char* exS = bufS(i);
@@ -126,40 +133,34 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         };
         put_state(0);
         __syncthreads();
-        RT V[2][4], Vn[2][4];
-        if (nch > 0) load_v(0, Vn);
+        float V[2][4];
+        if (nch > 0) load_v(0);
         for (int c = 0; c < nch; c++) {
             if (!begin(c)) return;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) V[t][e] = Vn[t][e];
-            if (c + 1 < nch) load_v(c + 1, Vn);
-            const uint32_t st = sb + stage(c) * ST::BYTES;
-            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
+            Vn.tiles(V, vbuf[grp * 4 + w], lane, vec);
+            if (c + 1 < nch) load_v(c + 1);
+            const uint32_t st = sb + slot * ST::BYTES;
+            const float* tk = (const float*)(sm + slot * ST::BYTES + ST::oTok);
             const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
             const unsigned char* exS = bufS(c);
-            float X[2][4], part[2][4], dn, up;
+            float X[2][4], part[4][2][4], dn, up;
             zero(X);
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                zero(part);
+            for (int k0 = 0; k0 < DKP / 16; k0 += 4) {
+                mma_blocks<4, 2, NPK, 2>(
+                    part, [&](int k, uint32_t (&a)[2][4]) { FS::template get<2>(exS, k0 + k, lane, a); },
+                    [&](int k, int p, int, uint32_t (&f)[4]) {
+                        ldm4(f, st + p * PK + wide_off<C>(w * 16 + lb_row(lane), (k0 + k) * 16 + lb_col(lane)));
+                    });
 #pragma unroll
-                for (int b = 0; b < KBW; b++) {
-                    const int kk = s * KBW + b;
-                    uint32_t a[2][4];
-                    FS::template get<2>(exS, kk, lane, a);
-                    const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-                    mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * PK + o); });
-                }
-                add_scaled(X, part, FS::scale(exS, s * KBW));
+                for (int k = 0; k < 4; k++) add_scaled(X, part[k], FS::scale(exS, k0 + k));
             }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int i = t * 8 + (e & 1);
-                    X[t][e] = from_raw(V[t][e]) - tw[TOK_EG * C + i] * tw[TOK_FK * C + i] * X[t][e];
+                    X[t][e] = V[t][e] - tw[TOK_EG * C + i] * tw[TOK_FK * C + i] * X[t][e];
                 }
             frag_scale(X, up, dn);
             FX::put(exX, w, lane, X, up, dn);
@@ -168,16 +169,13 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             float W[2][4];
             zero(W);
             const float fm = tk[TOK_MISC * C + w];
+            mma_blocks<4, 2, 2, 2>(
+                part, [&](int k, uint32_t (&a)[2][4]) { FX::template get<2>(exX, k, lane, a); },
+                [&](int k, int p, int, uint32_t (&f)[4]) {
+                    ldm4(f, st + ST::oT + p * ST::TT + tile_off<C>(w * 16 + lb_row(lane), k * 16 + lb_col(lane)));
+                });
 #pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                if (kk > w) continue;
-                uint32_t a[2][4];
-                FX::template get<2>(exX, kk, lane, a);
-                const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-                zero(part);
-                mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oT + p * ST::TT + o); });
-                add_scaled(W, part, FX::scale(exX, kk) * fm);
-            }
+            for (int k = 0; k < 4; k++) add_masked(W, part[k], FX::scale(exX, k) * fm, k <= w ? ~0u : 0u);
             put_acc(bufW(c), w * 2, lane, W);
 #pragma unroll
             for (int t = 0; t < 2; t++)
@@ -196,16 +194,17 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             for (int t = 0; t < KTW; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) S[t][e] *= last;
+            constexpr int KB = KTW == 2 || NU == 1 ? 4 : 2;   // blocks at a time: what registers allow
 #pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[2][4];
-                float ps[KTW][4];
-                FX::template get<2>(exU, kk, lane, a);
-                zero(ps);
-                mma_row<2, NPK>(ps, a, 0, KTW / 2, [&](int p, int t2, uint32_t (&f)[4]) {
-                    ldm4t(f, st + p * PK + wide_off<C>(kk * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
-                });
-                add_scaled(S, ps, FX::scale(exU, kk));
+            for (int k0 = 0; k0 < C / 16; k0 += KB) {
+                float ps[KB][KTW][4];
+                mma_blocks<KB, 2, NPK, KTW>(
+                    ps, [&](int k, uint32_t (&a)[2][4]) { FX::template get<2>(exU, k0 + k, lane, a); },
+                    [&](int k, int p, int t2, uint32_t (&f)[4]) {
+                        ldm4t(f, st + p * PK + wide_off<C>((k0 + k) * 16 + la_row(lane), (w * KTW + t2 * 2) * 8 + la_col(lane)));
+                    });
+#pragma unroll
+                for (int k = 0; k < KB; k++) add_scaled(S, ps[k], FX::scale(exU, k0 + k));
             }
             put_state(c + 1);
         }
@@ -225,8 +224,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         float O[2][4];
         const auto from_state = [&](int c) {   // the first term
             const unsigned char* exS = bufS(c);
-            const uint32_t st = sb + stage(c) * ST::BYTES;
-            const float* tw = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok) + w * 16 + c2;
+            const uint32_t st = sb + slot * ST::BYTES;
+            const float* tw = (const float*)(sm + slot * ST::BYTES + ST::oTok) + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
             float part[2][4];
             zero(O);
@@ -255,9 +254,9 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
                     O[t][e] *= tw[TOK_EG * C + i] * tw[TOK_FQ * C + i];
                 }
         };
-        const auto from_chunk = [&](int c) {   // the second, and out
-            const uint32_t st = sb + stage(c) * ST::BYTES;
-            const float* tk = (const float*)(sm + stage(c) * ST::BYTES + ST::oTok);
+        const auto from_chunk = [&](int c, int s) {   // the second (tiles in stage s), and out
+            const uint32_t st = sb + s * ST::BYTES;
+            const float* tk = (const float*)(sm + s * ST::BYTES + ST::oTok);
             const float* tw = tk + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
             float W[2][4], part[2][4], dn, up;
@@ -280,13 +279,12 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
             const float fp = tk[TOK_MISC * C + 4 + w];
 #pragma unroll
             for (int kk = 0; kk < C / 16; kk++) {
-                if (kk > w) continue;
                 uint32_t a[NPO][4];
                 FO::template get<NPO>(exO, kk, lane, a);
                 const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                 zero(part);
                 mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });
-                add_scaled(O, part, FO::scale(exO, kk) * fp);
+                add_masked(O, part, FO::scale(exO, kk) * fp, kk <= w ? ~0u : 0u);
             }
             const long long t0 = (long long)c * C + w * 16;
             IO* po = (IO*)d.o + (start + t0) * d.ld_o + (long long)hv * d.dv + col[0];
@@ -304,17 +302,17 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d) {
         for (int c = 0; c < nch; c++) {
             if (!begin(c)) return;
             if (LAG && c > 0) {
-                from_chunk(c - 1);
+                from_chunk(c - 1, last_slot);
             }
             from_state(c);
             if (!LAG) {
                 unit_bar(grp);
-                from_chunk(c);
+                from_chunk(c, slot);
             }
         }
         if (LAG) {
             __syncthreads();
-            if (nch > 0) from_chunk(nch - 1);
+            if (nch > 0) from_chunk(nch - 1, slot);
         }
     }
 }
@@ -326,7 +324,8 @@ cudaError_t go(const DeltaDesc& d, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)d.nseq * d.Hv * ((d.units + NU - 1) / NU);
-    return launch(kern, dim3((unsigned)blocks), dim3(256 * NU), SMEM, st, d.nch > 0, d);
+    const int vec = sizeof(IO) == 2 && d.dv % 8 == 0 && d.ld_v % 8 == 0 && ((uintptr_t)d.v & 15) == 0;
+    return launch(kern, dim3((unsigned)blocks), dim3(256 * NU), SMEM, st, d.nch > 0, d, vec);
 }
 template <int DKP, typename IO>
 cudaError_t pick(const DeltaDesc& d, bool keep, cudaStream_t st) {

@@ -277,6 +277,44 @@ __device__ __forceinline__ void decay_tables(const DecaySmem& s, int tid) {   //
     }
 }
 
+// part[k] = A_k B_k for NK blocks of 16 of the sum, N tiles wide: all fragments are loaded before the first product and
+// the products of different blocks alternate, so that neither waits for the other.  load_a(k, a), load_b(k, piece,
+// t2, b).
+template <int NK, int NA, int NB, int N, typename LA, typename LB>
+__device__ __forceinline__ void mma_blocks(float (&part)[NK][N][4], LA load_a, LB load_b) {
+    constexpr int LIM = NA == 1 && NB == 1 ? 0 : 1;
+    uint32_t a[NK][NA][4], b[NK][NB][N / 2][4];
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        load_a(k, a[k]);
+#pragma unroll
+        for (int p = 0; p < NB; p++)
+#pragma unroll
+            for (int t = 0; t < N / 2; t++) load_b(k, p, t, b[k][p][t]);
+    }
+#pragma unroll
+    for (int k = 0; k < NK; k++)
+#pragma unroll
+        for (int t = 0; t < N; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[k][t][e] = 0.0f;
+#pragma unroll
+    for (int sum = LIM; sum >= 0; sum--)
+#pragma unroll
+        for (int pb = 0; pb < NB; pb++)
+#pragma unroll
+            for (int pa = 0; pa < NA; pa++)
+                if (pa + pb == sum) {
+#pragma unroll
+                    for (int k = 0; k < NK; k++)
+#pragma unroll
+                        for (int t = 0; t < N / 2; t++) {
+                            mma(part[k][2 * t], a[k][pa], b[k][pb][t][0], b[k][pb][t][1]);
+                            mma(part[k][2 * t + 1], a[k][pa], b[k][pb][t][2], b[k][pb][t][3]);
+                        }
+                }
+}
+
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -303,17 +341,23 @@ struct DeltaStage {
     static constexpr int TOK = TOK_SIZE * 4;
     static constexpr int BYTES = oTok + TOK;
 
-    // one thread: bulk copies of one chunk into the stage at `dst`, M or T from `tiles`
+    // Bulk copies of one chunk into the stage at `dst`, M or T from `tiles`, by four threads (part 0 .. 3): issuing
+    // all of them takes a warp some 500 cycles.  A copy may complete before part 0 has announced the bytes.
     static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t dst, uint32_t bar,
-                                                int chunk, int hv) {
+                                                int chunk, int hv, int part) {
         const int hk = hv / d.grp;
         const size_t kh = ((size_t)chunk * d.Hk + hk) * NPK * C * DKP, vh = (size_t)chunk * d.Hv + hv;
-        mbar_expect_tx(bar, BYTES);
-        bulk(dst, d.Kt + kh, KQ, bar);
-        bulk(dst + oQ, d.Qt + kh, KQ, bar);
-        bulk(dst + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
-        bulk(dst + oP, d.Pt + vh * 2 * C * C, NPP * TT, bar);
-        bulk(dst + oTok, d.tok + vh * TOK_SIZE, TOK, bar);
+        if (part == 0) {
+            mbar_expect_tx(bar, BYTES);
+            bulk(dst + oTok, d.tok + vh * TOK_SIZE, TOK, bar);
+            bulk(dst + oP, d.Pt + vh * 2 * C * C, NPP * TT, bar);
+        } else if (part == 1) {
+            bulk(dst, d.Kt + kh, KQ, bar);
+        } else if (part == 2) {
+            bulk(dst + oQ, d.Qt + kh, KQ, bar);
+        } else {
+            bulk(dst + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
+        }
     }
     static __device__ __forceinline__ void bulk(uint32_t dst, const void* src, unsigned bytes, uint32_t bar) {
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -394,10 +438,68 @@ __device__ __forceinline__ void add_scaled(float (&acc)[N][4], const float (&par
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[i][e] = fmaf(part[i][e], f, acc[i][e]);
 }
+// acc += f part if `on` (0 or ~0).  The triangular products run over all blocks without a branch, so that they overlap;
+// those outside the triangle, whose factors hold anything, are masked out here.
+template <int N>
+__device__ __forceinline__ void add_masked(float (&acc)[N][4], const float (&part)[N][4], float f, uint32_t on) {
+    f = __uint_as_float(__float_as_uint(f) & on);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            acc[i][e] = fmaf(__uint_as_float(__float_as_uint(part[i][e]) & on), f, acc[i][e]);
+}
 // barriers of unit g: its chain warps, its side warps, all of them
 __device__ __forceinline__ void chain_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 1) : "memory"); }
 __device__ __forceinline__ void side_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 2) : "memory"); }
 __device__ __forceinline__ void unit_bar(int g) { asm volatile("bar.sync %0, 256;" ::"r"(3 * g + 3) : "memory"); }
+// A warp's 16 tokens x 16 columns of v or dO as accumulator tiles [16 columns][2 x 8 tokens].  bf16 rows on 16-byte
+// boundaries (vec): one 16-byte load per lane, held as it is until the tiles are needed, then transposed by ldmatrix
+// through 512 bytes of the warp's own; else entry by entry.
+template <typename IO>
+struct TokenTile {
+    using RT = typename RawOf<IO>::type;
+    uint4 w;
+    RT e[2][4];
+    __device__ __forceinline__ void load(const void* base, long long tok, long long ld, long long at, int cols, int n,
+                                         int lane, bool vec) {
+        if (sizeof(IO) == 2 && vec) {
+            const int t = lane >> 1, c = (lane & 1) * 8;
+            w = t < n && c < cols ? *(const uint4*)((const RT*)base + (tok + t) * ld + at + c) : make_uint4(0, 0, 0, 0);
+            return;
+        }
+        const int r = lane >> 2, c2 = (lane & 3) * 2;
+        const RT* p = (const RT*)base + tok * ld + at + r;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = t * 8 + c2 + (k & 1);
+                e[t][k] = i < n && r + (k >> 1) * 8 < cols ? p[(long long)i * ld + (k >> 1) * 8] : RT(0);
+            }
+    }
+    __device__ __forceinline__ void tiles(float (&x)[2][4], unsigned char* scratch, int lane, bool vec) const {
+        if (sizeof(IO) == 2 && vec) {
+            *(uint4*)(scratch + lane * 16) = w;   // [token][16 columns]
+            __syncwarp();
+            uint32_t f[4];   // columns 0-7, 8-15 of tokens 0-7, then of 8-15
+            ldm4t(f, (uint32_t)__cvta_generic_to_shared(scratch) + ((lane & 7) + (lane >> 4) * 8) * 32 + ((lane >> 3) & 1) * 16);
+            __syncwarp();
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    x[t][h * 2] = __uint_as_float(f[t * 2 + h] << 16);
+                    x[t][h * 2 + 1] = __uint_as_float(f[t * 2 + h] & 0xffff0000u);
+                }
+            return;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[t][k] = from_raw(e[t][k]);
+    }
+};
 // accumulator tiles through shared memory, [tile][lane] 16 bytes
 template <int N>
 __device__ __forceinline__ void put_acc(unsigned char* base, int tile, int lane, const float (&t)[N][4]) {
