@@ -680,7 +680,8 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
         const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
         d.Tt = (__half*)take(cv * 2 * C * C * 2);
         d.gam = (double*)take(cv * C * 8);
-        d.Sh = (__half*)take(u * 2 * DKP);
+        d.Sh = (__half*)take(u * NPK * DKP);
+        d.Sf = (float*)take(u * 2 * DKP);
         d.Wh = (__half*)take(u * NPK * C);
         d.Of = (float*)take(u * 2 * C);
         d.Wf = (float*)take(u * 2 * C);

@@ -256,8 +256,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         }
         put_acc(exR, w * 2, lane, Y);
     };
-    uint32_t sr[KBW][2][2][2];   // the warp's part of the state at the start of the last chunk done
-    float fs = 0.0f;
+    float sr[KTW][4];   // the warp's part of the state at the start of the last chunk done
+    zero(sr);
     // <S_0, dS_0> at the start of chunk c, from the fragments that the chain left
     const auto anchor = [&](int c) {
         float an = 0.0f;
@@ -267,15 +267,15 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             FS::template get<2>(exS, w * KBW + b, lane, a);
 #pragma unroll
             for (int i = 0; i < 4; i++) {   // fragment word i: row half i & 1, tile i >> 1
-                const float2 x = join(a[0][i], a[1][i]), y = join(sr[b][i >> 1][i & 1][0], sr[b][i >> 1][i & 1][1]);
-                an = fmaf(x.x, y.x, an);
-                an = fmaf(x.y, y.y, an);
+                const float2 x = join(a[0][i], a[1][i]);
+                const float (&y)[4] = sr[2 * b + (i >> 1)];
+                an = fmaf(x.x, y[(i & 1) * 2], an);
+                an = fmaf(x.y, y[(i & 1) * 2 + 1], an);
             }
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) an += __shfl_xor_sync(0xffffffffu, an, o);
-        // magnitudes are up to 2^30 and more per product: the scales are applied one after the other
-        if (on && lane == 0) d.anchor[unit_at(c) * 4 + w] = an * fs * FS::scale(exS, w * KBW);
+        if (on && lane == 0) d.anchor[unit_at(c) * 4 + w] = an * FS::scale(exS, w * KBW);
     };
     if (nch > 0) load_go(nch - 1);
     __syncthreads();
@@ -299,12 +299,9 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             if (on) {
                 put_frag<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
                 if (lane == 0) mx[MX_DS] = FS::scale(exS, w * KBW);
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    get_tile<DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, ((w * KBW + b) * 2 + t) * 8, sr[b][t]);
-                fs = mx[MX_S];
             }
         }
+        if (on) get_acc((const unsigned char*)(d.Sf + fb * 16 * DKP), w * KTW, lane, sr);
         // (scale e^gamma dO)^T Q
         {
             float Z[KTW][4], ps[KTW][4];
@@ -524,10 +521,9 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             for (int i = tid; i < nx * NP * SM::NH * 128; i += 256) {
                 const int x = i / (NP * SM::NH * 128), p = i / (SM::NH * 128) % NP, h = i / 128 % SM::NH, o = (i & 127) * 16;
                 const size_t g = (((head * d.units + u0 + x) * NP + p) * SM::NH + h) * 2048 + o;
-                const size_t gs = (((head * d.units + u0 + x) * 2 + p) * SM::NH + h) * 2048 + o;
                 const uint32_t s = sb + p * SM::SD + h * 8192 + x * 2048 + o;
                 cp16(s + SM::oD, (const char*)d.dSh + g);
-                cp16(s + SM::oS, (const char*)d.Sh + gs);
+                cp16(s + SM::oS, (const char*)d.Sh + g);
             }
             cp_commit();
         };

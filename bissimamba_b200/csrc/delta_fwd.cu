@@ -122,6 +122,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         };
         const auto put_state = [&](int i) {   // for step i
             unsigned char* exS = bufS(i);
+            if (KEEP && on && i < nch)
+                put_acc((unsigned char*)(d.Sf + (((size_t)(chunk0 + i) * d.Hv + hv) * d.units + u) * 16 * DKP), w * KTW, lane, S);
             float up, dn;
             frag_scale(S, up, dn);
 #pragma unroll
@@ -238,7 +240,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     const int kk = s * KBW + b;
                     uint32_t a[2][4];
                     FS::template get<2>(exS, kk, lane, a);
-                    if (KEEP && on && s == w) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, kk * 16, a);
+                    if (KEEP && on && s == w) put_frag<NPK, DKP>(d.Sh + fb * NPK * 16 * DKP, 16 * DKP, lane, kk * 16, a);
                     const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                     mma_row<NPO, NPK>(part, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
                                       [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });

@@ -66,9 +66,9 @@ struct DeltaDesc {
     const int* order;            // packed: sequences, the longest first (NULL: as they are)
     // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
     // scaled by a power of two (mx)
-    __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [pieces][16 * C]
+    __half *Sh, *Wh;             // state at the chunk's start [pieces][16 * DKP], W [pieces][16 * C]
     __half *Gh, *Rh, *dSh;       // backward: dO, dR = T^T dU [pieces][16 * C], adjoint of the state at the end
-    float *Of, *Wf, *Rf;         // O, W and dR in accumulator order [C / 8 tiles][32 lanes][4]
+    float *Sf, *Of, *Wf, *Rf;    // state, O, W and dR in accumulator order [tiles][32 lanes][4]
     float* anchor;               // [nch][Hv][units][4 warps]: <S_0, dS_0> of their parts
     float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: what the tiles of S, W, dO, dR, dS are times
     // gradients
@@ -128,11 +128,12 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[NP]) 
     }
 }
 // Power of two that takes m (the largest magnitude of a row) into [2^14, 2^15), and its inverse.  Rows below
-// 2^-112 (zero rows among them) take the factors of 2^-112; an infinite or NaN entry stays one.
+// 2^-112 (zero rows among them) take the factors of 2^-112.  Beside an infinity nothing finite would be left, so it
+// makes the row NaN; a NaN entry stays one.
 __device__ __forceinline__ void row_scale(float m, float& up, float& down) {
     int e = (int)(__float_as_uint(m) >> 23);
     e = e < 15 ? 15 : e;
-    up = __uint_as_float((uint32_t)(268 - e) << 23);
+    up = __uint_as_float(e == 255 ? 0x7fffffffu : (uint32_t)(268 - e) << 23);
     down = __uint_as_float((uint32_t)(e - 14) << 23);
 }
 // of all entries of the warp's accumulator tiles: one warp-wide maximum (of the bits: magnitudes order as integers)
