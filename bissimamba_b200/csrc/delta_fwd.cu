@@ -2,7 +2,14 @@
 // (kmb_delta.cuh: a unit of 16 columns of dv, four warps):
 //   X = V - e^gamma K S;  W = M X;  U = beta W;  O = scale (e^gamma Q S + P U);  S <- e^gamma_C S + K^T (G_C. U)
 // all transposed.  The chain of a chunk is latency: three products that each wait
-// for the last, with fp16 pieces made and passed on between them.
+// for the last, with fp16 pieces made and passed on between them.  Where the
+// cycles of a chunk of dk = 128 go (3400 of them): the barrier and the tiles'
+// arrival 200, v 280, the three products 700 + 570 + 500, making pieces and row
+// scales 750.  So all fragments of a product are loaded before its first
+// instruction, blocks alternate in the tensor cores, and what is not the chain is
+// the side warps'.
+// Measured (16384 tokens, 16 heads of 128, bf16): 440 us, 1.7 us a chunk; one warp
+// for all of dk took 6.5 us, four warps with everything in them 2.1 us.
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 

@@ -15,10 +15,19 @@
  * Offsets outside [0, T] are clamped to it and tokens that no sequence holds are
  * neither read nor written.
  *
- * Calls only enqueue work on `stream` (NULL = default), allocate nothing, keep
- * nothing between calls, and give the same bits every time.  0 on success, -1
- * with kmb_last_error() set otherwise; a bounded wait that runs out is recorded
- * in the device status word (kmb_device_status). */
+ * Accuracy: bf16 inputs are exact, every product is good to 2^-22 and every sum
+ * fp32; bf16 results are rounded once.  Factors are scaled by blocks of 16 tokens
+ * (or a quarter of dk) times 16 columns of dv: an entry below 2^-40 of its block's
+ * largest counts as zero, and an infinity makes its block NaN.  A NaN at a token
+ * reaches the tokens of its block of 16 before it as well as all behind.  Scale
+ * keys so that beta |k|^2 <= 2 and g <= 0, as the rule itself needs to stay
+ * bounded.
+ *
+ * Calls only enqueue work on `stream` (NULL = default), allocate nothing (but for
+ * the device status word in a host thread's first call), keep nothing between
+ * calls, and give the same bits every time.  0 on success, -1 with
+ * kmb_last_error() set otherwise; a bounded wait that runs out is recorded in the
+ * device status word (kmb_device_status). */
 #ifndef KMB200_DELTA_H
 #define KMB200_DELTA_H
 #include <stddef.h>

@@ -180,6 +180,26 @@ def test_hard_values(kmb, cuda, kind, dtype):
     _compare(_run(kmb, cuda, x), _reference(x), dtype)
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_that_are_not_finite(kmb, cuda, dtype, bad):
+    """One at token 70, column 3 of v: the blocks of 16 tokens before it, the other 16-column units and the other head
+    keep their bits, and in its unit nothing finite is wrong."""
+    x = _inputs(1, 140, 2, 2, 64, 48, dtype, seed=13)
+    clean = _run(kmb, cuda, x, backward=False)
+    ref_o = _reference(x, backward=False)["o"]
+    x["v"][0, 70, 0, 3] = bad
+    got = _run(kmb, cuda, x, backward=False)
+    assert torch.equal(got["o"][0, :64], clean["o"][0, :64])
+    assert torch.equal(got["o"][0, :, 1], clean["o"][0, :, 1]) and torch.equal(got["hT"][0, 1], clean["hT"][0, 1])
+    assert torch.equal(got["o"][0, :, 0, 16:], clean["o"][0, :, 0, 16:])
+    rest, want = got["o"][0, 64:, 0, :16].double().cpu(), ref_o[0, 64:, 0, :16]
+    fine = torch.isfinite(rest)
+    assert not fine[7:, 3].any()   # behind the token its own column has no value
+    fine[:, 3] = False
+    assert (rest - want)[fine].abs().max() <= 1e-2 * want.abs().max() if fine.any() else True
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_slices_of_one_projection(kmb, cuda, dtype, shift):
