@@ -19,10 +19,11 @@
 // not add up along the sequence), and dbeta_t = dR_t.w_t.  Both are sums
 // over dv of what the recurrences leave in fp32.
 //
-// Measured (8 x 4096 tokens, 8 heads of 64, bf16): recurrence 186 us (2.9 us a
-// chunk; bound by the side warps' instructions, then by the chain's latency), dV and
-// gates 85 us (3.5 TB/s), the other gradients 189 us (two blocks per SM, latency of
-// shared memory and tensor cores in turn: a third of the issue slots).
+// Measured (8 x 4096 tokens, 8 heads of 64, bf16): recurrence 183 us (2.9 us a
+// chunk; bound by the side warps' instructions, then by the chain's latency); dV and
+// the gates end some 64 us after it (launched early, so their own time overlaps it); the
+// other gradients 185 us (latency of shared memory and tensor cores in turn: 0.31 of
+// the issue slots at 512 chunks and heads).
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 

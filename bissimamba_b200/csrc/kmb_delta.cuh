@@ -519,7 +519,7 @@ __device__ __forceinline__ void get_acc(const unsigned char* base, int tile, int
 
 int delta_sms();
 // Units per block.  One gives the shorter chain (a chunk of dk = dv = 64: forward 2.2 us against 3.1, backward 4.0
-// against 5.2 with two), two more units per SM.  So one where every SM gets a unit at most; with sequences of one
+// against 5.2 with two, before later steps brought two to 3.2 and 2.9), two more units per SM.  So one where every SM gets a unit at most; with sequences of one
 // length two above that.  Packed sequences are of unknown lengths, and the longest's chain is what counts
 // until there are several times as many units as SMs.
 inline int delta_units(const DeltaDesc& d) {

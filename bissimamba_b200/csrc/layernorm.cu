@@ -15,9 +15,9 @@
 // not depend on scheduling.
 //
 // Measured at 131072 x 512 bf16 with residual: forward 82 us (537 MB, 6.5 TB/s: a
-// copy's rate), backward with the weight's gradient 120 us (4.5 TB/s; its 500
-// instructions a row and warp are half of the time); 10007 x 1001 fp32: 23 and
-// 38 us, rows of blocks of 128 threads that wait for two block sums each.
+// copy's rate), backward with the weight's gradient 121 us (4.4 TB/s; its 500
+// instructions a row and warp fill half of the issue slots); 10007 x 1001 fp32: 24 and
+// 42 us, rows of blocks of 128 threads that wait for two block sums each.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cmath>
@@ -249,7 +249,7 @@ ln_fwd_kernel(const LnDesc d) {
 // Backward.  Blocks walk rows with the grid's stride; the normalised entries are computed twice.  Where a warp's rows
 // are aligned (PRE) they come through a ring of shared memory filled by cp.async, two rows ahead (each lane reads
 // what it copied itself, so the warp never waits for another): keeping two rows in registers instead held 128
-// of them and took 135 us at 131072 x 512 bf16, against 115; three blocks per SM spill: 160.  Elsewhere a row stays in registers as it is in memory.
+// of them and took 135 us at 131072 x 512 bf16, against 104; three blocks per SM spilled (179 in that form).  Elsewhere a row stays in registers as it is in memory.
 template <typename T, int VEC, int NCH, bool BLOCK>
 struct LnBwd {
     static constexpr int E = NCH * VEC;
