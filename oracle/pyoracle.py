@@ -72,7 +72,7 @@ def build(force: bool = False) -> None:
     targets = []
     if force or not os.path.exists(ORACLE_SO):
         targets.append("oracle")
-    if REF_SRC and os.path.isdir(REF_SRC) and (force or not os.path.exists(REF_SO)):
+    if REF_SRC and os.path.isfile(os.path.join(REF_SRC, "src", "scan_nd.c")) and (force or not os.path.exists(REF_SO)):
         targets.append("ref")
     if targets:
         subprocess.run(["make", "-s", "-C", HERE, f"REF={REF_SRC}"] + targets, check=True)
