@@ -33,7 +33,7 @@ namespace {
 template <int DKP, typename IO>
 struct BwdSmem {
     static constexpr int C = kDeltaC, NPK = sizeof(IO) == 4 ? 2 : 1, KT = DKP / 8;
-    using ST = DeltaStage<C, DKP, NPK, 2>;
+    using ST = DeltaStage<C, DKP, NPK>;
     using FS = FragBuf<DKP / 16, 2>;
     using FX = FragBuf<C / 16, 2>;
     using FG = FragBuf<C / 16, NPK>;
@@ -83,7 +83,8 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     // the chain warps of the first unit copy the tiles of the recurrence's step i (the side warps have more to do)
     const bool copies = warp < 4 && lane == 0;
     const auto fetch = [&](int i) {
-        ST::load(d, d.Tt, sb + stage(i) * ST::BYTES, smem_u32(&full[stage(i)]), chunk0 + nch - 1 - i, hv, w);
+        const uint32_t st = sb + stage(i) * ST::BYTES;
+        ST::load(d, d.Tt, st, st + ST::FRONT, smem_u32(&full[stage(i)]), chunk0 + nch - 1 - i, hv, w);
     };
     const auto arrived = [&](int i) { return mbar_wait(smem_u32(&full[stage(i)]), (i / NS) & 1); };
     if (threadIdx.x == 0) {
@@ -127,7 +128,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         for (int it = 0; it < nch; it++) {
             if (!begin(it)) return;
             const uint32_t st = sb + stage(it) * ST::BYTES;
-            const float* tk = (const float*)(sm + stage(it) * ST::BYTES + ST::oTok);
+            const float* tk = (const float*)(sm + stage(it) * ST::BYTES + ST::FRONT + ST::oTok);
             const float* tw = tk + w * 16 + c2;
             // dU = diag(G_C.) K dS_C + scale P^T dO (the latter from the side warps)
             float X[2][4], Y[2][4], part[2][4];
@@ -224,7 +225,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     // ahead of chunk c (tile stage `s`): dO's fragments, plain and with the factors of the state's product; P^T dO
     const auto ahead = [&](int c, int s) {
         const uint32_t st = sb + s * ST::BYTES;
-        const float* tk = (const float*)(sm + s * ST::BYTES + ST::oTok);
+        const float* tk = (const float*)(sm + s * ST::BYTES + ST::FRONT + ST::oTok);
         const float* tw = tk + w * 16 + c2;
         uint32_t a[NPK][4];
         Gn.tiles(G, exR + w * 1024, lane, vec);   // the place of the dR that this warp has read
@@ -255,7 +256,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             FG::template get<NPK>(exX, kk, lane, a1);
             const uint32_t o = tile_off<C>(kk * 16 + la_row(lane), w * 16 + la_col(lane));
             zero(part);
-            mma_row<NPK, 2>(part, a1, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::oP + p * ST::TT + o); });
+            mma_row<NPK, 2>(part, a1, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4t(f, st + ST::FRONT + p * ST::TT + o); });
             add_scaled(Y, part, FG::scale(exX, kk) * (tk[TOK_MISC * C + 4 + kk] * d.scale));
         }
         put_acc(exR, w * 2, lane, Y);

@@ -2,53 +2,54 @@
 // (kmb_delta.cuh: a unit of 16 columns of dv, four warps):
 //   X = V - e^gamma K S;  W = M X;  U = beta W;  O = scale (e^gamma Q S + P U);  S <- e^gamma_C S + K^T (G_C. U)
 // all transposed.  The chain of a chunk is latency: three products that each wait
-// for the last, with fp16 pieces made and passed on between them.  Where the
-// cycles of a chunk of dk = 128 go (3400 of them): the barrier and the tiles'
-// arrival 200, v 280, the three products 700 + 570 + 500, making pieces and row
-// scales 750.  So all fragments of a product are loaded before its first
-// instruction, blocks alternate in the tensor cores, and what is not the chain is
-// the side warps'.
-// Measured (16384 tokens, 16 heads of 128, bf16): 449 us, 1.75 us a chunk; one warp
-// for all of dk took 6.5 us, four warps with everything in them 2.1 us.
+// for the last, with fp16 pieces made and passed on between them.  So all fragments
+// of a product are loaded before its first instruction, blocks alternate in the
+// tensor cores, and what is not the chain is the side warps'.  These have two
+// pieces of every fp32 factor too (o is rounded once, whether or not the backward
+// follows): their products share the tensor cores with the chain's, so blocks above
+// the diagonal are left out there (long prompt 615 -> 592 us).
+// Measured (16384 tokens, 16 heads of 128, bf16): 484 us, 1.89 us a chunk, of which one
+// piece in the side warps' products would save 0.14; one warp for all of dk took
+// 6.5 us, four warps with everything in them 2.1 us.
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 
 namespace kmb {
 namespace {
 
-template <int DKP, typename IO, bool KEEP>
+template <int DKP, typename IO>
 struct FwdSmem {
     static constexpr int C = kDeltaC;
     static constexpr int NPK = sizeof(IO) == 4 ? 2 : 1;
-    static constexpr int NPO = (sizeof(IO) == 4 || KEEP) ? 2 : 1;   // pieces behind o: it is rounded to bf16 unless it is kept in fp32
-    using ST = DeltaStage<C, DKP, NPK, NPO>;
+    using ST = DeltaStage<C, DKP, NPK>;
     using FS = FragBuf<DKP / 16, 2>;
     using FX = FragBuf<C / 16, 2>;
-    using FO = FragBuf<C / 16, NPO>;
     // of a unit: fragments of S, X, G_C. U and U, W as accumulators
-    static constexpr int SW = FS::BYTES + 4096, XUO = 2 * FX::BYTES + FO::BYTES;
-    // Where three stages of tiles and two buffers of S and W fit, the side warps finish a chunk's outputs during the
-    // next chunk (LAG), and only one barrier a chunk holds the chain to them.  Else two stages, and the chain waits
-    // for them between its own steps.
-    static constexpr bool lag(int nu) { return 3 * ST::BYTES + nu * (2 * SW + XUO) + nu * 2048 + 128 <= 227 * 1024; }
-    static constexpr int stages(int nu) { return lag(nu) ? 3 : 2; }
+    static constexpr int SW = FS::BYTES + 4096, XUO = 3 * FX::BYTES;
+    // Where two stages of K, Q and M, three of P and the token factors and two buffers of S and W fit, the side warps
+    // finish a chunk's outputs during the next chunk (LAG), and only one barrier a chunk holds the chain to them.
+    // Else two stages of all, and the chain waits for them between its own steps.
+    static constexpr bool lag(int nu) {
+        return 2 * ST::FRONT + 3 * ST::REAR + nu * (2 * SW + XUO) + nu * 2048 + 128 <= 227 * 1024;
+    }
+    static constexpr int rears(int nu) { return lag(nu) ? 3 : 2; }
+    static constexpr int tiles(int nu) { return 2 * ST::FRONT + rears(nu) * ST::REAR; }
     static constexpr int ex(int nu) { return (lag(nu) ? 2 : 1) * SW + XUO; }
-    static constexpr int bytes(int nu) { return stages(nu) * ST::BYTES + nu * ex(nu); }
+    static constexpr int bytes(int nu) { return tiles(nu) + nu * ex(nu); }
 };
 
 template <int DKP, typename IO, bool KEEP, int NU>
 __global__ void __launch_bounds__(256 * NU, 1)
 delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
-    using SM = FwdSmem<DKP, IO, KEEP>;
-    constexpr int C = kDeltaC, NPK = SM::NPK, NPO = SM::NPO;
+    using SM = FwdSmem<DKP, IO>;
+    constexpr int C = kDeltaC, NPK = SM::NPK;
     using ST = typename SM::ST;
     using FS = typename SM::FS;
     using FX = typename SM::FX;
-    using FO = typename SM::FO;
     constexpr int KT = DKP / 8, KTW = KT / 4, KBW = DKP / 64;   // dk tiles, of a warp; its blocks of 16
     constexpr int PK = C * DKP * 2;              // bytes of a K or Q piece
     extern __shared__ __align__(128) unsigned char sm[];
-    constexpr int NS = SM::stages(NU);
+    constexpr int NS = SM::rears(NU);
     constexpr bool LAG = SM::lag(NU);
     __shared__ __align__(8) uint64_t full[NS];
     __shared__ int dead;
@@ -56,10 +57,10 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
     const bool chain = (warp & 4) == 0;
-    unsigned char* ex = sm + NS * ST::BYTES + grp * SM::ex(NU);
+    unsigned char* ex = sm + SM::tiles(NU) + grp * SM::ex(NU);
     unsigned char *exX = ex, *exU = exX + FX::BYTES, *exO = exU + FX::BYTES;
     // buffers of step i
-    const auto bufS = [&](int i) { return exO + FO::BYTES + (LAG ? (i & 1) * SM::SW : 0); };
+    const auto bufS = [&](int i) { return exO + FX::BYTES + (LAG ? (i & 1) * SM::SW : 0); };
     const auto bufW = [&](int i) { return bufS(i) + FS::BYTES; };
     const int ub = (d.units + NU - 1) / NU;
     const int u = (int)(blockIdx.x % ub) * NU + grp;
@@ -78,10 +79,14 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     const int nch = (int)((len + C - 1) / C);
     const size_t sbase = ((size_t)n * d.Hv + hv) * d.dk * d.dv;
 
-    // the side warps of the first unit copy the tiles of the recurrence's step i into stage s
+    // stages of step i's tiles (s: its P and token factors)
+    const auto front = [&](int i) { return sb + (i & 1) * ST::FRONT; };
+    const auto rear = [&](int s) { return sb + 2 * ST::FRONT + s * ST::REAR; };
+    const auto factors = [&](int s) { return (const float*)(sm + 2 * ST::FRONT + s * ST::REAR + ST::oTok); };
+    // the side warps of the first unit copy the tiles of the recurrence's step i into its stages
     const bool copies = warp >= 4 && warp < 8 && lane == 0;
     const auto fetch = [&](int i, int s) {
-        ST::load(d, d.Mt, sb + s * ST::BYTES, smem_u32(&full[s]), chunk0 + i, hv, w);
+        ST::load(d, d.Mt, front(i), rear(s), smem_u32(&full[s]), chunk0 + i, hv, w);
     };
     if (threadIdx.x == 0) {
         dead = 0;
@@ -90,8 +95,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     }
     __syncthreads();
     if (copies && nch > 0) fetch(0, 0);
-    // The chunk's tiles are there, the state's fragments too, and the stage before the last (LAG; else the last) is
-    // read; false: a wait ran out.
+    // The chunk's tiles are there, the state's fragments too, and what the next step's tiles replace is read; false:
+    // a wait ran out.
     int slot = 0, phase = 0, last_slot = 0;   // of the step's tiles, of the last step's
     const auto begin = [&](int i) {
         if (i > 0) {
@@ -148,8 +153,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             if (!begin(c)) return;
             Vn.tiles(V, vbuf[grp * 4 + w], lane, vec);
             if (c + 1 < nch) load_v(c + 1);
-            const uint32_t st = sb + slot * ST::BYTES;
-            const float* tk = (const float*)(sm + slot * ST::BYTES + ST::oTok);
+            const uint32_t st = front(c);
+            const float* tk = factors(slot);
             const float* tw = tk + w * 16 + c2;      // factors of the warp's tokens
             const unsigned char* exS = bufS(c);
             float X[2][4], part[4][2][4], dn, up;
@@ -233,8 +238,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         float O[2][4];
         const auto from_state = [&](int c) {   // the first term
             const unsigned char* exS = bufS(c);
-            const uint32_t st = sb + slot * ST::BYTES;
-            const float* tw = (const float*)(sm + slot * ST::BYTES + ST::oTok) + w * 16 + c2;
+            const uint32_t st = front(c);
+            const float* tw = factors(slot) + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
             float part[2][4];
             zero(O);
@@ -249,8 +254,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     FS::template get<2>(exS, kk, lane, a);
                     if (KEEP && on && s == w) put_frag<NPK, DKP>(d.Sh + fb * NPK * 16 * DKP, 16 * DKP, lane, kk * 16, a);
                     const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
-                    mma_row<NPO, NPK>(part, reinterpret_cast<const uint32_t (&)[NPO][4]>(a), 0, 1,
-                                      [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });
+                    mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });
                 }
                 add_scaled(O, part, f);
                 if (KEEP && on && s == w && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = f;
@@ -263,9 +267,9 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     O[t][e] *= tw[TOK_EG * C + i] * tw[TOK_FQ * C + i];
                 }
         };
-        const auto from_chunk = [&](int c, int s) {   // the second (tiles in stage s), and out
-            const uint32_t st = sb + s * ST::BYTES;
-            const float* tk = (const float*)(sm + s * ST::BYTES + ST::oTok);
+        const auto from_chunk = [&](int c, int s) {   // the second (P in stage s), and out
+            const uint32_t st = rear(s);
+            const float* tk = factors(s);
             const float* tw = tk + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
             float W[2][4], part[2][4], dn, up;
@@ -283,17 +287,18 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) W[t][e] *= tw[TOK_BETA * C + t * 8 + (e & 1)];   // U
             frag_scale(W, up, dn);
-            FO::put(exO, w, lane, W, up, dn);
+            FX::put(exO, w, lane, W, up, dn);
             side_bar(grp);
             const float fp = tk[TOK_MISC * C + 4 + w];
 #pragma unroll
-            for (int kk = 0; kk < C / 16; kk++) {
-                uint32_t a[NPO][4];
-                FO::template get<NPO>(exO, kk, lane, a);
+            for (int kk = 0; kk < C / 16; kk++) {   // row i of P reaches columns j <= i only
+                if (kk > w) continue;
+                uint32_t a[2][4];
+                FX::template get<2>(exO, kk, lane, a);
                 const uint32_t o = tile_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                 zero(part);
-                mma_row<NPO, NPO>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + ST::oP + p * ST::TT + o); });
-                add_masked(O, part, FO::scale(exO, kk) * fp, kk <= w ? ~0u : 0u);
+                mma_row<2, 2>(part, a, 0, 1, [&](int p, int, uint32_t (&f)[4]) { ldm4(f, st + p * ST::TT + o); });
+                add_scaled(O, part, FX::scale(exO, kk) * fp);
             }
             const long long t0 = (long long)c * C + w * 16;
             IO* po = (IO*)d.o + (start + t0) * d.ld_o + (long long)hv * d.dv + col[0];
@@ -328,7 +333,8 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 
 template <int DKP, typename IO, bool KEEP, int NU>
 cudaError_t go(const DeltaDesc& d, cudaStream_t st) {
-    constexpr int SMEM = FwdSmem<DKP, IO, KEEP>::bytes(NU);
+    constexpr int SMEM = FwdSmem<DKP, IO>::bytes(NU);
+    static_assert(SMEM + NU * 2048 + 128 <= 227 * 1024, "shared memory of a block");
     auto kern = delta_chain_fwd_kernel<DKP, IO, KEEP, NU>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;

@@ -334,30 +334,33 @@ __device__ __forceinline__ void cp_wait() {
 // chunk.  The chain of a chunk is bound by latency and by the warps' instructions, so four more warps of the unit do
 // what does not carry it: the outputs, what is kept, what can be computed ahead.  A block holds NU units that
 // share the staged tiles.
-template <int C, int DKP, int NPK, int NPP>
+template <int C, int DKP, int NPK>
 struct DeltaStage {
     static constexpr int KQ = NPK * C * DKP * 2;   // bytes of K (and of Q)
     static constexpr int TT = C * C * 2;           // one piece of M, T or P
-    static constexpr int oQ = KQ, oT = 2 * KQ, oP = oT + 2 * TT, oTok = oP + NPP * TT;
     static constexpr int TOK = TOK_SIZE * 4;
-    static constexpr int BYTES = oTok + TOK;
+    // K, Q and M or T; P and the token factors, which outputs that lag behind read a chunk later
+    static constexpr int oQ = KQ, oT = 2 * KQ, FRONT = oT + 2 * TT;
+    static constexpr int oTok = 2 * TT, REAR = oTok + TOK;
+    static constexpr int BYTES = FRONT + REAR;
 
-    // Bulk copies of one chunk into the stage at `dst`, M or T from `tiles`, by four threads (part 0 .. 3): issuing
-    // all of them takes a warp some 500 cycles.  A copy may complete before part 0 has announced the bytes.
-    static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t dst, uint32_t bar,
-                                                int chunk, int hv, int part) {
+    // Bulk copies of one chunk into the stage at `front` and `rear`, M or T from `tiles`, by four threads (part
+    // 0 .. 3): issuing all of them takes a warp some 500 cycles.  A copy may complete before part 0 has announced
+    // the bytes.
+    static __device__ __forceinline__ void load(const DeltaDesc& d, const __half* tiles, uint32_t front, uint32_t rear,
+                                                uint32_t bar, int chunk, int hv, int part) {
         const int hk = hv / d.grp;
         const size_t kh = ((size_t)chunk * d.Hk + hk) * NPK * C * DKP, vh = (size_t)chunk * d.Hv + hv;
         if (part == 0) {
             mbar_expect_tx(bar, BYTES);
-            bulk(dst + oTok, d.tok + vh * TOK_SIZE, TOK, bar);
-            bulk(dst + oP, d.Pt + vh * 2 * C * C, NPP * TT, bar);
+            bulk(rear + oTok, d.tok + vh * TOK_SIZE, TOK, bar);
+            bulk(rear, d.Pt + vh * 2 * C * C, 2 * TT, bar);
         } else if (part == 1) {
-            bulk(dst, d.Kt + kh, KQ, bar);
+            bulk(front, d.Kt + kh, KQ, bar);
         } else if (part == 2) {
-            bulk(dst + oQ, d.Qt + kh, KQ, bar);
+            bulk(front + oQ, d.Qt + kh, KQ, bar);
         } else {
-            bulk(dst + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
+            bulk(front + oT, tiles + vh * 2 * C * C, 2 * TT, bar);
         }
     }
     static __device__ __forceinline__ void bulk(uint32_t dst, const void* src, unsigned bytes, uint32_t bar) {
