@@ -625,6 +625,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 }
             }
         }
+        __syncthreads();   // the decay tables are there (with dv <= 64 no slice's barrier came in between)
         // weighted matrices: E = scale G dO U^T with the key's and with the query's tile scale, F = -beta G dR U^T
         // with the key's of either side
         float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
