@@ -484,7 +484,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int HN = DKP / 2, HT = HN / 8;
     constexpr int PK = C * DKP * 2;
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ float red[4][8];
+    __shared__ float wf[4][4][4];   // of the weighted matrices: what block (row block, column block) is times
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     float* tk = (float*)(sm + SM::oTok);
     float* mx = (float*)(sm + SM::oMx);
@@ -627,38 +627,34 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
         }
         __syncthreads();   // the decay tables are there (with dv <= 64 no slice's barrier came in between)
         // weighted matrices: E = scale G dO U^T with the key's and with the query's tile scale, F = -beta G dR U^T
-        // with the key's of either side
-        float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // with the key's of either side.  Each block of 16 x 16 has its power of two, like all other factors.
+        float eu[4][2];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            if (ch * 2 + (t >> 1) > rg) continue;
+        for (int t2 = 0; t2 < 2; t2++) {
+            const int cb = ch * 2 + t2;
+            if (cb > rg) continue;
+            float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = rg * 16 + r + (e >> 1) * 8, j = ch * 32 + t * 8 + c2 + (e & 1);
-                const float g = dec.at(i, j, ch * 2 + (t >> 1) == rg, rg) * tk[TOK_BETA * C + j];
-                dP[t][e] = j <= i ? g * d.scale * dP[t][e] : 0.0f;
-                dA[t][e] = j < i ? -g * tk[TOK_BETA * C + i] * dA[t][e] : 0.0f;
-                m[0] = fmaxf(m[0], fabsf(dP[t][e] * tk[TOK_FK * C + j]));
-                m[1] = fmaxf(m[1], fabsf(dP[t][e] * tk[TOK_FQ * C + i]));
-                m[2] = fmaxf(m[2], fabsf(dA[t][e] * tk[TOK_FK * C + j]));
-                m[3] = fmaxf(m[3], fabsf(dA[t][e] * tk[TOK_FK * C + i]));
+            for (int t = t2 * 2; t < t2 * 2 + 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = rg * 16 + r + (e >> 1) * 8, j = ch * 32 + t * 8 + c2 + (e & 1);
+                    const float g = dec.at(i, j, cb == rg, rg) * tk[TOK_BETA * C + j];
+                    dP[t][e] = j <= i ? g * d.scale * dP[t][e] : 0.0f;
+                    dA[t][e] = j < i ? -g * tk[TOK_BETA * C + i] * dA[t][e] : 0.0f;
+                    m[0] = fmaxf(m[0], fabsf(dP[t][e] * tk[TOK_FK * C + j]));
+                    m[1] = fmaxf(m[1], fabsf(dP[t][e] * tk[TOK_FQ * C + i]));
+                    m[2] = fmaxf(m[2], fabsf(dA[t][e] * tk[TOK_FK * C + j]));
+                    m[3] = fmaxf(m[3], fabsf(dA[t][e] * tk[TOK_FK * C + i]));
+                }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float down;
+                warp_scale(m[k], eu[k][t2], down);
+                if (lane == 0) wf[k][rg][cb] = down;
             }
         }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
-            if (lane == 0) red[k][warp] = m[k];
-        }
         __syncthreads();   // the slices are read
-        float eu[4], ed[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            float x = red[k][0];
-#pragma unroll
-            for (int w = 1; w < 8; w++) x = fmaxf(x, red[k][w]);
-            row_scale(x, eu[k], ed[k]);
-        }
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             if (ch * 2 + (t >> 1) > rg) continue;   // blocks above the diagonal are never read
@@ -673,7 +669,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     uint32_t p[NP];
-                    split_pair<NP>(v[k][0] * eu[k], v[k][1] * eu[k], p);
+                    split_pair<NP>(v[k][0] * eu[k][t >> 1], v[k][1] * eu[k][t >> 1], p);
 #pragma unroll
                     for (int x = 0; x < NP; x++) *(uint32_t*)(sm + SM::oE + (k * NP + x) * SM::TE + o) = p[x];
                 }
@@ -684,8 +680,7 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             // k: 0 E K -> dQ, 2 F K -> dK (rows i, sum over j <= i); 1 E^T Q, 3 F^T K -> dK (rows j, sum over i >= j)
-            float acc[HT][4];
-            zero(acc);
+            float (&to)[HT][4] = k == 0 ? dQ : dK;
 #pragma unroll
             for (int kk = 0; kk < C / 16; kk++) {
                 if ((k & 1) ? kk < rg : kk > rg) continue;
@@ -696,18 +691,14 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                     if (k & 1) ldm4t(a[p], base + tile_off<C>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane)));
                     else ldm4(a[p], base + tile_off<C>(rg * 16 + la_row(lane), kk * 16 + la_col(lane)));
                 }
+                float acc[HT][4];
+                zero(acc);
                 mma_row<NP, NP>(acc, a, 0, HN / 16, [&](int p, int t2, uint32_t (&b)[4]) {
                     ldm4t(b, sb + (k == 1 ? SM::oQ : SM::oK) + p * PK +
                                  wide_off<C>(kk * 16 + la_row(lane), ch * HN + t2 * 16 + la_col(lane)));
                 });
+                add_scaled(to, acc, (k & 1) ? wf[k][kk][rg] : wf[k][rg][kk]);
             }
-#pragma unroll
-            for (int t = 0; t < HT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (k == 0) dQ[t][e] = fmaf(ed[k], acc[t][e], dQ[t][e]);
-                    else dK[t][e] = fmaf(ed[k], acc[t][e], dK[t][e]);
-                }
         }
     }
 #pragma unroll
