@@ -680,15 +680,15 @@ size_t layout(const KMBDeltaParams* p, bool train, float* ws, DeltaDesc& d, int&
         const size_t u = cv * d.units * 16 * 2;   // bytes of a column of a unit's tile
         d.Tt = (__half*)take(cv * 2 * C * C * 2);
         d.gam = (double*)take(cv * C * 8);
-        d.Sh = (__half*)take(u * NPK * DKP);
+        d.Sh = (__half*)take(u * 2 * DKP);
         d.Sf = (float*)take(u * 2 * DKP);
-        d.Wh = (__half*)take(u * NPK * C);
+        d.Wh = (__half*)take(u * 2 * C);
         d.Of = (float*)take(u * 2 * C);
         d.Wf = (float*)take(u * 2 * C);
         d.Rf = (float*)take(u * 2 * C);
         d.Gh = (__half*)take(u * NPK * C);
-        d.Rh = (__half*)take(u * NPK * C);
-        d.dSh = (__half*)take(u * NPK * DKP);
+        d.Rh = (__half*)take(u * 2 * C);
+        d.dSh = (__half*)take(u * 2 * DKP);
         d.anchor = (float*)take(cv * d.units * 4 * 4);
         d.mx = (float*)take(cv * d.units * 4 * MX_ROWS * 4);
     }

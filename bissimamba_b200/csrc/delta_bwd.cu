@@ -19,11 +19,12 @@
 // not add up along the sequence), and dbeta_t = dR_t.w_t.  Both are sums
 // over dv of what the recurrences leave in fp32.
 //
-// Measured (8 x 4096 tokens, 8 heads of 64, bf16): recurrence 183 us (2.9 us a
+// Measured (8 x 4096 tokens, 8 heads of 64, bf16): recurrence 195 us (3.0 us a
 // chunk; bound by the side warps' instructions, then by the chain's latency); dV and
-// the gates end some 64 us after it (launched early, so their own time overlaps it); the
-// other gradients 185 us (latency of shared memory and tensor cores in turn: 0.31 of
-// the issue slots at 512 chunks and heads).
+// the gates end some 66 us after it (launched early, so their own time overlaps it); the
+// other gradients 231 us (latency of shared memory and tensor cores in turn).  One
+// piece of every factor, 11 bits, took 182 and 183 us, and put the results 1e-3 off
+// the fp32 sums rounded to bf16.
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 
@@ -302,7 +303,7 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             uint32_t a[2][4];
             FS::template get<2>(exS, w * KBW + b, lane, a);
             if (on) {
-                put_frag<NPK, DKP>(d.dSh + fb * NPK * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
+                put_frag<2, DKP>(d.dSh + fb * 2 * 16 * DKP, 16 * DKP, lane, (w * KBW + b) * 16, a);
                 if (lane == 0) mx[MX_DS] = FS::scale(exS, w * KBW);
             }
         }
@@ -328,10 +329,10 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         float Y[2][4];   // dR, kept
         get_acc(exR, w * 2, lane, Y);
         if (on) {
-            uint32_t a[NPK][4];
+            uint32_t a[2][4];
             frag_scale(Y, up, dn);
-            frag_pieces<NPK>(Y[0], Y[1], up, a);
-            put_frag<NPK, 64>(d.Rh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+            frag_pieces<2>(Y[0], Y[1], up, a);
+            put_frag<2, 64>(d.Rh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
             if (lane == 0) mx[MX_R] = dn;
             put_acc((unsigned char*)(d.Rf + fb * 16 * C), w * 2, lane, Y);
         }
@@ -456,18 +457,18 @@ delta_gates_kernel(const __grid_constant__ DeltaDesc d) {
 
 // ------------------------------------------------------------------ gradients without recurrence
 // Eight warps: 16 token rows x half of dk (and half of the 64 columns of dP, dA) each.  dv is walked in slices of
-// four units, whose fp16 tiles come as the recurrences left them: one piece for bf16 results (11 bits are enough
-// before the rounding), two for fp32.  A unit is one step of 16 in the products over dv, so its powers of two are
+// four units, whose fp16 tiles come as the recurrences left them: one piece for what is exact in one (K, Q and dO in
+// bf16), two for all else, so that dQ and dK are fp32 sums rounded once.  A unit is one step of 16 in the products over dv, so its powers of two are
 // applied when the step's products are added to the fp32 sums.
-template <int DKP, int NP>
+template <int DKP, int NK>
 struct GradSmem {
     static constexpr int C = kDeltaC, NH = DKP / 64;
-    static constexpr int KQ = NP * C * DKP * 2, T64 = 64 * C * 2, SD = NH * 64 * 128;
-    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oW = oG + NP * T64, oR = oW + NP * T64, oS = oR + NP * T64,
-                         oD = oS + NP * SD, oEnd = oD + NP * SD;
+    static constexpr int KQ = NK * C * DKP * 2, T64 = 64 * C * 2, SD = NH * 64 * 128;
+    static constexpr int oK = 0, oQ = KQ, oG = 2 * KQ, oW = oG + NK * T64, oR = oW + 2 * T64, oS = oR + 2 * T64,
+                         oD = oS + 2 * SD, oEnd = oD + 2 * SD;
     // the four weighted matrices take the place of the slices
     static constexpr int oE = oG, TE = C * C * 2;
-    static constexpr int oTok = (oE + 4 * NP * TE > oEnd ? oE + 4 * NP * TE : oEnd);
+    static constexpr int oTok = (oE + 8 * TE > oEnd ? oE + 8 * TE : oEnd);
     static constexpr int oMx = oTok + TOK_SIZE * 4;
     static constexpr int oGam = oMx + 8 * 4 * MX_ROWS * 4;
     static constexpr int oRow = oGam + C * 8, oCol = oRow + C * 4;
@@ -478,9 +479,8 @@ template <int DKP, typename IO>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1)
 delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     constexpr int C = kDeltaC;
-    constexpr bool F32 = sizeof(IO) == 4;
-    constexpr int NP = F32 ? 2 : 1;
-    using SM = GradSmem<DKP, NP>;
+    constexpr int NK = sizeof(IO) == 4 ? 2 : 1;   // pieces of K, Q and dO
+    using SM = GradSmem<DKP, NK>;
     constexpr int HN = DKP / 2, HT = HN / 8;
     constexpr int PK = C * DKP * 2;
     extern __shared__ __align__(128) unsigned char sm[];
@@ -497,8 +497,8 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
     int cnt;
     if (!chunk_range<C>(d, chunk, tok0, cnt)) return;   // the offsets are the forward's
     {
-        const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NP * C * DKP);
-        const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NP * C * DKP);
+        const char* ks = (const char*)(d.Kt + ((size_t)chunk * d.Hk + hk) * NK * C * DKP);
+        const char* qs = (const char*)(d.Qt + ((size_t)chunk * d.Hk + hk) * NK * C * DKP);
         for (int i = tid; i < SM::KQ / 16; i += 256) {
             cp16(sb + SM::oK + i * 16, ks + i * 16);
             cp16(sb + SM::oQ + i * 16, qs + i * 16);
@@ -516,17 +516,17 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
         // tiles of units u0 .. u0 + 3
         const auto slice = [&](int u0) {
             const int nx = d.units - u0 < 4 ? d.units - u0 : 4;
-            for (int i = tid; i < nx * NP * 128; i += 256) {
-                const int x = i / (NP * 128), p = i / 128 % NP, o = (i & 127) * 16;
-                const size_t g = ((head * d.units + u0 + x) * NP + p) * 2048 + o;
+            for (int i = tid; i < nx * 256; i += 256) {
+                const int x = i / 256, p = i / 128 % 2, o = (i & 127) * 16;
+                const size_t un = head * d.units + u0 + x, g = (un * 2 + p) * 2048 + o;
                 const uint32_t s = sb + p * SM::T64 + x * 2048 + o;
-                cp16(s + SM::oG, (const char*)d.Gh + g);
+                if (p < NK) cp16(s + SM::oG, (const char*)d.Gh + (un * NK + p) * 2048 + o);
                 cp16(s + SM::oR, (const char*)d.Rh + g);
                 cp16(s + SM::oW, (const char*)d.Wh + g);
             }
-            for (int i = tid; i < nx * NP * SM::NH * 128; i += 256) {
-                const int x = i / (NP * SM::NH * 128), p = i / (SM::NH * 128) % NP, h = i / 128 % SM::NH, o = (i & 127) * 16;
-                const size_t g = (((head * d.units + u0 + x) * NP + p) * SM::NH + h) * 2048 + o;
+            for (int i = tid; i < nx * 2 * SM::NH * 128; i += 256) {
+                const int x = i / (2 * SM::NH * 128), p = i / (SM::NH * 128) % 2, h = i / 128 % SM::NH, o = (i & 127) * 16;
+                const size_t g = (((head * d.units + u0 + x) * 2 + p) * SM::NH + h) * 2048 + o;
                 const uint32_t s = sb + p * SM::SD + h * 8192 + x * 2048 + o;
                 cp16(s + SM::oD, (const char*)d.dSh + g);
                 cp16(s + SM::oS, (const char*)d.Sh + g);
@@ -565,11 +565,12 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
             for (int kk = 0; kk < nx; kk++) {
                 const float* m4 = mx + (u0 + kk) * 4 * MX_ROWS;
                 const float sG = m4[rg * MX_ROWS + MX_DO], sR = m4[rg * MX_ROWS + MX_R], sW = m4[rg * MX_ROWS + MX_W];
-                uint32_t aG[NP][4], aR[NP][4], aW[NP][4];
+                uint32_t aG[NK][4], aR[2][4], aW[2][4];
                 const uint32_t oa = tile_off<64>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane));
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    ldm4t(aG[p], sb + SM::oG + p * SM::T64 + oa);
+                for (int p = 0; p < NK; p++) ldm4t(aG[p], sb + SM::oG + p * SM::T64 + oa);
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
                     ldm4t(aR[p], sb + SM::oR + p * SM::T64 + oa);
                     ldm4t(aW[p], sb + SM::oW + p * SM::T64 + oa);
                 }
@@ -584,8 +585,8 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                     float part[2][4], par2[2][4];
                     zero(part);
                     zero(par2);
-                    mma_row<NP, NP>(part, aG, 0, 1, ldw);
-                    mma_row<NP, NP>(par2, aR, 0, 1, ldw);
+                    mma_row<NK, 2>(part, aG, 0, 1, ldw);
+                    mma_row<2, 2>(par2, aR, 0, 1, ldw);
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -614,13 +615,13 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                             for (int e = 0; e < 4; e++) to[qd * QT + t][e] = fmaf(part[t][e], f[e >> 1] * s, to[qd * QT + t][e]);
                     };
                     zero(part);
-                    mma_row<NP, NP>(part, aG, 0, QT / 2, lds);
+                    mma_row<NK, 2>(part, aG, 0, QT / 2, lds);
                     add(dQ, fq, sG * sS);
                     zero(part);
-                    mma_row<NP, NP>(part, aR, 0, QT / 2, lds);
+                    mma_row<2, 2>(part, aR, 0, QT / 2, lds);
                     add(dK, fz, sR * sS);
                     zero(part);
-                    mma_row<NP, NP>(part, aW, 0, QT / 2, ldd);
+                    mma_row<2, 2>(part, aW, 0, QT / 2, ldd);
                     add(dK, fu, sW * sD);
                 }
             }
@@ -668,10 +669,10 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
                 const uint32_t o = tile_off<C>(i, j);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    uint32_t p[NP];
-                    split_pair<NP>(v[k][0] * eu[k][t >> 1], v[k][1] * eu[k][t >> 1], p);
+                    uint32_t p[2];
+                    split_pair<2>(v[k][0] * eu[k][t >> 1], v[k][1] * eu[k][t >> 1], p);
 #pragma unroll
-                    for (int x = 0; x < NP; x++) *(uint32_t*)(sm + SM::oE + (k * NP + x) * SM::TE + o) = p[x];
+                    for (int x = 0; x < 2; x++) *(uint32_t*)(sm + SM::oE + (k * 2 + x) * SM::TE + o) = p[x];
                 }
             }
         }
@@ -684,16 +685,16 @@ delta_grads_kernel(const __grid_constant__ DeltaDesc d) {
 #pragma unroll
             for (int kk = 0; kk < C / 16; kk++) {
                 if ((k & 1) ? kk < rg : kk > rg) continue;
-                uint32_t a[NP][4];
+                uint32_t a[2][4];
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    const uint32_t base = sb + SM::oE + (k * NP + p) * SM::TE;
+                for (int p = 0; p < 2; p++) {
+                    const uint32_t base = sb + SM::oE + (k * 2 + p) * SM::TE;
                     if (k & 1) ldm4t(a[p], base + tile_off<C>(kk * 16 + lb_row(lane), rg * 16 + lb_col(lane)));
                     else ldm4(a[p], base + tile_off<C>(rg * 16 + la_row(lane), kk * 16 + la_col(lane)));
                 }
                 float acc[HT][4];
                 zero(acc);
-                mma_row<NP, NP>(acc, a, 0, HN / 16, [&](int p, int t2, uint32_t (&b)[4]) {
+                mma_row<2, NK>(acc, a, 0, HN / 16, [&](int p, int t2, uint32_t (&b)[4]) {
                     ldm4t(b, sb + (k == 1 ? SM::oQ : SM::oK) + p * PK +
                                  wide_off<C>(kk * 16 + la_row(lane), ch * HN + t2 * 16 + la_col(lane)));
                 });

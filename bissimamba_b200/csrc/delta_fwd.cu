@@ -252,7 +252,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     const int kk = s * KBW + b;
                     uint32_t a[2][4];
                     FS::template get<2>(exS, kk, lane, a);
-                    if (KEEP && on && s == w) put_frag<NPK, DKP>(d.Sh + fb * NPK * 16 * DKP, 16 * DKP, lane, kk * 16, a);
+                    if (KEEP && on && s == w) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, kk * 16, a);
                     const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                     mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });
                 }
@@ -275,10 +275,10 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             float W[2][4], part[2][4], dn, up;
             get_acc(bufW(c), w * 2, lane, W);
             if (KEEP && on) {
-                uint32_t a[NPK][4];
+                uint32_t a[2][4];
                 frag_scale(W, up, dn);
-                frag_pieces<NPK>(W[0], W[1], up, a);
-                put_frag<NPK, 64>(d.Wh + fb * NPK * 16 * C, 16 * C, lane, w * 16, a);
+                frag_pieces<2>(W[0], W[1], up, a);
+                put_frag<2, 64>(d.Wh + fb * 2 * 16 * C, 16 * C, lane, w * 16, a);
                 put_acc((unsigned char*)(d.Wf + fb * 16 * C), w * 2, lane, W);
                 if (lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_W] = dn;
             }

@@ -17,9 +17,9 @@
 // [2^14, 2^15) and cut into two fp16 pieces x = x0 + x1, each rounded to nearest:
 // 22 bits down to 2^-18 of the largest entry, and an absolute floor 2^-40 below
 // it, so it holds what an fp32 product needs.  The three products x0 y0, x0 y1,
-// x1 y0 are summed; a bf16 row is a single piece (8 bits fit in 11).  Where a sum is rounded to bf16 right
-// after, one piece of each factor (11 bits) serves.  Three bf16 pieces would take
-// six products for the same accuracy.  The powers of two are undone in the fp32
+// x1 y0 are summed; a bf16 row is a single piece (8 bits fit in 11), everything
+// computed is two, whatever type the result is rounded to.  Three bf16 pieces would
+// take six products for the same accuracy.  The powers of two are undone in the fp32
 // factors that multiply the accumulators anyway.
 #pragma once
 #include <cuda_bf16.h>
@@ -66,8 +66,8 @@ struct DeltaDesc {
     const int* order;            // packed: sequences, the longest first (NULL: as they are)
     // kept for the backward, per unit: swizzled fp16 tiles of 16 rows (columns of dv), in pieces, each warp's part
     // scaled by a power of two (mx)
-    __half *Sh, *Wh;             // state at the chunk's start [pieces][16 * DKP], W [pieces][16 * C]
-    __half *Gh, *Rh, *dSh;       // backward: dO, dR = T^T dU [pieces][16 * C], adjoint of the state at the end
+    __half *Sh, *Wh;             // state at the chunk's start [2][16 * DKP], W [2][16 * C]
+    __half *Gh, *Rh, *dSh;       // backward: dO [pieces of v][16 * C], dR = T^T dU [2][16 * C], adjoint of the state at the end
     float *Sf, *Of, *Wf, *Rf;    // state, O, W and dR in accumulator order [tiles][32 lanes][4]
     float* anchor;               // [nch][Hv][units][4 warps]: <S_0, dS_0> of their parts
     float* mx;                   // [nch][Hv][units][4 warps][MX_ROWS]: what the tiles of S, W, dO, dR, dS are times

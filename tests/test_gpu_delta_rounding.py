@@ -42,3 +42,11 @@ def test_keeping_for_the_backward_changes_no_bit(kmb, cuda, shape, dtype):
         outs.append((o, hT))
     torch.cuda.synchronize()
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gradients_are_rounded_once(kmb, cuda, shape):
+    x = _inputs(*shape, torch.bfloat16, seed=sum(shape) + 1)
+    got, want = _run(kmb, cuda, x), _reference(x)
+    for n in ("o", "dq", "dk", "dv"):
+        assert _once(got[n], want[n]) <= ONCE, n
