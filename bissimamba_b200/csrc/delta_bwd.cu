@@ -99,7 +99,10 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     const auto begin = [&](int i) {
         const bool got = arrived(i);
         if (!__syncthreads_and(got)) {
-            if (!got) set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+            if (!got) {
+                set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+                arrived(i);   // the block's memory stays its own for another limit
+            }
             return false;
         }
         if (copies && i + NS - 1 < nch) fetch(i + NS - 1);

@@ -52,7 +52,6 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
     constexpr int NS = SM::rears(NU);
     constexpr bool LAG = SM::lag(NU);
     __shared__ __align__(8) uint64_t full[NS];
-    __shared__ int dead;
     __shared__ __align__(16) unsigned char vbuf[NU * 4][512];
     const uint32_t sb = (uint32_t)__cvta_generic_to_shared(sm);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = warp >> 3, w = warp & 3;
@@ -89,7 +88,6 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         ST::load(d, d.Mt, front(i), rear(s), smem_u32(&full[s]), chunk0 + i, hv, w);
     };
     if (threadIdx.x == 0) {
-        dead = 0;
         for (int i = 0; i < NS; i++) mbar_init(smem_u32(&full[i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -106,13 +104,15 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 phase ^= 1;
             }
         }
-        // (the side warps wait for the copies; the barrier passes on what they saw)
-        if (!chain && !mbar_wait(smem_u32(&full[slot]), phase)) {
-            set_status(d.status, KMB_ERR_TIMEOUT_FULL);
-            dead = 1;
+        // The side warps wait for the copies; the barrier passes on what they saw, and all threads leave together.
+        const bool got = chain || mbar_wait(smem_u32(&full[slot]), phase);
+        if (!__syncthreads_and(got)) {
+            if (!got) {
+                set_status(d.status, KMB_ERR_TIMEOUT_FULL);
+                mbar_wait(smem_u32(&full[slot]), phase);   // the block's memory stays its own for another limit
+            }
+            return false;
         }
-        __syncthreads();
-        if (dead) return false;
         if (copies && i + 1 < nch) fetch(i + 1, slot + 1 == NS ? 0 : slot + 1);
         return true;
     };
