@@ -521,13 +521,14 @@ __device__ __forceinline__ void get_acc(const unsigned char* base, int tile, int
 }
 
 int delta_sms();
-// Units per block.  One gives the shorter chain (a chunk of dk = dv = 64: forward 2.2 us against 3.1, backward 4.0
-// against 5.2 with two, before later steps brought two to 3.2 and 2.9), two more units per SM.  So one where every SM gets a unit at most; with sequences of one
-// length two above that.  Packed sequences are of unknown lengths, and the longest's chain is what counts
-// until there are several times as many units as SMs.
+// Units per block.  One gives the shorter chain, two more units per SM.  Sequences of one length: two above one unit
+// per SM (16384 tokens, 8 heads of 64, bf16, forward with keep / backward in us, one and two: 128 units 192 / 293 and 262 /
+// 348, 256 units 191 / 295 and 166 / 253).  Packed sequences are of unknown lengths, and the longest's chain is what
+// counts until there are several times as many units as SMs (random lengths, heads of 64: 512 units 190 / 300 and 251 / 342,
+// 1024 units 204 / 311 and 183 / 275; heads of 128: 512 units 390 / 702 and 369 / 721, 1024 units 393 / 707 and 339 / 688).
 inline int delta_units(const DeltaDesc& d) {
     const long long all = (long long)d.nseq * d.Hv * d.units;
-    return d.units > 1 && all > (d.cu ? 8 : 1) * delta_sms() ? 2 : 1;
+    return d.units > 1 && all > (d.cu ? 4 : 1) * delta_sms() ? 2 : 1;
 }
 
 cudaError_t delta_chain_fwd(const DeltaDesc& d, int DKP, bool bf16, bool keep, cudaStream_t st);

@@ -91,3 +91,17 @@ def test_many_packed_sequences(kmb, cuda, n, T, Hk, Hv, dk, dv, dtype):
     cu = _offsets(n, T, n)
     x = _inputs(1, T, Hk, Hv, dk, dv, dtype, seed=n, seqs=n)
     _compare(_run(kmb, cuda, x, cu=cu), _want(x, cuda, cu=cu), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_sequence_does_not_depend_on_the_others(kmb, cuda, packed, dtype):
+    """The same bits alone and among so many that blocks take two units."""
+    n, T, Hk, Hv, dk, dv = 100, 70, 1, 2, 64, 80   # 1000 units
+    x = _inputs(1 if packed else n, T * n if packed else T, Hk, Hv, dk, dv, dtype, seed=5, seqs=n)
+    few = {m: t[:2] if not packed or m in ("h0", "dhT") else t[:, :2 * T].contiguous() for m, t in x.items()}
+    cu = [T * i for i in range(n + 1)] if packed else None
+    many, two = _run(kmb, cuda, x, cu=cu), _run(kmb, cuda, few, cu=None if cu is None else cu[:3])
+    for m in two:
+        part = many[m][:2] if not packed or m in ("hT", "dh0") else many[m][:, :2 * T]
+        assert torch.equal(part, two[m]), m
