@@ -528,7 +528,7 @@ def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=No
     p.h0, p.hT = _ptr(h0), _ptr(hT)
     p.ld_q, p.ld_k, p.ld_v, p.ld_o = (_rows_ld(t, 2, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
     p._keep = (q, k, v, g, beta, o, h0, hT, cu_seqlens)
-    p._entry = Hv * dk * dv
+    p._state = (Hv, dk, dv)
     return p
 
 
@@ -569,8 +569,11 @@ def delta_backward(p, grads, ws, stream=None):
 def delta_step(p, pool, slots=None, stream=None):
     """Recurrent form: the T tokens of each row against its state in pool [entries, Hv, dk, dv], updated in place."""
     n = len(pool)
-    if pool.numel() != n * p._entry or not pool.is_contiguous():
-        raise ValueError("pool: a contiguous [entries, Hv, dk, dv] tensor is expected")
+    if _dtype_of(pool) != DTYPE_F32 or pool.shape[1:] != p._state or not pool.is_contiguous():
+        raise ValueError("pool: a contiguous float32 [entries, Hv, dk, dv] tensor is expected")
+    if slots is not None and (not str(slots.dtype).endswith("int32") or slots.numel() != p.batch
+                              or not slots.is_contiguous()):
+        raise ValueError("slots: a contiguous int32 tensor with one entry per row is expected")
     if (_lib or lib()).kmb_delta_step(p, pool.data_ptr(), n, None if slots is None else slots.data_ptr(), stream):
         check(-1, "kmb_delta_step")
 
