@@ -504,6 +504,12 @@ def _typed(t, like, shape, what):
         raise ValueError(f"{what}: {like.dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
 
 
+def _space(t, what, floats):
+    """A workspace or result that the library writes: contiguous float32, at least so long."""
+    if _dtype_of(t) != DTYPE_F32 or not t.is_contiguous() or t.numel() < floats:
+        raise ValueError(f"{what}: a contiguous float32 tensor of at least {floats} entries is expected")
+
+
 def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=None):
     """KMBDeltaParams of device tensors: q, k [batch, T, Hk, dk], v, o [batch, T, Hv, dv] (slices of a wider token row
     are fine), g, beta [batch, T, Hv] or None, states [sequences, Hv, dk, dv] or None, cu_seqlens int32
@@ -557,11 +563,13 @@ def delta_grads(p, do, dq, dk, dv, dg=None, dbeta=None, dh0=None, dhT=None):
 
 def delta_forward(p, ws, keep=False, stream=None):
     """Chunked gated delta rule; keep=True leaves in ws (a training workspace) what delta_backward reads."""
+    _space(ws, "delta workspace", delta_workspace_floats(p, keep))
     if (_lib or lib()).kmb_delta_forward(p, ws.data_ptr(), 1 if keep else 0, stream):
         check(-1, "kmb_delta_forward")
 
 
 def delta_backward(p, grads, ws, stream=None):
+    _space(ws, "delta workspace", delta_workspace_floats(p, True))
     if (_lib or lib()).kmb_delta_backward(p, grads, ws.data_ptr(), stream):
         check(-1, "kmb_delta_backward")
 
@@ -625,6 +633,8 @@ def norm_forward(p, stream=None):
 
 
 def norm_backward(p, grads, ws=None, stream=None):
+    if ws is not None:
+        _space(ws, "norm workspace", norm_workspace_floats(p) if grads.dw or grads.db else 0)
     if (_lib or lib()).kmb_layernorm_backward(p, grads, _ptr(ws), stream):
         check(-1, "kmb_layernorm_backward")
 
@@ -649,6 +659,9 @@ def grad_clip_workspace_floats(lst):
 
 def grad_clip(lst, max_norm, result, ws, stream=None):
     """Global norm of a grad_list and clipping by it; result: float32 [2], norm and coefficient."""
+    if result is not None:
+        _space(result, "result", 2)
+    _space(ws, "clip workspace", grad_clip_workspace_floats(lst))
     if (_lib or lib()).kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream):
         check(-1, "kmb_grad_clip")
 

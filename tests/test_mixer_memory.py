@@ -24,3 +24,36 @@ def test_pool_and_slots(kmb):
                 slots.float(), slots.short()):
         with pytest.raises(ValueError, match="slots"):
             kmb.delta_step(p, pool, slots=bad)
+
+
+def _wrong(floats):
+    """Workspaces that do not hold so many fp32 entries in a row."""
+    yield torch.zeros(floats - 1)
+    yield torch.zeros(floats, dtype=torch.bfloat16)
+    yield torch.zeros(2 * floats)[::2]
+
+
+def test_workspaces(kmb):
+    t = torch.zeros
+    q, v, g = t(1, 70, 1, 8), t(1, 70, 2, 4), t(1, 70, 2)
+    p = kmb.delta_params(q, q, v, g, g, t(1, 70, 2, 4))
+    grads = kmb.delta_grads(p, v, q, q, v)
+    for keep in (False, True):
+        for ws in _wrong(kmb.delta_workspace_floats(p, keep)):
+            with pytest.raises(ValueError, match="workspace"):
+                kmb.delta_forward(p, ws, keep=keep)
+    for ws in _wrong(kmb.delta_workspace_floats(p, True)):
+        with pytest.raises(ValueError, match="workspace"):
+            kmb.delta_backward(p, grads, ws)
+    x = t(9, 16)
+    n = kmb.norm_params(x, t(16), None, t(9, 16), stats=t(2, 9))
+    for ws in _wrong(kmb.norm_workspace_floats(n)):
+        with pytest.raises(ValueError, match="workspace"):
+            kmb.norm_backward(n, kmb.norm_grads(n, x, dx=t(9, 16), dw=t(16)), ws)
+    lst = kmb.grad_list([t(100)])
+    for ws in _wrong(kmb.grad_clip_workspace_floats(lst)):
+        with pytest.raises(ValueError, match="workspace"):
+            kmb.grad_clip(lst, 1.0, t(2), ws)
+    for result in _wrong(2):
+        with pytest.raises(ValueError, match="result"):
+            kmb.grad_clip(lst, 1.0, result, t(kmb.grad_clip_workspace_floats(lst)))
