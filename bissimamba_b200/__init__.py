@@ -510,6 +510,21 @@ def _space(t, what, floats):
         raise ValueError(f"{what}: a contiguous float32 tensor of at least {floats} entries is expected")
 
 
+def _one_device(like, **tensors):
+    for what, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise ValueError(f"{what}: on {t.device}, expected on {like.device}")
+
+
+def _on_device(p, *tensors):
+    """The kernels read device memory: a call takes only CUDA tensors of its parameters' device."""
+    if not p._cuda:
+        raise ValueError("CUDA tensors are expected")
+    for t in tensors:
+        if t is not None and t.device != p._device:
+            raise ValueError(f"a tensor is on {t.device}, its call's parameters on {p._device}")
+
+
 def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=None):
     """KMBDeltaParams of device tensors: q, k [batch, T, Hk, dk], v, o [batch, T, Hv, dv] (slices of a wider token row
     are fine), g, beta [batch, T, Hv] or None, states [sequences, Hv, dk, dv] or None, cu_seqlens int32
@@ -526,6 +541,7 @@ def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=No
     n = B if cu_seqlens is None else cu_seqlens.numel() - 1
     for t, name in ((h0, "h0"), (hT, "hT")):
         _f32(t, name, (n, Hv, dk, dv))
+    _one_device(q, k=k, v=v, g=g, beta=beta, o=o, h0=h0, hT=hT, cu_seqlens=cu_seqlens)
     p = KMBDeltaParams()
     p.batch, p.T, p.Hk, p.Hv, p.dk, p.dv = B, T, Hk, Hv, dk, dv
     p.dtype, p.scale = _dtype_of(q), float(scale)
@@ -534,7 +550,7 @@ def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=No
     p.h0, p.hT = _ptr(h0), _ptr(hT)
     p.ld_q, p.ld_k, p.ld_v, p.ld_o = (_rows_ld(t, 2, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
     p._keep = (q, k, v, g, beta, o, h0, hT, cu_seqlens)
-    p._state = (Hv, dk, dv)
+    p._state, p._device, p._cuda = (Hv, dk, dv), q.device, q.is_cuda
     return p
 
 
@@ -552,6 +568,7 @@ def delta_grads(p, do, dq, dk, dv, dg=None, dbeta=None, dh0=None, dhT=None):
     seqs = p.n_seq if p.cu_seqlens else p.batch
     for t, n in ((dh0, "dh0"), (dhT, "dhT")):
         _f32(t, n, (seqs, p.Hv, p.dk, p.dv))
+    _one_device(q, do=do, dq=dq, dk=dk, dv=dv, dg=dg, dbeta=dbeta, dh0=dh0, dhT=dhT)
     g = KMBDeltaGrads()
     g.do_, g.dhT, g.dq, g.dk, g.dv = _ptr(do), _ptr(dhT), _ptr(dq), _ptr(dk), _ptr(dv)
     g.dg, g.dbeta, g.dh0 = _ptr(dg), _ptr(dbeta), _ptr(dh0)
@@ -564,12 +581,14 @@ def delta_grads(p, do, dq, dk, dv, dg=None, dbeta=None, dh0=None, dhT=None):
 def delta_forward(p, ws, keep=False, stream=None):
     """Chunked gated delta rule; keep=True leaves in ws (a training workspace) what delta_backward reads."""
     _space(ws, "delta workspace", delta_workspace_floats(p, keep))
+    _on_device(p, ws)
     if (_lib or lib()).kmb_delta_forward(p, ws.data_ptr(), 1 if keep else 0, stream):
         check(-1, "kmb_delta_forward")
 
 
 def delta_backward(p, grads, ws, stream=None):
     _space(ws, "delta workspace", delta_workspace_floats(p, True))
+    _on_device(p, ws)
     if (_lib or lib()).kmb_delta_backward(p, grads, ws.data_ptr(), stream):
         check(-1, "kmb_delta_backward")
 
@@ -582,6 +601,7 @@ def delta_step(p, pool, slots=None, stream=None):
     if slots is not None and (not str(slots.dtype).endswith("int32") or slots.numel() != p.batch
                               or not slots.is_contiguous()):
         raise ValueError("slots: a contiguous int32 tensor with one entry per row is expected")
+    _on_device(p, pool, slots)
     if (_lib or lib()).kmb_delta_step(p, pool.data_ptr(), n, None if slots is None else slots.data_ptr(), stream):
         check(-1, "kmb_delta_step")
 
@@ -596,6 +616,7 @@ def norm_params(x, w, b, y, eps=1e-5, residual=None, total=None, stats=None):
     for t, n in ((w, "w"), (b, "b")):
         _f32(t, n, (D,))
     _f32(stats, "stats", (2, rows))
+    _one_device(x, w=w, b=b, y=y, residual=residual, total=total, stats=stats)
     p = KMBNormParams()
     p.rows, p.D, p.dtype, p.eps = rows, D, _dtype_of(x), float(eps)
     p.x, p.residual, p.total, p.y, p.w, p.b = _ptr(x), _ptr(residual), _ptr(total), _ptr(y), _ptr(w), _ptr(b)
@@ -604,6 +625,7 @@ def norm_params(x, w, b, y, eps=1e-5, residual=None, total=None, stats=None):
     p.ld_x, p.ld_residual, p.ld_total, p.ld_y = (0 if t is None else _rows_ld(t, 1, n) for t, n in
                                                  ((x, "x"), (residual, "residual"), (total, "total"), (y, "y")))
     p._keep = (x, w, b, y, residual, total, stats)
+    p._device, p._cuda = x.device, x.is_cuda
     return p
 
 
@@ -614,6 +636,7 @@ def norm_grads(p, dy, dx=None, dw=None, db=None, dtotal=None, accumulate=False):
         _typed(t, x, x.shape, n)
     for t, n in ((dw, "dw"), (db, "db")):
         _f32(t, n, (p.D,))
+    _one_device(x, dy=dy, dx=dx, dw=dw, db=db, dtotal=dtotal)
     g = KMBNormGrads()
     g.dy, g.dtotal, g.dx, g.dw, g.db = _ptr(dy), _ptr(dtotal), _ptr(dx), _ptr(dw), _ptr(db)
     g.ld_dy, g.ld_dtotal, g.ld_dx = (0 if t is None else _rows_ld(t, 1, n) for t, n in
@@ -628,6 +651,7 @@ def norm_workspace_floats(p):
 
 
 def norm_forward(p, stream=None):
+    _on_device(p)
     if (_lib or lib()).kmb_layernorm_forward(p, stream):
         check(-1, "kmb_layernorm_forward")
 
@@ -635,6 +659,7 @@ def norm_forward(p, stream=None):
 def norm_backward(p, grads, ws=None, stream=None):
     if ws is not None:
         _space(ws, "norm workspace", norm_workspace_floats(p) if grads.dw or grads.db else 0)
+    _on_device(p, ws)
     if (_lib or lib()).kmb_layernorm_backward(p, grads, _ptr(ws), stream):
         check(-1, "kmb_layernorm_backward")
 
@@ -648,8 +673,10 @@ def grad_list(grads, outs=None):
             raise ValueError("grad_list: contiguous tensors are expected")
         if o is not None and (o.dtype != t.dtype or o.numel() != t.numel() or not o.is_contiguous()):
             raise ValueError("grad_list: an output does not match its gradient")
+        _one_device(grads[0], gradient=t, output=o)
         e.in_, e.out, e.n, e.dtype = t.data_ptr(), _ptr(o), t.numel(), _dtype_of(t)
     arr._keep = (list(grads), list(outs))
+    arr._device, arr._cuda = (grads[0].device, grads[0].is_cuda) if len(grads) else (None, True)
     return arr
 
 
@@ -662,6 +689,10 @@ def grad_clip(lst, max_norm, result, ws, stream=None):
     if result is not None:
         _space(result, "result", 2)
     _space(ws, "clip workspace", grad_clip_workspace_floats(lst))
+    if not ws.is_cuda:
+        raise ValueError("CUDA tensors are expected")
+    if len(lst):
+        _on_device(lst, ws, result)
     if (_lib or lib()).kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream):
         check(-1, "kmb_grad_clip")
 

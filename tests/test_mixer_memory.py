@@ -57,3 +57,30 @@ def test_workspaces(kmb):
     for result in _wrong(2):
         with pytest.raises(ValueError, match="result"):
             kmb.grad_clip(lst, 1.0, result, t(kmb.grad_clip_workspace_floats(lst)))
+
+
+def test_host_tensors_and_other_devices(kmb):
+    """A host pointer is no device pointer; "meta" stands for another device."""
+    t = torch.zeros
+    q, v, g = t(1, 4, 1, 8), t(1, 4, 2, 4), t(1, 4, 2)
+    p = kmb.delta_params(q, q, v, g, g, t(1, 4, 2, 4))
+    grads = kmb.delta_grads(p, v, q, q, v)
+    ws = t(kmb.delta_workspace_floats(p, True))
+    x = t(9, 16)
+    n = kmb.norm_params(x, None, None, t(9, 16), stats=t(2, 9))
+    lst, clip_ws = kmb.grad_list([x]), t(kmb.grad_clip_workspace_floats(kmb.grad_list([x])))
+    for call in (lambda: kmb.delta_forward(p, ws), lambda: kmb.delta_backward(p, grads, ws),
+                 lambda: kmb.delta_step(p, t(1, 2, 8, 4)), lambda: kmb.norm_forward(n),
+                 lambda: kmb.norm_backward(n, kmb.norm_grads(n, x, dx=t(9, 16))),
+                 lambda: kmb.grad_clip(lst, 1.0, t(2), clip_ws),
+                 lambda: kmb.grad_clip(kmb.grad_list([]), 1.0, t(2), clip_ws)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    m = lambda s: s.to("meta")
+    for call in (lambda: kmb.delta_params(q, m(q), v, g, g, v), lambda: kmb.delta_params(q, q, v, g, m(g), v),
+                 lambda: kmb.delta_params(q, q, v, g, g, v, h0=m(t(1, 2, 8, 4))),
+                 lambda: kmb.delta_params(q, q, v, g, g, v, h0=t(2, 2, 8, 4), cu_seqlens=m(t(3, dtype=torch.int32))),
+                 lambda: kmb.delta_grads(p, m(v), q, q, v), lambda: kmb.norm_params(x, m(t(16)), None, x),
+                 lambda: kmb.norm_grads(n, m(x)), lambda: kmb.grad_list([x, m(x)]), lambda: kmb.grad_list([x], [m(x)])):
+        with pytest.raises(ValueError, match="expected on cpu"):
+            call()
