@@ -667,6 +667,8 @@ def norm_backward(p, grads, ws=None, stream=None):
 def grad_list(grads, outs=None):
     """KMBGradTensor array of contiguous gradient tensors; outs: where the clipped ones go (default: in place)."""
     outs = grads if outs is None else outs
+    if len(outs) != len(grads):
+        raise ValueError(f"grad_list: {len(grads)} gradients, {len(outs)} outputs")
     arr = (KMBGradTensor * len(grads))()
     for e, t, o in zip(arr, grads, outs):
         if not t.is_contiguous():

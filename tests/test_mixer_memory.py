@@ -84,3 +84,10 @@ def test_host_tensors_and_other_devices(kmb):
                  lambda: kmb.norm_grads(n, m(x)), lambda: kmb.grad_list([x, m(x)]), lambda: kmb.grad_list([x], [m(x)])):
         with pytest.raises(ValueError, match="expected on cpu"):
             call()
+
+
+def test_a_list_without_its_outputs(kmb):
+    a = [torch.zeros(3) for _ in range(3)]
+    for outs in (a[:2], [], a + a):
+        with pytest.raises(ValueError, match="3 gradients"):
+            kmb.grad_list(a, outs)
