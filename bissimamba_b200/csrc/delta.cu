@@ -546,6 +546,12 @@ delta_step_kernel(const __grid_constant__ StepDesc d, int vec) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
             vc[e] = c0 + e < d.dv ? ldt(v, tok * d.ld_v + (long long)hv * d.dv + c0 + e) : 0.0f;
+        if (al == 0.0f) {   // forgotten, whatever it holds (0 times an infinity or NaN would stay one)
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) S[i][e] = 0.0f;
+        }
         float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NR; i++)
