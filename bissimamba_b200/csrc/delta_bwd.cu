@@ -202,7 +202,6 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                 });
                 add_scaled(S, ps, FX::scale(exF, kk));
             }
-            if (fresh(tk)) zero(S);
             put_state();
         }
         __syncthreads();   // the side warps read the last fragments
@@ -312,7 +311,6 @@ delta_chain_bwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
             }
         }
         if (on) get_acc((const unsigned char*)(d.Sf + fb * 16 * DKP), w * KTW, lane, sr);
-        if (fresh((const float*)(sm + stage(it) * ST::BYTES + ST::FRONT + ST::oTok))) zero(sr);
         // (scale e^gamma dO)^T Q
         {
             float Z[KTW][4], ps[KTW][4];

@@ -119,12 +119,14 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 
     if (chain) {
         float S[KTW][4];
+        // a reset at the first token forgets the initial state, whatever it holds (0 times an infinity or NaN would stay one)
+        const bool carry = d.h0 && !(d.g && len > 0 && expf(d.g[start * d.Hv + hv]) == 0.0f);
 #pragma unroll
         for (int t = 0; t < KTW; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = (w * KTW + t) * 8 + c2 + (e & 1);
-                S[t][e] = (d.h0 && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
+                S[t][e] = (carry && i < d.dk && cok[e >> 1]) ? d.h0[sbase + (size_t)i * d.dv + col[e >> 1]] : 0.0f;
             }
         TokenTile<IO> Vn;   // v of the warp's tokens of the next chunk
         const auto load_v = [&](int c) {
@@ -169,7 +171,6 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) add_scaled(X, part[k], FS::scale(exS, k0 + k));
             }
-            if (fresh(tk)) zero(X);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -208,7 +209,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
 #pragma unroll
             for (int t = 0; t < KTW; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) S[t][e] = fresh(tk) ? 0.0f : S[t][e] * last;
+                for (int e = 0; e < 4; e++) S[t][e] *= last;
             constexpr int KB = KTW == 2 || NU == 1 ? 4 : 2;   // blocks at a time: what registers allow
 #pragma unroll
             for (int k0 = 0; k0 < C / 16; k0 += KB) {
@@ -240,8 +241,7 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
         const auto from_state = [&](int c) {   // the first term
             const unsigned char* exS = bufS(c);
             const uint32_t st = front(c);
-            const float* tk = factors(slot);
-            const float* tw = tk + w * 16 + c2;
+            const float* tw = factors(slot) + w * 16 + c2;
             const size_t fb = (((size_t)(chunk0 + c) * d.Hv + hv) * d.units + u);
             float part[2][4];
             zero(O);
@@ -254,17 +254,13 @@ delta_chain_fwd_kernel(const __grid_constant__ DeltaDesc d, int vec) {
                     const int kk = s * KBW + b;
                     uint32_t a[2][4];
                     FS::template get<2>(exS, kk, lane, a);
-                    if (KEEP && on && s == w) {
-                        uint32_t k2[2][4] = {};
-                        put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, kk * 16, fresh(tk) ? k2 : a);
-                    }
+                    if (KEEP && on && s == w) put_frag<2, DKP>(d.Sh + fb * 2 * 16 * DKP, 16 * DKP, lane, kk * 16, a);
                     const uint32_t o = wide_off<C>(w * 16 + lb_row(lane), kk * 16 + lb_col(lane));
                     mma_row<2, NPK>(part, a, 0, 1, [&](int p, int, uint32_t (&b4)[4]) { ldm4(b4, st + ST::oQ + p * PK + o); });
                 }
                 add_scaled(O, part, f);
                 if (KEEP && on && s == w && lane == 0) d.mx[(fb * 4 + w) * MX_ROWS + MX_S] = f;
             }
-            if (fresh(tk)) zero(O);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll

@@ -453,9 +453,6 @@ __device__ __forceinline__ void add_masked(float (&acc)[N][4], const float (&par
         for (int e = 0; e < 4; e++)
             acc[i][e] = fmaf(__uint_as_float(__float_as_uint(part[i][e]) & on), f, acc[i][e]);
 }
-// A reset at the chunk's first token: none of it depends on the state before, whatever that holds (0 times an
-// infinity or NaN would stay one).  tk: the chunk's token factors.
-__device__ __forceinline__ bool fresh(const float* tk) { return tk[TOK_EG * kDeltaC] == 0.0f; }
 // barriers of unit g: its chain warps, its side warps, all of them
 __device__ __forceinline__ void chain_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 1) : "memory"); }
 __device__ __forceinline__ void side_bar(int g) { asm volatile("bar.sync %0, 128;" ::"r"(3 * g + 2) : "memory"); }
