@@ -506,7 +506,7 @@ def _typed(t, like, shape, what):
 
 def _space(t, what, floats):
     """A workspace or result that the library writes: contiguous float32, at least so long."""
-    if _dtype_of(t) != DTYPE_F32 or not t.is_contiguous() or t.numel() < floats:
+    if t.element_size() != 4 or not t.is_floating_point() or not t.is_contiguous() or t.numel() < floats:
         raise ValueError(f"{what}: a contiguous float32 tensor of at least {floats} entries is expected")
 
 
@@ -518,11 +518,11 @@ def _one_device(like, **tensors):
 
 def _on_device(p, *tensors):
     """The kernels read device memory: a call takes only CUDA tensors of its parameters' device."""
-    if not p._cuda:
+    if p._device < 0:
         raise ValueError("CUDA tensors are expected")
     for t in tensors:
-        if t is not None and t.device != p._device:
-            raise ValueError(f"a tensor is on {t.device}, its call's parameters on {p._device}")
+        if t is not None and t.get_device() != p._device:
+            raise ValueError(f"a tensor is on {t.device}, its call's parameters on cuda:{p._device}")
 
 
 def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=None):
@@ -550,7 +550,8 @@ def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=No
     p.h0, p.hT = _ptr(h0), _ptr(hT)
     p.ld_q, p.ld_k, p.ld_v, p.ld_o = (_rows_ld(t, 2, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
     p._keep = (q, k, v, g, beta, o, h0, hT, cu_seqlens)
-    p._state, p._device, p._cuda = (Hv, dk, dv), q.device, q.is_cuda
+    import torch   # loaded already: the tensors are its own
+    p._state, p._device, p._index_type = (Hv, dk, dv), q.get_device(), torch.int32
     return p
 
 
@@ -595,14 +596,14 @@ def delta_backward(p, grads, ws, stream=None):
 
 def delta_step(p, pool, slots=None, stream=None):
     """Recurrent form: the T tokens of each row against its state in pool [entries, Hv, dk, dv], updated in place."""
-    n = len(pool)
-    if _dtype_of(pool) != DTYPE_F32 or pool.shape[1:] != p._state or not pool.is_contiguous():
+    shape = pool.shape
+    if (len(shape) != 4 or shape != (shape[0],) + p._state or pool.element_size() != 4 or not pool.is_floating_point()
+            or not pool.is_contiguous()):
         raise ValueError("pool: a contiguous float32 [entries, Hv, dk, dv] tensor is expected")
-    if slots is not None and (not str(slots.dtype).endswith("int32") or slots.numel() != p.batch
-                              or not slots.is_contiguous()):
+    if slots is not None and (slots.dtype is not p._index_type or slots.numel() != p.batch or not slots.is_contiguous()):
         raise ValueError("slots: a contiguous int32 tensor with one entry per row is expected")
     _on_device(p, pool, slots)
-    if (_lib or lib()).kmb_delta_step(p, pool.data_ptr(), n, None if slots is None else slots.data_ptr(), stream):
+    if (_lib or lib()).kmb_delta_step(p, pool.data_ptr(), shape[0], None if slots is None else slots.data_ptr(), stream):
         check(-1, "kmb_delta_step")
 
 
@@ -625,7 +626,7 @@ def norm_params(x, w, b, y, eps=1e-5, residual=None, total=None, stats=None):
     p.ld_x, p.ld_residual, p.ld_total, p.ld_y = (0 if t is None else _rows_ld(t, 1, n) for t, n in
                                                  ((x, "x"), (residual, "residual"), (total, "total"), (y, "y")))
     p._keep = (x, w, b, y, residual, total, stats)
-    p._device, p._cuda = x.device, x.is_cuda
+    p._device = x.get_device()
     return p
 
 
@@ -678,7 +679,8 @@ def grad_list(grads, outs=None):
         _one_device(grads[0], gradient=t, output=o)
         e.in_, e.out, e.n, e.dtype = t.data_ptr(), _ptr(o), t.numel(), _dtype_of(t)
     arr._keep = (list(grads), list(outs))
-    arr._device, arr._cuda = (grads[0].device, grads[0].is_cuda) if len(grads) else (None, True)
+    arr._device = grads[0].get_device() if len(grads) else None
+    arr._space = grad_clip_workspace_floats(arr)
     return arr
 
 
@@ -690,11 +692,11 @@ def grad_clip(lst, max_norm, result, ws, stream=None):
     """Global norm of a grad_list and clipping by it; result: float32 [2], norm and coefficient."""
     if result is not None:
         _space(result, "result", 2)
-    _space(ws, "clip workspace", grad_clip_workspace_floats(lst))
-    if not ws.is_cuda:
-        raise ValueError("CUDA tensors are expected")
+    _space(ws, "clip workspace", lst._space)
     if len(lst):
         _on_device(lst, ws, result)
+    elif ws.get_device() < 0:
+        raise ValueError("CUDA tensors are expected")
     if (_lib or lib()).kmb_grad_clip(lst, len(lst), max_norm, _ptr(result), ws.data_ptr(), stream):
         check(-1, "kmb_grad_clip")
 
