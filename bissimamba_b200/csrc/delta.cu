@@ -2,6 +2,7 @@
 // per-chunk matrices that need no state, and the recurrent form.
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include "kmb_delta.cuh"
 #include "kmb_launch.cuh"
 #include "../../include/kmamba_delta.h"
@@ -636,6 +637,17 @@ const char* check(const KMBDeltaParams* p) {
         return "delta: a token stride is at most 2^31 - 1 elements";
     return nullptr;
 }
+// whether one of the pointers is off its element's boundary (an access there is an error of the device)
+bool off(size_t size, std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if ((uintptr_t)p % size) return true;
+    return false;
+}
+constexpr const char* kOff = "delta: a tensor is not aligned to its elements";
+size_t elem(const KMBDeltaParams* p) { return p->dtype == KMB_DTYPE_BF16 ? 2 : 4; }
+bool off(const KMBDeltaParams* p) {
+    return off(elem(p), {p->q, p->k, p->v, p->o}) || off(4, {p->g, p->beta, p->h0, p->hT, p->cu_seqlens});
+}
 const char* check_launch(const KMBDeltaParams* p, const DeltaDesc& d) {
     if ((double)d.nseq * d.Hv * d.units > 2147483647.0) return "delta: too many sequences times heads for one launch";
     if ((double)d.nch * d.Hv > 2147483647.0) return "delta: too many chunks times heads for one launch";
@@ -736,6 +748,7 @@ int kmb_delta_forward(const KMBDeltaParams* p, float* ws, int keep, void* stream
     layout(p, keep != 0, ws, d, DKP);
     if (d.nseq == 0) return 0;
     if (d.total > 0 && (!p->q || !p->k || !p->v || !p->o)) return set_error("delta: q, k, v and o are required");
+    if (off(p)) return set_error(kOff);
     if (!ws || ((uintptr_t)ws & 15)) return set_error("delta: a 16-byte aligned workspace is required");
     if (const char* m = check_launch(p, d)) return set_error(m);
     const bool bf16 = p->dtype == KMB_DTYPE_BF16;
@@ -766,6 +779,8 @@ int kmb_delta_backward(const KMBDeltaParams* p, const KMBDeltaGrads* g, float* w
         return set_error("delta backward: a token stride is shorter than a token");
     if (g->ld_do > 0x7fffffffL || g->ld_dq > 0x7fffffffL || g->ld_dk > 0x7fffffffL || g->ld_dv > 0x7fffffffL)
         return set_error("delta backward: a token stride is at most 2^31 - 1 elements");
+    if (off(p) || off(elem(p), {g->do_, g->dq, g->dk, g->dv}) || off(4, {g->dhT, g->dg, g->dbeta, g->dh0}))
+        return set_error(kOff);
     if (!ws || ((uintptr_t)ws & 15)) return set_error("delta backward: the forward's workspace is required");
     if (const char* m = check_launch(p, d)) return set_error(m);
     d.go = g->do_; d.dhT = g->dhT; d.dq = g->dq; d.dkk = g->dk; d.dvv = g->dv;
@@ -789,6 +804,7 @@ int kmb_delta_step(const KMBDeltaParams* p, float* pool, long n_slots, const int
     if (p->batch == 0 || p->T == 0) return 0;
     if (!p->q || !p->k || !p->v || !p->o || !pool) return set_error("kmb_delta_step: q, k, v, o and the pool are required");
     if (n_slots < 0) return set_error("kmb_delta_step: n_slots must be >= 0");
+    if (off(p) || off(4, {pool, slots})) return set_error(kOff);
     StepDesc d{};
     d.batch = p->batch; d.T = p->T; d.Hk = (int)p->Hk; d.Hv = (int)p->Hv; d.grp = d.Hv / d.Hk;
     d.dk = (int)p->dk; d.dv = (int)p->dv; d.units = (d.dv + 15) / 16; d.scale = p->scale;

@@ -353,6 +353,7 @@ int kmb_grad_clip(const KMBGradTensor* ts, long n, float max_norm, float* result
         if (((uintptr_t)ts[i].in & m) || ((uintptr_t)ts[i].out & m))
             return set_error("kmb_grad_clip: a tensor is not aligned to its elements");
     }
+    if ((uintptr_t)result & 3) return set_error("kmb_grad_clip: result is not aligned to its elements");
     bool too_long = false;
     const long parts = launches_of(n > 0 ? n : 1) * GC_MAX_BLOCKS;
     cudaStream_t st = (cudaStream_t)stream;

@@ -22,6 +22,7 @@
 #include <cuda_runtime.h>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include "../../include/kmamba_norm.h"
 #include "kmb_launch.cuh"
 
@@ -578,6 +579,17 @@ const char* check(const KMBNormParams* p) {
         if (l != 0 && l < p->D) return "layernorm: a row stride is shorter than D";
     return nullptr;
 }
+// whether one of the pointers is off its element's boundary (an access there is an error of the device)
+bool off(size_t size, std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if ((uintptr_t)p % size) return true;
+    return false;
+}
+constexpr const char* kOff = "layernorm: a tensor is not aligned to its elements";
+size_t elem(const KMBNormParams* p) { return p->dtype == KMB_DTYPE_BF16 ? 2 : 4; }
+bool off(const KMBNormParams* p) {
+    return off(elem(p), {p->x, p->residual, p->total, p->y}) || off(4, {p->w, p->b, p->mean, p->rstd});
+}
 long long or_d(long ld, long D) { return ld ? ld : D; }
 
 }  // namespace
@@ -593,6 +605,7 @@ int kmb_layernorm_forward(const KMBNormParams* p, void* stream) {
     if (p->rows == 0) return 0;
     if (!p->x || !p->y) return set_error("layernorm: x and y are required");
     if (p->total && !p->residual) return set_error("layernorm: total without a residual");
+    if (off(p)) return set_error(kOff);
     LnDesc d{};
     d.rows = p->rows; d.D = (int)p->D; d.eps = p->eps;
     d.x = p->x; d.res = p->residual; d.tot = p->total; d.y = p->y; d.w = p->w; d.b = p->b;
@@ -632,6 +645,7 @@ int kmb_layernorm_backward(const KMBNormParams* p, const KMBNormGrads* g, float*
     if (!s) return set_error("layernorm backward: the normalised input (total, or x without a residual) is required");
     if (!p->mean || !g->dy) return set_error("layernorm backward: mean, rstd and dy are required");
     if (wgrad && !ws) return set_error("layernorm backward: dw and db need the workspace");
+    if (off(p) || off(elem(p), {g->dy, g->dtotal, g->dx}) || off(4, {g->dw, g->db, ws})) return set_error(kOff);
     LnDesc d{};
     d.rows = p->rows; d.D = (int)p->D; d.eps = p->eps;
     d.x = s; d.ld_x = p->residual ? or_d(p->ld_total, p->D) : or_d(p->ld_x, p->D);
