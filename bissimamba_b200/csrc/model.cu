@@ -506,7 +506,7 @@ int kmb_model_optimizer_step(KMamba* m, void* stream) {
 
 int kmb_model_clip_gradients(KMamba* m, float max_norm, float* result, float* ws, void* stream) {
     if (!m) return set_error("kmb_model_clip_gradients: null model");
-    if (!(max_norm > 0.0f)) {
+    if (max_norm <= 0.0f) {
         if (!m->training) return set_error("kmb_model_clip_gradients: clip_norm needs kmamba_enable_training");
         max_norm = m->opt.clip_norm;
     }
