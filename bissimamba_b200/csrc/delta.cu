@@ -486,7 +486,7 @@ struct StepRow {
                 w[i] = r0 + i * (16 / (int)sizeof(IO)) < dk ? *(const uint4*)(p + r0 + i * (16 / (int)sizeof(IO)))
                                                             : make_uint4(0, 0, 0, 0);
         } else {
-            IO e[NR];
+            alignas(16) IO e[NR];
 #pragma unroll
             for (int i = 0; i < NR; i++) {
                 if (r0 + i < dk) e[i] = p[r0 + i];
