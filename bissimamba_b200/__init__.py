@@ -528,7 +528,8 @@ def _on_device(p, *tensors):
 def delta_params(q, k, v, g, beta, o, scale=1.0, h0=None, hT=None, cu_seqlens=None):
     """KMBDeltaParams of device tensors: q, k [batch, T, Hk, dk], v, o [batch, T, Hv, dv] (slices of a wider token row
     are fine), g, beta [batch, T, Hv] or None, states [sequences, Hv, dk, dv] or None, cu_seqlens int32
-    [sequences + 1] with batch 1.  The struct holds pointers: keep the tensors alive while it is used."""
+    [sequences + 1] with batch 1.  The struct holds its tensors, the outputs among them: an autograd function that kept it
+    on its context would keep itself alive."""
     B, T, Hk, dk = q.shape
     Hv, dv = v.shape[2], v.shape[3]
     _typed(k, q, q.shape, "k")

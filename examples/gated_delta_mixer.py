@@ -48,22 +48,26 @@ class Linear(torch.autograd.Function):
         return product(dy, w.t()), product(dy, x, 1)
 
 
+# A parameter struct holds its tensors, the outputs among them.  A context that kept one would keep itself alive through
+# them, and the workspace with it, until Python's collector comes by: the backward makes its own.
 class Norm(torch.autograd.Function):
     """(y, s): s = x + residual, y = its layer norm"""
 
     @staticmethod
     def forward(ctx, x, residual, w, b):
-        y, s, stats = torch.empty_like(x), torch.empty_like(x), torch.empty(2, x.shape[0], device=x.device)
-        ctx.p = kmb.norm_params(x, w, b, y, residual=residual, total=s, stats=stats)
-        kmb.norm_forward(ctx.p, stream=_stream())
+        y, s, ctx.stats = torch.empty_like(x), torch.empty_like(x), torch.empty(2, x.shape[0], device=x.device)
+        kmb.norm_forward(kmb.norm_params(x, w, b, y, residual=residual, total=s, stats=ctx.stats), stream=_stream())
+        ctx.save_for_backward(s, w)
         return y, s
 
     @staticmethod
     def backward(ctx, dy, ds):
+        s, w = ctx.saved_tensors
         dy, ds = dy.contiguous(), ds.contiguous()
-        dx, dw = torch.empty_like(dy), torch.empty(2, ctx.p.D, device=dy.device)
-        g = kmb.norm_grads(ctx.p, dy, dx=dx, dw=dw[0], db=dw[1], dtotal=ds)
-        kmb.norm_backward(ctx.p, g, torch.empty(kmb.norm_workspace_floats(ctx.p), device=dy.device), stream=_stream())
+        dx, dw = torch.empty_like(dy), torch.empty(2, s.shape[1], device=dy.device)
+        p = kmb.norm_params(s, w, None, dx, stats=ctx.stats)   # the backward reads the sum, not what it was made of
+        g = kmb.norm_grads(p, dy, dx=dx, dw=dw[0], db=dw[1], dtotal=ds)
+        kmb.norm_backward(p, g, torch.empty(kmb.norm_workspace_floats(p), device=dy.device), stream=_stream())
         return dx, dx, dw[0], dw[1]
 
 
@@ -75,18 +79,20 @@ class GatedDelta(torch.autograd.Function):
         o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         hT = torch.empty(cu.numel() - 1, v.shape[2], k.shape[3], v.shape[3], device=v.device)
         g, beta = g.contiguous(), beta.contiguous()
-        ctx.p = kmb.delta_params(q, k, v, g, beta, o, scale=scale, hT=hT, cu_seqlens=cu)
-        ctx.ws = torch.empty(kmb.delta_workspace_floats(ctx.p, True), device=v.device)
-        kmb.delta_forward(ctx.p, ctx.ws, keep=True, stream=_stream())
+        p = kmb.delta_params(q, k, v, g, beta, o, scale=scale, hT=hT, cu_seqlens=cu)
+        ctx.ws, ctx.scale = torch.empty(kmb.delta_workspace_floats(p, True), device=v.device), scale
+        kmb.delta_forward(p, ctx.ws, keep=True, stream=_stream())
+        ctx.save_for_backward(q, k, v, g, beta, cu)
         ctx.mark_non_differentiable(hT)
         return o, hT
 
     @staticmethod
     def backward(ctx, do, _):
-        q, k, v, g, beta = ctx.p._keep[:5]
+        q, k, v, g, beta, cu = ctx.saved_tensors
         dq, dk, dv, dg, db = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta))
-        grads = kmb.delta_grads(ctx.p, do.contiguous(), dq, dk, dv, dg=dg, dbeta=db)
-        kmb.delta_backward(ctx.p, grads, ctx.ws, stream=_stream())
+        p = kmb.delta_params(q, k, v, g, beta, dv, scale=ctx.scale, cu_seqlens=cu)   # o is not read
+        grads = kmb.delta_grads(p, do.contiguous(), dq, dk, dv, dg=dg, dbeta=db)
+        kmb.delta_backward(p, grads, ctx.ws, stream=_stream())
         return dq, dk, dv, dg, db, None, None
 
 
