@@ -40,7 +40,7 @@ int kmb_grad_clip(const KMBGradTensor *tensors, long n_tensors, float max_norm, 
                   void *stream);
 /* The model's gradient arena in place, between kmb_model_forward_backward and
  * kmb_model_optimizer_step.  max_norm <= 0 takes MBOptimConfig.clip_norm of
- * kmamba_enable_training. */
+ * kmamba_enable_training; NaN is refused. */
 int kmb_model_clip_gradients(KMamba *m, float max_norm, float *result, float *ws, void *stream);
 
 #ifdef __cplusplus

@@ -16,12 +16,15 @@
  * neither read nor written.
  *
  * Accuracy: bf16 inputs are exact, every product is good to 2^-22 and every sum
- * fp32; bf16 results are rounded once.  Factors are scaled by blocks of 16 tokens
- * (or a quarter of dk) times 16 columns of dv: an entry below 2^-40 of its block's
- * largest counts as zero, and an infinity makes its block NaN.  A NaN at a token
- * reaches the tokens of its block of 16 before it as well as all behind.  Scale
- * keys so that beta |k|^2 <= 2 and g <= 0, as the rule itself needs to stay
- * bounded.
+ * fp32; bf16 results are rounded once, and o has the same bits with keep = 0 and 1.
+ * Factors are scaled by blocks of 16 tokens (or a quarter of dk) times 16 columns of
+ * dv, keys and queries by rows: an entry below 2^-40 of its block's largest counts
+ * as zero, and an infinity makes its block NaN.  A NaN at a token reaches the tokens
+ * of its block of 16 before it as well as all behind; one in do reaches the tokens of
+ * its block behind it as well as all before.  dg is a running sum over a chunk of 64
+ * tokens: its error is relative to the chunk's largest, and a NaN in do makes the
+ * chunk's dg NaN.  Scale keys so that beta |k|^2 <= 2 and g <= 0, as the rule itself
+ * needs to stay bounded.
  *
  * Calls only enqueue work on `stream` (NULL = default), allocate nothing (but for
  * the device status word in a host thread's first call), keep nothing between
@@ -50,7 +53,8 @@ typedef struct {
     const int *cu_seqlens;      /* device [n_seq + 1], or NULL */
     long n_seq;                 /* with cu_seqlens */
     const void *q, *k, *v;
-    const float *g;             /* log decay, NULL = 0; -INFINITY forgets the state */
+    const float *g;             /* log decay, NULL = 0; -INFINITY forgets the state; at a sequence's first token, and at
+                                   any token of kmb_delta_step, also a state that holds infinities or NaN */
     const float *beta;          /* NULL = 1 */
     void *o;
     const float *h0;            /* initial states, NULL = 0 */
